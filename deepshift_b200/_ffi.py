@@ -48,8 +48,22 @@ class StagedOut(ctypes.Structure):
     ]
 
 
+class Adapters(ctypes.Structure):
+    """Mirror of ``ds_adapters_t``."""
+    _fields_ = [
+        ("rows", ctypes.c_int), ("k", ctypes.c_int), ("n", ctypes.c_int), ("rank", ctypes.c_int), ("count", ctypes.c_int),
+        ("act_type", ctypes.c_int), ("weight_type", ctypes.c_int), ("plan", ctypes.c_void_p),
+        ("down", ctypes.c_void_p), ("up", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_longlong), ("base", ctypes.c_void_p), ("base_stride", ctypes.c_longlong),
+        ("out", ctypes.c_void_p), ("out_stride", ctypes.c_longlong), ("h", ctypes.c_void_p), ("h_bytes", ctypes.c_longlong),
+        ("grad", ctypes.c_void_p), ("grad_stride", ctypes.c_longlong), ("dx", ctypes.c_void_p), ("dx_stride", ctypes.c_longlong),
+        ("ddown", ctypes.c_void_p), ("dup", ctypes.c_void_p), ("dh", ctypes.c_void_p), ("dh_bytes", ctypes.c_longlong),
+    ]
+
+
 IN_I32, IN_F32_CONV, IN_F32_LINEAR, IN_I32_CLAMP = 0, 1, 2, 3
 OUT_I32, OUT_F32 = 0, 1
+T_F32, T_BF16, T_F16 = 0, 1, 2
 
 _VP, _I, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 _SIGNATURES = {
@@ -92,6 +106,10 @@ _SIGNATURES = {
     "ds_staged_prepare": [_VP, _I, _I, _I, _I, _I, _I, _VP, _LL, ctypes.POINTER(ctypes.c_longlong), _VP],
     "ds_staged_conv2d": [ctypes.POINTER(Staged), _VP, _LL, _VP] + [_I] * 7 + [ctypes.POINTER(StagedOut), _VP, _LL, _VP],
     "ds_maxpool_nhwc": [_VP] + [_I] * 7 + [_VP, ctypes.POINTER(Staged), _I, _I, _VP],
+    "ds_rows_plan": [_VP, _I, _I, _VP, _LL, _VP],
+    "ds_adapters_apply": [ctypes.POINTER(Adapters), _VP],
+    "ds_adapters_backward": [ctypes.POINTER(Adapters), _VP],
+    "ds_clip_norm": [_VP, _I, ctypes.c_float, _VP, _VP, _LL, _VP],
     "ds_avgpool_fix_nhwc": [_VP, _VP, _I, _I, _I, _I, _I, _VP],
 }
 
@@ -123,6 +141,9 @@ def lib():
         l.ds_launch_count.restype = ctypes.c_longlong
         l.ds_planes_bytes.argtypes = [_I] * 5
         l.ds_planes_bytes.restype = ctypes.c_longlong
+        for name, n in (("ds_rows_plan_bytes", 2), ("ds_adapters_h_bytes", 6), ("ds_clip_bytes", 1)):
+            getattr(l, name).argtypes = [_I] * n
+            getattr(l, name).restype = ctypes.c_longlong
         l.ds_staged_bytes.argtypes = [_I] * 5
         l.ds_staged_bytes.restype = ctypes.c_longlong
         _lib = l

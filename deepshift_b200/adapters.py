@@ -1,0 +1,255 @@
+"""Low-rank adapters of many requests beside a shared projection.
+
+A packed shift layer cannot be trained; what adapts it is a pair of small matrices beside it,
+
+    y[m] = base[m] + scale[a] * up[a]^T (down[a] x[m]),     a = the adapter of row m,
+
+one pair for each task or request.  ``apply`` adds the adapters of all rows of a batch to the projection's output in two
+kernels, whichever rows use whichever adapters: one token of each of many requests, prompts one behind another, or any
+mixture; rows of index -1 have none.  It is differentiable in ``x``, ``down``, ``up`` and ``base``.  ``AdaptedLinear`` puts a
+set of adapters beside a layer.
+
+Rows are sorted by adapter once a batch (``plan_rows``), on the GPU and without a synchronisation, and the plan serves every
+layer and both directions.  All calls run on torch's current stream of their tensors' device; scratch comes from torch's
+allocator.  No counterpart in the reference.
+"""
+import functools
+import math
+
+import torch
+import torch.nn as nn
+
+from . import _ffi
+from .kernels import _stream_ptr
+
+TYPES = {torch.float32: _ffi.T_F32, torch.bfloat16: _ffi.T_BF16, torch.float16: _ffi.T_F16}
+
+MAX_RANK, MAX_COUNT, MAX_ROWS, MAX_WIDTH = 256, 65535, 1 << 24, 1 << 20
+
+
+class RowPlan:
+    """The rows of a batch sorted by adapter.  ``rows`` and ``count`` are those it was made for."""
+    __slots__ = ("rows", "count", "data", "device")
+
+    def __init__(self, rows, count, data):
+        self.rows, self.count, self.data, self.device = rows, count, data, data.device
+
+    def invalid(self):
+        """How many rows had an index outside -1 .. count - 1 (they count as rows without an adapter).  Synchronises."""
+        return int(self.data[1])
+
+
+def plan_rows(ids, count, device=None):
+    """The plan of a batch whose row m uses adapter ``ids[m]`` of ``count`` (-1: none).
+
+    ``ids``: a one-dimensional integer tensor, or a list.  Values on the host are checked here; those on the GPU are not read
+    by the host (see ``RowPlan.invalid``)."""
+    count = int(count)
+    if not 1 <= count <= MAX_COUNT:
+        raise RuntimeError("count must be in 1 .. %d, got %d" % (MAX_COUNT, count))
+    if not isinstance(ids, torch.Tensor):
+        ids = torch.tensor(ids, dtype=torch.int64).reshape(-1)
+    if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("ids must be a one-dimensional int32 or int64 tensor, got %s of %s" % (ids.dtype, tuple(ids.shape)))
+    if ids.numel() > MAX_ROWS:
+        raise RuntimeError("at most %d rows a plan, got %d" % (MAX_ROWS, ids.numel()))
+    if not ids.is_cuda:
+        if ids.numel() and (int(ids.min()) < -1 or int(ids.max()) >= count):
+            raise RuntimeError("ids must be in -1 .. %d" % (count - 1))
+        ids = ids.to(device if device is not None else "cuda")
+    # an int64 index outside 32 bits stays outside
+    ids = (ids if ids.dtype == torch.int32 else ids.clamp(-2, MAX_COUNT).to(torch.int32)).contiguous()
+    n = _ffi.lib().ds_rows_plan_bytes(ids.numel(), count)
+    data = torch.empty(n // 4, dtype=torch.int32, device=ids.device)
+    with torch.cuda.device(ids.device):
+        _ffi.check(_ffi.lib().ds_rows_plan(ids.data_ptr(), ids.numel(), count, data.data_ptr(), n, _stream_ptr(ids.device)), "plan_rows")
+    return RowPlan(ids.numel(), count, data)
+
+
+@functools.lru_cache(maxsize=4096)
+def _h_bytes(rows, width, rank, count, act, weight):
+    return _ffi.lib().ds_adapters_h_bytes(rows, width, rank, count, act, weight)
+
+
+def _rows(t, name, width, like):
+    """A tensor as [rows, width] with consecutive elements in a row: itself where it is one, or its leading dimensions folded."""
+    if t.dim() < 1 or t.size(-1) != width:
+        raise RuntimeError("%s must have %d elements a row, got %s" % (name, width, tuple(t.shape)))
+    if t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError("%s must be %s on %s, got %s on %s" % (name, like.dtype, like.device, t.dtype, t.device))
+    if t.dim() != 2:
+        if not t.is_contiguous():
+            raise RuntimeError("%s must be contiguous, or two-dimensional" % name)
+        t = t.view(-1, width)
+    if width > 1 and t.stride(1) != 1:
+        raise RuntimeError("the elements of a row of %s must be contiguous" % name)
+    return t
+
+
+def _check(x, down, up, scale, plan):
+    if not x.is_cuda:
+        raise RuntimeError("x must be a CUDA tensor")
+    if x.dtype not in TYPES or down.dtype not in TYPES:
+        raise RuntimeError("x and the adapters must be float32, bfloat16 or float16, got %s and %s" % (x.dtype, down.dtype))
+    if x.dtype != down.dtype and torch.float32 not in (x.dtype, down.dtype):
+        raise RuntimeError("x is %s and the adapters %s: one of two types has to be float32" % (x.dtype, down.dtype))
+    for t, name in ((down, "down"), (up, "up")):
+        if t.dim() != 3 or not t.is_contiguous():
+            raise RuntimeError("%s must be contiguous, [count, rank, width]" % name)
+        if t.device != x.device or t.dtype != down.dtype:
+            raise RuntimeError("down and up must be of one type, on the device of x")
+    count, rank, k = down.shape
+    if up.shape[:2] != down.shape[:2]:
+        raise RuntimeError("down is %s and up %s: count and rank must agree" % (tuple(down.shape), tuple(up.shape)))
+    n = up.shape[2]
+    if not 1 <= rank <= MAX_RANK or not 1 <= k <= MAX_WIDTH or not 1 <= n <= MAX_WIDTH:
+        raise RuntimeError("ranks are 1 .. %d and widths 1 .. %d, got %d, %d and %d" % (MAX_RANK, MAX_WIDTH, rank, k, n))
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (count,) or not scale.is_contiguous() or
+                              scale.device != x.device):
+        raise RuntimeError("scale must be float32 [%d], contiguous, on the device of x" % count)
+    if plan.count != count or plan.device != x.device:
+        raise RuntimeError("the plan is for %d adapters on %s, not for %d on %s" % (plan.count, plan.device, count, x.device))
+    return count, rank, k, n
+
+
+def _struct(plan, down, up, scale, rank, k, n, act, weight):
+    a = _ffi.Adapters()
+    a.rows, a.k, a.n, a.rank, a.count = plan.rows, k, n, rank, plan.count
+    a.act_type, a.weight_type = act, weight
+    a.plan, a.down, a.up = plan.data.data_ptr(), down.data_ptr(), up.data_ptr()
+    a.scale = scale.data_ptr() if scale is not None else None
+    return a
+
+
+def _forward(x, down, up, scale, plan, base, out):
+    count, rank, k, n = _check(x, down, up, scale, plan)
+    shape = x.shape[:-1] + (n,)
+    rows = _rows(x, "x", k, x)
+    if rows.size(0) != plan.rows:
+        raise RuntimeError("x has %d rows, the plan is for %d" % (rows.size(0), plan.rows))
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape:
+        raise RuntimeError("out must be %s, got %s" % (tuple(shape), tuple(out.shape)))
+    to = _rows(out, "out", n, x)
+    act, weight = TYPES[x.dtype], TYPES[down.dtype]
+    a = _struct(plan, down, up, scale, rank, k, n, act, weight)
+    a.x, a.x_stride, a.out, a.out_stride = rows.data_ptr(), rows.stride(0), to.data_ptr(), to.stride(0)
+    if base is not None:
+        if base.shape != shape:
+            raise RuntimeError("base must be %s, got %s" % (tuple(shape), tuple(base.shape)))
+        add = _rows(base, "base", n, x)
+        if add.data_ptr() == to.data_ptr() and add.stride(0) != to.stride(0):
+            raise RuntimeError("base and out overlap")
+        a.base, a.base_stride = add.data_ptr(), add.stride(0)
+    nbytes = _h_bytes(plan.rows, k, rank, count, act, weight)
+    h = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
+    a.h, a.h_bytes = h.data_ptr(), nbytes
+    with torch.cuda.device(x.device):
+        _ffi.check(_ffi.lib().ds_adapters_apply(a, _stream_ptr(x.device)), "adapters.apply")
+    return out, h
+
+
+class _Apply(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, down, up, scale, plan, base):
+        out, h = _forward(x, down, up, scale, plan, base, None)
+        ctx.save_for_backward(x, down, up, scale, h)
+        ctx.plan = plan
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, down, up, scale, h = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if not any(need[:3]):
+            return None, None, None, None, None, grad if need[5] else None
+        plan, (count, rank, k), n = ctx.plan, down.shape, up.shape[2]
+        rows = _rows(x, "x", k, x)
+        g = grad.reshape(-1, n)
+        if n > 1 and g.stride(1) != 1:
+            g = g.contiguous()
+        act, weight = TYPES[x.dtype], TYPES[down.dtype]
+        a = _struct(plan, down, up, scale, rank, k, n, act, weight)
+        a.x, a.x_stride, a.grad, a.grad_stride = rows.data_ptr(), rows.stride(0), g.data_ptr(), g.stride(0)
+        dx = ddown = dup = None
+        if need[0]:
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            a.dx, a.dx_stride = dx.data_ptr(), k
+        if need[1]:
+            ddown = torch.empty_like(down)
+            a.ddown = ddown.data_ptr()
+        if need[2]:
+            dup = torch.empty_like(up)
+            a.dup = dup.data_ptr()
+        a.h, a.h_bytes = h.data_ptr(), 4 * h.numel()
+        nbytes = _h_bytes(plan.rows, n, rank, count, act, weight)
+        dh = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
+        a.dh, a.dh_bytes = dh.data_ptr(), nbytes
+        with torch.cuda.device(x.device):
+            _ffi.check(_ffi.lib().ds_adapters_backward(a, _stream_ptr(x.device)), "adapters.apply (backward)")
+        return dx, ddown, dup, None, None, grad if need[5] else None
+
+
+def apply(x, down, up, scale, plan, base=None, out=None):
+    """``base + scale[a] * up[a]^T (down[a] x)`` for every row of ``x`` and its adapter a; ``base`` alone where a row has none.
+
+    ``x`` [..., K], ``base`` [..., N] and the result share one type (float32, bfloat16 or float16); ``down`` [count, rank, K] and
+    ``up`` [count, rank, N] another (float32 goes with any, two 16-bit types have to be the same); ``scale`` float32 [count], or
+    None for 1.  Two-dimensional ``x``, ``base`` and ``out`` may have any distance between rows.  ``out`` may be ``base`` itself.
+    Products are exact to 21 bits at least and sums are fp32, whatever the types; the result is rounded once.
+    Differentiable in ``x``, ``down``, ``up`` and ``base`` (not in ``scale``), unless ``out`` is given."""
+    if torch.is_grad_enabled() and (x.requires_grad or down.requires_grad or up.requires_grad or
+                                    (base is not None and base.requires_grad)):
+        if out is not None:
+            raise RuntimeError("out= cannot be differentiated")
+        return _Apply.apply(x, down, up, scale, plan, base)
+    return _forward(x, down, up, scale, plan, base, out)[0]
+
+
+class AdaptedLinear(nn.Module):
+    """``count`` low-rank adapters beside ``base``, a linear layer that stays as it is (a ``LinearShift`` with packed weights, or
+    any module of ``in_features`` -> ``out_features``).  ``up`` starts at zero: at first the layer computes what ``base`` does.
+
+    ``forward(x, plan)`` adds the adapter of each row (``plan_rows``) to the layer's output.  The gradient of ``x`` is the
+    adapters' and the layer's own; a shift layer's goes through its weights as powers of two."""
+
+    def __init__(self, base, count, rank, alpha=None, in_features=None, out_features=None, dtype=torch.float32, device=None):
+        super().__init__()
+        self.base = base
+        for p in base.parameters():
+            p.requires_grad_(False)
+        self.in_features = in_features if in_features is not None else base.in_features
+        self.out_features = out_features if out_features is not None else base.out_features
+        self.count, self.rank = int(count), int(rank)
+        self.down = nn.Parameter(torch.empty(count, rank, self.in_features, dtype=dtype, device=device))
+        self.up = nn.Parameter(torch.zeros(count, rank, self.out_features, dtype=dtype, device=device))
+        nn.init.normal_(self.down, std=1 / math.sqrt(self.in_features))
+        self.register_buffer("scale", torch.full((count,), float(alpha if alpha is not None else rank) / rank, device=device))
+
+    def forward(self, x, plan):
+        if torch.is_grad_enabled() and x.requires_grad and hasattr(self.base, "_float_weight"):
+            shared = _Frozen.apply(x, self.base)
+        else:
+            with torch.set_grad_enabled(torch.is_grad_enabled() and x.requires_grad):
+                shared = self.base(x)
+        return apply(x, self.down, self.up, self.scale, plan, base=shared.to(x.dtype))
+
+    def extra_repr(self):
+        return 'count={}, rank={}'.format(self.count, self.rank)
+
+
+class _Frozen(torch.autograd.Function):
+    """A frozen shift layer in a graph: its packed kernel forward, and its weights as the powers of two that they are backward.
+    The quantisation of the input passes the gradient on as it is (straight through)."""
+
+    @staticmethod
+    def forward(ctx, x, layer):
+        ctx.layer, ctx.dtype = layer, x.dtype
+        return layer(x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return (grad.float() @ ctx.layer._float_weight().float()).to(ctx.dtype), None

@@ -1,0 +1,354 @@
+// Low-rank adapters beside a shared projection: the plan of rows, and the entry points (kernels in ds_adapters.cuh).
+#include "ds_adapters.cuh"
+
+#include <type_traits>
+
+namespace ds {
+namespace adapters {
+namespace {
+
+constexpr int PLAN_THREADS = 1024, PLAN_WARPS = 32;
+
+__device__ __forceinline__ int row_key(const int* __restrict__ ids, int m, int count)
+{
+    const int a = ids[m];
+    return a >= 0 && a < count ? a : count;
+}
+
+// Exclusive scan of one value a thread over the CTA, and the total.
+__device__ int cta_scan(int v, int& total)
+{
+    __shared__ int sums[PLAN_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int s = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+        if (lane >= d) s += o;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int i = 0; i < PLAN_WARPS; ++i) {
+        if (i < warp) before += sums[i];
+        total += sums[i];
+    }
+    return before + s - v;
+}
+
+// Rows sorted by adapter, each adapter's in their own order (a stable counting sort, eight bits of the index a pass), and cut
+// into tiles of one adapter.  One CTA: 8192 rows are 8 steps a warp and pass, and a batch needs one plan for all its layers.
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* __restrict__ ids, int rows, int count, int* plan, int* spare,
+                                                            int passes, int tile_rows)
+{
+    __shared__ int counter[PLAN_WARPS][256];
+    __shared__ int invalid;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int* offsets = plan + PLAN_HEAD;
+    int4* tiles = reinterpret_cast<int4*>(plan + plan_tiles_at(count));
+    int* order = plan + plan_order_at(rows, count);
+    int* first_tile = spare + rows;
+    if (threadIdx.x == 0) invalid = 0;
+    const int part = ((rows + PLAN_WARPS - 1) / PLAN_WARPS + 31) / 32 * 32;   // rows of a warp, a multiple of 32
+    const int begin = min(rows, warp * part), end = min(rows, begin + part);
+    for (int pass = 0; pass < passes; ++pass) {
+        int* to = (passes - pass) & 1 ? order : spare;
+        const int* from = (passes - pass) & 1 ? spare : order;
+        for (int i = threadIdx.x; i < PLAN_WARPS * 256; i += PLAN_THREADS) counter[0][i] = 0;
+        __syncthreads();
+        for (int base = begin; base < end; base += 32) {
+            const int i = base + lane;
+            const unsigned live = __ballot_sync(0xFFFFFFFFu, i < end);
+            if (i < end) {
+                const int m = pass ? from[i] : i, key = row_key(ids, m, count), digit = key >> (8 * pass) & 255;
+                const unsigned same = __match_any_sync(live, digit);
+                if (lane == __ffs(same) - 1) counter[warp][digit] += __popc(same);
+                if (pass == 0 && key == count && ids[m] != -1) atomicAdd(&invalid, 1);
+            }
+            __syncwarp();
+        }
+        __syncthreads();
+        int total = 0, all;
+        if (threadIdx.x < 256)
+            for (int w = 0; w < PLAN_WARPS; ++w) total += counter[w][threadIdx.x];
+        int at = cta_scan(total, all);
+        if (threadIdx.x < 256)
+            for (int w = 0; w < PLAN_WARPS; ++w) {
+                const int n = counter[w][threadIdx.x];
+                counter[w][threadIdx.x] = at;
+                at += n;
+            }
+        __syncthreads();
+        for (int base = begin; base < end; base += 32) {
+            const int i = base + lane;
+            const unsigned live = __ballot_sync(0xFFFFFFFFu, i < end);
+            if (i < end) {
+                const int m = pass ? from[i] : i, digit = row_key(ids, m, count) >> (8 * pass) & 255;
+                const unsigned same = __match_any_sync(live, digit);
+                const int start = counter[warp][digit];
+                __syncwarp(live);
+                to[start + __popc(same & ((1u << lane) - 1))] = m;
+                if (lane == __ffs(same) - 1) counter[warp][digit] = start + __popc(same);
+            }
+            __syncwarp();
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i <= rows; i += PLAN_THREADS) {
+        const int before = i ? row_key(ids, order[i - 1], count) : -1, here = i < rows ? row_key(ids, order[i], count) : count + 1;
+        for (int a = before + 1; a <= here; ++a) offsets[a] = i;
+    }
+    __syncthreads();
+    int tiles_before = 0;
+    for (int base = 0; base <= count; base += PLAN_THREADS) {
+        const int a = base + threadIdx.x;
+        const int n = a <= count ? (offsets[a + 1] - offsets[a] + tile_rows - 1) / tile_rows : 0;
+        int all;
+        const int at = cta_scan(n, all);
+        if (a <= count) first_tile[a] = tiles_before + at;
+        tiles_before += all;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows; i += PLAN_THREADS) {
+        const int a = row_key(ids, order[i], count), in = i - offsets[a];
+        if (in % tile_rows == 0) tiles[first_tile[a] + in / tile_rows] = make_int4(a, i, min(tile_rows, offsets[a + 1] - i), 0);
+    }
+    if (threadIdx.x == 0) {
+        plan[0] = tiles_before;
+        plan[1] = invalid;
+    }
+}
+
+int passes_of(int count)
+{
+    int passes = 1;
+    while (passes < 4 && count >> (8 * passes)) ++passes;
+    return passes;
+}
+
+// ---- launches ----
+bool aligned(const void* p, long long stride, int type)
+{
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * (type == DS_T_F32 ? 4 : 2) % 16 == 0;
+}
+
+// CTAs a tile's sums are shared by: until there are two for each SM, as long as every warp keeps a piece of its own.
+int splits_of(int rows, int width, int rank, int count, bool same16)
+{
+    const long long tiles = plan_tiles(rows, count) * ((rank + 63) / 64);
+    const int pieces = (width + (same16 ? 31 : 15)) / (same16 ? 32 : 16) / WARPS;
+    long long s = 296 / (tiles < 1 ? 1 : tiles);   // no rows, no tiles
+    if (s > pieces) s = pieces;
+    return s < 1 ? 1 : s > 16 ? 16 : int(s);
+}
+
+int finish()
+{
+    note_launch();
+    return cudaGetLastError() == cudaSuccess ? DS_OK : DS_ERR_CUDA;
+}
+
+// More than 48 KB of shared memory has to be allowed for each kernel, once a device.
+template <auto KERNEL>
+bool allow_smem(int bytes)
+{
+    if (bytes <= 48 * 1024) return true;
+    static bool done[kMaxDevices];
+    const int dev = device_slot();
+    if (dev >= 0 && done[dev]) return true;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    if (dev >= 0) done[dev] = true;
+    return true;
+}
+
+template <class X, class W, int MT, int NT, bool VEC>
+int launch_down(const Args& a, cudaStream_t st)
+{
+    const int smem = WARPS * 16 * MT * 8 * NT * 4;
+    static_assert(WARPS * 16 * MT * 8 * NT * 4 <= 65536, "shared memory of the sums");
+    if (!allow_smem<down_kernel<X, W, MT, NT, VEC>>(smem)) return DS_ERR_CUDA;
+    const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), a.splits, (a.rank8 + 8 * NT - 1) / (8 * NT));
+    down_kernel<X, W, MT, NT, VEC><<<grid, THREADS, smem, st>>>(a);
+    return finish();
+}
+
+template <class X, class W>
+int down(const Args& a, bool vec, cudaStream_t st)
+{
+    const bool wide = plan_tile_rows(a.rows) == 32;
+    if (!vec) return wide ? launch_down<X, W, 2, 8, false>(a, st) : launch_down<X, W, 1, 8, false>(a, st);
+    if (a.rank8 <= 8) return wide ? launch_down<X, W, 2, 1, true>(a, st) : launch_down<X, W, 1, 1, true>(a, st);
+    if (a.rank8 <= 16) return wide ? launch_down<X, W, 2, 2, true>(a, st) : launch_down<X, W, 1, 2, true>(a, st);
+    if (a.rank8 <= 32) return wide ? launch_down<X, W, 2, 4, true>(a, st) : launch_down<X, W, 1, 4, true>(a, st);
+    return wide ? launch_down<X, W, 2, 8, true>(a, st) : launch_down<X, W, 1, 8, true>(a, st);
+}
+
+template <class X, class W, int MT>
+int launch_up(const Args& a, bool vec, cudaStream_t st)
+{
+    const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS));
+    if (vec) up_kernel<X, W, MT, true><<<grid, THREADS, 0, st>>>(a);
+    else up_kernel<X, W, MT, false><<<grid, THREADS, 0, st>>>(a);
+    return finish();
+}
+
+template <class X, class W>
+int up(const Args& a, bool vec, cudaStream_t st)
+{
+    return plan_tile_rows(a.rows) == 32 ? launch_up<X, W, 2>(a, vec, st) : launch_up<X, W, 1>(a, vec, st);
+}
+
+template <class X, class W, int RT, int NJ, bool VEC>
+int launch_grad(const Args& a, cudaStream_t st)
+{
+    const int smem = WARPS * 16 * RT * 8 * NJ * 4;
+    if (!allow_smem<grad_kernel<X, W, RT, NJ, VEC>>(smem)) return DS_ERR_CUDA;
+    const dim3 grid((a.width + 8 * NJ - 1) / (8 * NJ), a.count, (a.rank + 16 * RT - 1) / (16 * RT));
+    grad_kernel<X, W, RT, NJ, VEC><<<grid, THREADS, smem, st>>>(a);
+    return finish();
+}
+
+template <class X, class W>
+int grad(const Args& a, bool vec, cudaStream_t st)
+{
+    constexpr int NJ = is_f32<X> ? 4 : 8;
+    if (!vec) return launch_grad<X, W, 2, NJ, false>(a, st);
+    return a.rank <= 16 ? launch_grad<X, W, 1, NJ, true>(a, st) : launch_grad<X, W, 2, NJ, true>(a, st);
+}
+
+// Calls f(X{}, W{}) with the types of a call.
+template <class F>
+int by_type(int act, int weight, F f)
+{
+    if (act == DS_T_F32) {
+        if (weight == DS_T_F32) return f(float{}, float{});
+        if (weight == DS_T_BF16) return f(float{}, bf16{});
+        if (weight == DS_T_F16) return f(float{}, f16{});
+    } else if (act == DS_T_BF16) {
+        if (weight == DS_T_F32) return f(bf16{}, float{});
+        if (weight == DS_T_BF16) return f(bf16{}, bf16{});
+    } else if (act == DS_T_F16) {
+        if (weight == DS_T_F32) return f(f16{}, float{});
+        if (weight == DS_T_F16) return f(f16{}, f16{});
+    }
+    return DS_ERR_UNSUPPORTED;
+}
+
+int rank8(int rank) { return (rank + 7) / 8 * 8; }
+
+int check(const ds_adapters_t* a, bool backward)
+{
+    if (!a || a->rows < 0 || a->k < 1 || a->n < 1 || a->rank < 1 || a->count < 1) return DS_ERR_BAD_ARG;
+    if (a->rank > 256 || a->count > 65535) return DS_ERR_UNSUPPORTED;
+    if (a->rows > 1 << 24 || a->k > 1 << 20 || a->n > 1 << 20) return DS_ERR_RANGE;
+    if (!a->plan || !a->down || !a->up) return DS_ERR_BAD_ARG;
+    if (a->rows && (!a->x || !a->h)) return DS_ERR_BAD_ARG;
+    if (backward ? (a->rows && (!a->grad || !a->dh)) : (a->rows && !a->out)) return DS_ERR_BAD_ARG;
+    if (reinterpret_cast<uintptr_t>(a->plan) & 15 || reinterpret_cast<uintptr_t>(a->h) & 15 || reinterpret_cast<uintptr_t>(a->dh) & 15)
+        return DS_ERR_ALIGN;
+    if (a->h_bytes < ds_adapters_h_bytes(a->rows, a->k, a->rank, a->count, a->act_type, a->weight_type)) return DS_ERR_SCRATCH;
+    if (backward && a->dh_bytes < ds_adapters_h_bytes(a->rows, a->n, a->rank, a->count, a->act_type, a->weight_type)) return DS_ERR_SCRATCH;
+    return DS_OK;
+}
+
+Args common(const ds_adapters_t* a)
+{
+    Args p = {};
+    p.plan = plan_view(a->plan, a->rows, a->count);
+    p.scale = a->scale;
+    p.rows = a->rows, p.rank = a->rank, p.rank8 = rank8(a->rank), p.count = a->count;
+    return p;
+}
+
+// h = x down^T: a call of down_kernel on activations `x` [rows][width] and matrices `w`.
+Args down_args(const ds_adapters_t* a, const void* x, long long ldx, const void* w, int width, float* h)
+{
+    Args p = common(a);
+    p.x = x, p.ldx = ldx, p.w = w, p.width = width, p.h = h;
+    p.splits = splits_of(a->rows, width, a->rank, a->count, a->act_type != DS_T_F32 && a->act_type == a->weight_type);
+    return p;
+}
+
+}  // namespace
+}  // namespace adapters
+}  // namespace ds
+
+extern "C" long long ds_rows_plan_bytes(int rows, int count)
+{
+    if (rows < 0 || count < 1 || rows > 1 << 24 || count > 65535) return -1;
+    return (ds::adapters::plan_order_at(rows, count) + 2ll * rows + count + 2) * 4;
+}
+
+extern "C" int ds_rows_plan(const int32_t* ids, int rows, int count, int32_t* plan, long long plan_bytes, void* stream)
+{
+    using namespace ds::adapters;
+    if (rows < 0 || count < 1 || (rows && !ids) || !plan) return DS_ERR_BAD_ARG;
+    const long long need = ds_rows_plan_bytes(rows, count);
+    if (need < 0) return DS_ERR_RANGE;
+    if (plan_bytes < need) return DS_ERR_SCRATCH;
+    if (reinterpret_cast<uintptr_t>(plan) & 15) return DS_ERR_ALIGN;
+    plan_kernel<<<1, PLAN_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(ids, rows, count, plan, plan + plan_order_at(rows, count) + rows,
+                                                                           passes_of(count), plan_tile_rows(rows));
+    return finish();
+}
+
+extern "C" long long ds_adapters_h_bytes(int rows, int width, int rank, int count, int act_type, int weight_type)
+{
+    using namespace ds::adapters;
+    if (rows < 0 || width < 1 || rank < 1 || count < 1) return -1;
+    return (long long)splits_of(rows, width, rank, count, act_type != DS_T_F32 && act_type == weight_type) * rows * rank8(rank) * 4;
+}
+
+extern "C" int ds_adapters_apply(const ds_adapters_t* a, void* stream)
+{
+    using namespace ds::adapters;
+    if (const int e = check(a, false)) return e;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return by_type(a->act_type, a->weight_type, [&](auto x, auto w) {
+        using X = decltype(x);
+        using W = decltype(w);
+        if (a->rows == 0) return int(DS_OK);
+        Args p = down_args(a, a->x, a->x_stride, a->down, a->k, a->h);
+        if (const int e = down<X, W>(p, a->k % 8 == 0 && aligned(a->x, a->x_stride, a->act_type) && aligned(a->down, a->k, a->weight_type), st))
+            return e;
+        p.w = a->up, p.width = a->n;
+        p.base = a->base, p.ldbase = a->base_stride, p.out = a->out, p.ldout = a->out_stride;
+        const bool vec = a->n % 8 == 0 && aligned(a->up, a->n, a->weight_type) && aligned(a->out, a->out_stride, a->act_type) &&
+                         (!a->base || aligned(a->base, a->base_stride, a->act_type));
+        return up<X, W>(p, vec, st);
+    });
+}
+
+extern "C" int ds_adapters_backward(const ds_adapters_t* a, void* stream)
+{
+    using namespace ds::adapters;
+    if (const int e = check(a, true)) return e;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return by_type(a->act_type, a->weight_type, [&](auto x, auto w) {
+        using X = decltype(x);
+        using W = decltype(w);
+        const bool vec_k = a->k % 8 == 0 && aligned(a->x, a->x_stride, a->act_type) && aligned(a->down, a->k, a->weight_type);
+        const bool vec_n = a->n % 8 == 0 && aligned(a->grad, a->grad_stride, a->act_type) && aligned(a->up, a->n, a->weight_type);
+        const Args dh = down_args(a, a->grad, a->grad_stride, a->up, a->n, a->dh);
+        if ((a->dx || a->ddown) && a->rows)
+            if (const int e = down<X, W>(dh, vec_n, st)) return e;
+        if (a->dx && a->rows) {
+            Args p = dh;
+            p.w = a->down, p.width = a->k, p.out = a->dx, p.ldout = a->dx_stride;
+            if (const int e = up<X, W>(p, vec_k && aligned(a->dx, a->dx_stride, a->act_type), st)) return e;
+        }
+        if (a->ddown) {
+            Args p = dh;
+            p.x = a->x, p.ldx = a->x_stride, p.width = a->k, p.out = a->ddown;
+            if (const int e = grad<X, W>(p, vec_k && aligned(a->ddown, a->k, a->weight_type), st)) return e;
+        }
+        if (a->dup) {
+            Args p = down_args(a, a->grad, a->grad_stride, nullptr, a->k, a->h);   // the forward's h, its splits those of k
+            p.width = a->n, p.out = a->dup;
+            if (const int e = grad<X, W>(p, vec_n && aligned(a->dup, a->n, a->weight_type), st)) return e;
+        }
+        return int(DS_OK);
+    });
+}

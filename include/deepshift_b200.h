@@ -434,6 +434,66 @@ int ds_unopt_linear_f32(const float *x, const float *weight, const float *bias, 
 int ds_unopt_conv2d_f32(const float *x, const float *weight, const float *bias, float *out, int B, int C,
                         int H, int W, int OC, int KH, int KW, int sh, int sw, int ph, int pw, void *stream);
 
+/* Element types of the operators below. */
+typedef enum { DS_T_F32 = 0, DS_T_BF16 = 1, DS_T_F16 = 2 } ds_type;
+
+/*
+ * Low-rank adapters of many requests beside a shared projection (no counterpart in the reference):
+ *     h[m] = down[a] x[m],   out[m] = base[m] + scale[a] * up[a]^T h[m],   a = adapter of row m
+ * Rows without an adapter get out = base (0 without base).  Both matrices of an adapter lie by rank: down is
+ * [count][rank][k], up is [count][rank][n].  Activations (x, base, out, their gradients) share one type, the
+ * adapters another; fp32 goes with any, two 16-bit types have to be the same.  Sums are fp32 in any case.
+ *
+ * ds_rows_plan sorts the rows of a batch by adapter: ids [rows] on the device, -1 = none (an index outside
+ * -1 .. count - 1 counts as none too; plan[1] says how many there were).  One plan serves every layer and
+ * direction of the batch.  Up to 2^24 rows, 65535 adapters, a rank of 256, rows of 2^20 elements.
+ */
+typedef struct {
+    int rows, k, n, rank, count;
+    int act_type, weight_type;         /* ds_type                                                          */
+    const int32_t *plan;               /* of ds_rows_plan, for these rows and this count                   */
+    const void *down, *up;             /* [count][rank][k], [count][rank][n]                               */
+    const float *scale;                /* [count]; NULL = 1                                                */
+    const void *x;                     /* [rows][k], rows x_stride elements apart                          */
+    long long x_stride;
+    const void *base;                  /* [rows][n] or NULL; may be out itself                             */
+    long long base_stride;
+    void *out;                         /* [rows][n]                                                        */
+    long long out_stride;
+    float *h;                          /* ds_adapters_h_bytes(rows, k, ...): written by _apply, read by _backward */
+    long long h_bytes;
+    const void *grad;                  /* _backward only: gradient of out [rows][n]                        */
+    long long grad_stride;
+    void *dx;                          /* [rows][k] or NULL                                                */
+    long long dx_stride;
+    void *ddown, *dup;                 /* gradients of down and up, whole, in weight_type, or NULL         */
+    float *dh;                         /* ds_adapters_h_bytes(rows, n, ...)                                */
+    long long dh_bytes;
+} ds_adapters_t;
+
+long long ds_rows_plan_bytes(int rows, int count);
+int ds_rows_plan(const int32_t *ids, int rows, int count, int32_t *plan, long long plan_bytes, void *stream);
+long long ds_adapters_h_bytes(int rows, int width, int rank, int count, int act_type, int weight_type);
+int ds_adapters_apply(const ds_adapters_t *a, void *stream);
+int ds_adapters_backward(const ds_adapters_t *a, void *stream);
+
+/*
+ * Global norm of many tensors and their scaling (no counterpart in the reference):
+ *     *norm = sqrt(sum of all src^2),  dst = src * min(1, max_norm / (*norm + 1e-6))
+ * `tensors` is read on the host before the call returns; dst may be src; dst NULL in all of them = only the norm.
+ * norm lies on the device; scratch holds ds_clip_bytes(count).  The same call gives the same bits each time.
+ */
+typedef struct {
+    const void *src;
+    void *dst;
+    long long n;                       /* elements, one behind the other */
+    int src_type, dst_type;            /* ds_type                        */
+} ds_tensor_t;
+
+long long ds_clip_bytes(int count);
+int ds_clip_norm(const ds_tensor_t *tensors, int count, float max_norm, float *norm, void *scratch, long long scratch_bytes,
+                 void *stream);
+
 /*
  * Reads and clears the device-side flag that a kernel of this library sets when one of its
  * bounded waits ran out (its output is then undefined; it never happens in a correct run).

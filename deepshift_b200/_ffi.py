@@ -61,6 +61,17 @@ class Adapters(ctypes.Structure):
     ]
 
 
+class Loss(ctypes.Structure):
+    """Mirror of ``ds_loss_t``."""
+    _fields_ = [
+        ("rows", ctypes.c_int), ("d", ctypes.c_int), ("v", ctypes.c_int), ("type", ctypes.c_int), ("reduction", ctypes.c_int),
+        ("hidden", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("target", ctypes.c_void_p), ("ignore_index", ctypes.c_longlong),
+        ("each", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("count", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p), ("dhidden", ctypes.c_void_p), ("dweight", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_longlong),
+    ]
+
+
 IN_I32, IN_F32_CONV, IN_F32_LINEAR, IN_I32_CLAMP = 0, 1, 2, 3
 OUT_I32, OUT_F32 = 0, 1
 T_F32, T_BF16, T_F16 = 0, 1, 2
@@ -109,6 +120,8 @@ _SIGNATURES = {
     "ds_rows_plan": [_VP, _I, _I, _VP, _LL, _VP],
     "ds_adapters_apply": [ctypes.POINTER(Adapters), _VP],
     "ds_adapters_backward": [ctypes.POINTER(Adapters), _VP],
+    "ds_loss_forward": [ctypes.POINTER(Loss), _VP],
+    "ds_loss_backward": [ctypes.POINTER(Loss), _VP],
     "ds_clip_norm": [_VP, _I, ctypes.c_float, _VP, _VP, _LL, _VP],
     "ds_avgpool_fix_nhwc": [_VP, _VP, _I, _I, _I, _I, _I, _VP],
 }
@@ -141,7 +154,7 @@ def lib():
         l.ds_launch_count.restype = ctypes.c_longlong
         l.ds_planes_bytes.argtypes = [_I] * 5
         l.ds_planes_bytes.restype = ctypes.c_longlong
-        for name, n in (("ds_rows_plan_bytes", 2), ("ds_adapters_h_bytes", 6), ("ds_clip_bytes", 1)):
+        for name, n in (("ds_rows_plan_bytes", 2), ("ds_adapters_h_bytes", 6), ("ds_clip_bytes", 1), ("ds_loss_bytes", 5)):
             getattr(l, name).argtypes = [_I] * n
             getattr(l, name).restype = ctypes.c_longlong
         l.ds_staged_bytes.argtypes = [_I] * 5

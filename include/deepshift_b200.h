@@ -495,6 +495,37 @@ int ds_clip_norm(const ds_tensor_t *tensors, int count, float max_norm, float *n
                  void *stream);
 
 /*
+ * Softmax cross entropy of a linear head, loss[i] = logsumexp(W hidden[i]) - W[target[i]] . hidden[i], without its logits
+ * (no counterpart in the reference).  Operands are bf16 or fp16, sums fp32.  Rows whose target is ignore_index count for
+ * nothing: loss 0, gradient 0; a target that is neither that nor in 0 .. v - 1 makes its row's loss and the
+ * gradients that it enters NaN.  The mean of no rows is NaN, its gradient 0.
+ *
+ * ds_loss_forward writes each[rows] and lse[rows], and loss and count unless reduction is DS_LOSS_NONE;
+ * ds_loss_backward reads lse and count, and grad: the gradient of loss (one value), or of each[rows] for DS_LOSS_NONE.
+ * scratch (256-byte aligned) holds ds_loss_bytes(rows, d, v, backward, copies), copies = 1 where hidden or weight is not 16-byte
+ * aligned: they are copied then, as they are where d is no multiple of 8.  Rows and v up to 2^24, d up to 2^20.
+ */
+enum { DS_LOSS_NONE = 0, DS_LOSS_MEAN = 1, DS_LOSS_SUM = 2 };
+typedef struct {
+    int rows, d, v;
+    int type;                          /* DS_T_BF16 or DS_T_F16                     */
+    int reduction;                     /* DS_LOSS_*                                 */
+    const void *hidden, *weight;       /* [rows][d], [v][d]                         */
+    const int64_t *target;             /* [rows]                                    */
+    long long ignore_index;
+    float *each, *lse;                 /* [rows]                                    */
+    float *loss, *count;               /* one value each                            */
+    const float *grad;
+    void *dhidden, *dweight;           /* [rows][d], [v][d], 16-byte aligned; or NULL */
+    void *scratch;
+    long long scratch_bytes;
+} ds_loss_t;
+
+long long ds_loss_bytes(int rows, int d, int v, int backward, int copies);
+int ds_loss_forward(const ds_loss_t *a, void *stream);
+int ds_loss_backward(const ds_loss_t *a, void *stream);
+
+/*
  * Reads and clears the device-side flag that a kernel of this library sets when one of its
  * bounded waits ran out (its output is then undefined; it never happens in a correct run).
  * Synchronises the current device.  *flag = 0 means no error.

@@ -7,6 +7,7 @@ namespace ds {
 namespace adapters {
 namespace {
 
+constexpr int MAX_RANK = 256;
 constexpr int PLAN_THREADS = 1024, PLAN_WARPS = 32;
 
 __device__ __forceinline__ int row_key(const int* __restrict__ ids, int m, int count)
@@ -137,7 +138,7 @@ bool aligned(const void* p, long long stride, int type)
 // CTAs a tile's sums are shared by: until there are two for each SM, as long as every warp keeps a piece of its own.
 int splits_of(int rows, int width, int rank, int count, bool same16)
 {
-    const long long tiles = plan_tiles(rows, count) * ((rank + 63) / 64);
+    const long long tiles = plan_tiles(rows, count) * (same16 ? (rank + 63) / 64 : (rank + 31) / 32);
     const int pieces = (width + (same16 ? 31 : 15)) / (same16 ? 32 : 16) / WARPS;
     long long s = 296 / (tiles < 1 ? 1 : tiles);   // no rows, no tiles
     if (s > pieces) s = pieces;
@@ -166,56 +167,81 @@ bool allow_smem(int bytes)
 template <class X, class W, int MT, int NT, bool VEC>
 int launch_down(const Args& a, cudaStream_t st)
 {
-    const int smem = WARPS * 16 * MT * 8 * NT * 4;
-    static_assert(WARPS * 16 * MT * 8 * NT * 4 <= 65536, "shared memory of the sums");
+    constexpr int smem = Down<X, W, MT, NT>::smem(VEC);
+    static_assert(smem <= 227 * 1024, "shared memory of an SM");
     if (!allow_smem<down_kernel<X, W, MT, NT, VEC>>(smem)) return DS_ERR_CUDA;
     const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), a.splits, (a.rank8 + 8 * NT - 1) / (8 * NT));
     down_kernel<X, W, MT, NT, VEC><<<grid, THREADS, smem, st>>>(a);
     return finish();
 }
 
+// Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere, where 64 would not fit the
+// registers and the rows are read again from L2 instead.
+template <class X, class W, int MT>
+int down_tile(const Args& a, bool vec, cudaStream_t st)
+{
+    if (!vec) return a.rank8 <= 8 ? launch_down<X, W, MT, 1, false>(a, st) : launch_down<X, W, MT, 4, false>(a, st);
+    if (a.rank8 <= 8) return launch_down<X, W, MT, 1, true>(a, st);
+    if (a.rank8 <= 16) return launch_down<X, W, MT, 2, true>(a, st);
+    if constexpr (Down<X, W, MT, 8>::SAME)
+        if (a.rank8 > 32) return launch_down<X, W, MT, 8, true>(a, st);
+    return launch_down<X, W, MT, 4, true>(a, st);
+}
+
 template <class X, class W>
 int down(const Args& a, bool vec, cudaStream_t st)
 {
-    const bool wide = plan_tile_rows(a.rows) == 32;
-    if (!vec) return wide ? launch_down<X, W, 2, 8, false>(a, st) : launch_down<X, W, 1, 8, false>(a, st);
-    if (a.rank8 <= 8) return wide ? launch_down<X, W, 2, 1, true>(a, st) : launch_down<X, W, 1, 1, true>(a, st);
-    if (a.rank8 <= 16) return wide ? launch_down<X, W, 2, 2, true>(a, st) : launch_down<X, W, 1, 2, true>(a, st);
-    if (a.rank8 <= 32) return wide ? launch_down<X, W, 2, 4, true>(a, st) : launch_down<X, W, 1, 4, true>(a, st);
-    return wide ? launch_down<X, W, 2, 8, true>(a, st) : launch_down<X, W, 1, 8, true>(a, st);
+    return plan_tile_rows(a.rows) == 32 ? down_tile<X, W, 2>(a, vec, st) : down_tile<X, W, 1>(a, vec, st);
 }
 
-template <class X, class W, int MT>
-int launch_up(const Args& a, bool vec, cudaStream_t st)
+template <class X, class W, int MT, bool VEC>
+int launch_up(const Args& a, cudaStream_t st)
 {
+    // h of the tile in two parts, and the base's columns
+    const int smem = a.rank8 * 16 * MT * 8 + (VEC ? THREADS * 16 * 2 * MT * int(sizeof(X)) : 0);
+    if (!allow_smem<up_kernel<X, W, MT, VEC>>(MAX_RANK * 16 * MT * 8 + (VEC ? THREADS * 16 * 2 * MT * int(sizeof(X)) : 0))) return DS_ERR_CUDA;
     const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS));
-    if (vec) up_kernel<X, W, MT, true><<<grid, THREADS, 0, st>>>(a);
-    else up_kernel<X, W, MT, false><<<grid, THREADS, 0, st>>>(a);
+    up_kernel<X, W, MT, VEC><<<grid, THREADS, smem, st>>>(a);
     return finish();
 }
 
 template <class X, class W>
 int up(const Args& a, bool vec, cudaStream_t st)
 {
-    return plan_tile_rows(a.rows) == 32 ? launch_up<X, W, 2>(a, vec, st) : launch_up<X, W, 1>(a, vec, st);
+    if (plan_tile_rows(a.rows) == 32) return vec ? launch_up<X, W, 2, true>(a, st) : launch_up<X, W, 2, false>(a, st);
+    return vec ? launch_up<X, W, 1, true>(a, st) : launch_up<X, W, 1, false>(a, st);
 }
 
-template <class X, class W, int RT, int NJ, bool VEC>
+template <class X, class W, int RT, bool VEC>
 int launch_grad(const Args& a, cudaStream_t st)
 {
-    const int smem = WARPS * 16 * RT * 8 * NJ * 4;
-    if (!allow_smem<grad_kernel<X, W, RT, NJ, VEC>>(smem)) return DS_ERR_CUDA;
-    const dim3 grid((a.width + 8 * NJ - 1) / (8 * NJ), a.count, (a.rank + 16 * RT - 1) / (16 * RT));
-    grad_kernel<X, W, RT, NJ, VEC><<<grid, THREADS, smem, st>>>(a);
+    constexpr int sums = WARPS * 16 * RT * 64 * 4, queue = VEC ? GRAD_STAGES * THREADS * 16 * grad_pieces<X> : 0;
+    constexpr int smem = sums > queue ? sums : queue;
+    if (!allow_smem<grad_kernel<X, W, RT, VEC>>(smem)) return DS_ERR_CUDA;
+    const int columns = (a.width + 63) / 64, blocks = (a.rank + 16 * RT - 1) / (16 * RT);
+    // CTAs that share an adapter's rows: until two for each SM are at work, as long as each warp has two steps of rows, were the
+    // rows spread evenly
+    int shares = 1;
+    while (shares < 8 && (long long)columns * a.count * blocks * shares * 2 <= 296 && a.rows / a.count >= 2 * shares * 2 * WARPS * 8) shares *= 2;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(a.count * blocks, columns, shares);
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim = {1, 1, unsigned(shares)};
+    c.attrs = &cluster;
+    c.numAttrs = 1;
+    if (cudaLaunchKernelEx(&c, grad_kernel<X, W, RT, VEC>, a) != cudaSuccess) return DS_ERR_CUDA;
     return finish();
 }
 
 template <class X, class W>
 int grad(const Args& a, bool vec, cudaStream_t st)
 {
-    constexpr int NJ = is_f32<X> ? 4 : 8;
-    if (!vec) return launch_grad<X, W, 2, NJ, false>(a, st);
-    return a.rank <= 16 ? launch_grad<X, W, 1, NJ, true>(a, st) : launch_grad<X, W, 2, NJ, true>(a, st);
+    if (!vec) return launch_grad<X, W, 2, false>(a, st);
+    return a.rank <= 16 ? launch_grad<X, W, 1, true>(a, st) : launch_grad<X, W, 2, true>(a, st);
 }
 
 // Calls f(X{}, W{}) with the types of a call.
@@ -241,7 +267,7 @@ int rank8(int rank) { return (rank + 7) / 8 * 8; }
 int check(const ds_adapters_t* a, bool backward)
 {
     if (!a || a->rows < 0 || a->k < 1 || a->n < 1 || a->rank < 1 || a->count < 1) return DS_ERR_BAD_ARG;
-    if (a->rank > 256 || a->count > 65535) return DS_ERR_UNSUPPORTED;
+    if (a->rank > MAX_RANK || a->count > 65535) return DS_ERR_UNSUPPORTED;
     if (a->rows > 1 << 24 || a->k > 1 << 20 || a->n > 1 << 20) return DS_ERR_RANGE;
     if (!a->plan || !a->down || !a->up) return DS_ERR_BAD_ARG;
     if (a->rows && (!a->x || !a->h)) return DS_ERR_BAD_ARG;

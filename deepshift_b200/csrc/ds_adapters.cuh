@@ -153,12 +153,19 @@ __device__ __forceinline__ unsigned to_tf32(float v)
     return r;
 }
 
-// hi + lo = v to 21 bits; an infinity has no lo.
+// hi + lo = v to 21 bits (an infinity, whose lo is none, ends up as NaN).
 __device__ __forceinline__ void split(float v, unsigned& hi, unsigned& lo)
 {
     hi = __float_as_uint(v) & 0xFFFFE000u;
-    const float h = __uint_as_float(hi);
-    lo = h == v ? 0u : to_tf32(v - h);
+    lo = to_tf32(v - __uint_as_float(hi));
+}
+
+// A value that is a TF32 number already, or its two parts.
+template <bool EXACT>
+__device__ __forceinline__ void parts(float v, unsigned& hi, unsigned& lo)
+{
+    if (EXACT) hi = __float_as_uint(v), lo = 0;
+    else split(v, hi, lo);
 }
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
@@ -184,98 +191,188 @@ __device__ __forceinline__ void mma_16bit(float (&d)[4], unsigned a0, unsigned a
 // Row of lane's fragment rows: position p of the tile, or -1 behind its end.
 __device__ __forceinline__ int tile_row(const PlanView& plan, const int4& tile, int p) { return p < tile.z ? plan.order[tile.y + p] : -1; }
 
-// Loads of one 16-byte piece of a 16-bit row, as it is.
-template <class T, bool VEC>
-__device__ __forceinline__ uint4 load_raw(const T* p, int live)
+// Sixteen bytes from global to shared memory behind the thread's back, or zeros.  Each lane fills and reads slots of its own:
+// a queue deeper than registers would allow, and no barrier.
+__device__ __forceinline__ void copy16(unsigned to, const void* from, bool live)
 {
-    if (VEC && live >= 8) return *reinterpret_cast<const uint4*>(p);
-    unsigned w[4] = {0, 0, 0, 0};
-    if (!VEC) {
-        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+__device__ __forceinline__ uint4 slot(unsigned at)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+
+// The elements of N pieces as fp32.
+template <class T, int N>
+__device__ __forceinline__ void widen_pieces(const uint4 (&p)[N], float (&v)[N * 16 / sizeof(T)])
+{
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < live) w[i >> 1] |= unsigned(q[i]) << (16 * (i & 1));
+    for (int i = 0; i < N; ++i) {
+        const unsigned w[4] = {p[i].x, p[i].y, p[i].z, p[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (is_f32<T>) v[4 * i + e] = __uint_as_float(w[e]);
+            else {
+                v[8 * i + 2 * e] = widen<T>((unsigned short)(w[e] & 0xFFFFu));
+                v[8 * i + 2 * e + 1] = widen<T>((unsigned short)(w[e] >> 16));
+            }
+        }
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Shapes of down_kernel: elements a lane takes of a row at a time (sixteen bytes of the narrower type), the 16-byte pieces of
+// that in both operands, and how many such steps are on their way (96 KB a CTA, so that two fit an SM; two steps at least).
+template <class X, class W, int MT, int NT>
+struct Down {
+    static constexpr bool SAME = !is_f32<X> && __is_same(X, W);   // both of one 16-bit type: no conversion at all
+    static constexpr int LK = is_f32<X> && is_f32<W> ? 4 : 8, XP = LK * sizeof(X) / 16, WP = LK * sizeof(W) / 16;
+    static constexpr int PIECES = 2 * MT * XP + NT * WP, STAGE = THREADS * 16 * PIECES;
+    static constexpr int FIT = 98304 / STAGE, STAGES = FIT < 2 ? 2 : FIT > 6 ? 6 : FIT;
+    static constexpr int SUMS = WARPS * 16 * MT * 8 * NT * 4;
+    static constexpr int smem(bool vec) { return vec && STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS; }
+};
+
+// One step's products.  fp32 sums of a few products begin at zero and are added to the running ones by the adder, which rounds; the
+// tensor core's own additions cut off, and a chain of 200 of them had a relative error of 3e-6.
+template <class X, class W, int MT, int NT, int LK>
+__device__ __forceinline__ void down_step(float (&acc)[MT][NT][4], const float (&a)[2 * MT][LK], const float (&b)[NT][LK])
+{
+#pragma unroll
+    for (int e = 0; e < LK; e += 2) {
+        unsigned ah[MT][4], al[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            parts<!is_f32<X>>(a[2 * i][e], ah[i][0], al[i][0]);
+            parts<!is_f32<X>>(a[2 * i + 1][e], ah[i][1], al[i][1]);
+            parts<!is_f32<X>>(a[2 * i][e + 1], ah[i][2], al[i][2]);
+            parts<!is_f32<X>>(a[2 * i + 1][e + 1], ah[i][3], al[i][3]);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            unsigned h0, h1, l0, l1;
+            parts<!is_f32<W>>(b[j][e], h0, l0);
+            parts<!is_f32<W>>(b[j][e + 1], h1, l1);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float t[4] = {};
+                if (is_f32<X>) mma_tf32(t, al[i], h0, h1);
+                if (is_f32<W>) mma_tf32(t, ah[i], l0, l1);
+                mma_tf32(t, ah[i], h0, h1);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[i][j][q] += t[q];
+            }
+        }
+    }
 }
 
 // h for one tile of 16 MT rows: a CTA's warps share the summed index out among them, and so do `splits` CTAs (blockIdx.y),
 // each of which writes its own partial sums.  blockIdx.z: ranks by 8 NT.
 template <class X, class W, int MT, int NT, bool VEC>
-__global__ void __launch_bounds__(THREADS) down_kernel(const Args p)
+__global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
 {
-    extern __shared__ float red[];   // [WARPS][16 MT][8 NT]
+    using S = Down<X, W, MT, NT>;
+    constexpr int LK = S::LK, CHUNK = 4 * LK;
+    extern __shared__ __align__(16) unsigned char smem[];
     if (int(blockIdx.x) >= p.plan.head[0]) return;
     const int4 tile = p.plan.tiles[blockIdx.x];
     if (tile.x >= p.count) return;   // rows without an adapter: nothing reads their h
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int r0 = blockIdx.z * 8 * NT;
-    const W* w = static_cast<const W*>(p.w) + (long long)tile.x * p.rank * p.width;
+    // rows g, 8 + g, ... of this CTA's ranks, and where this lane's elements begin
+    const W* w = static_cast<const W*>(p.w) + ((long long)tile.x * p.rank + r0 + g) * p.width + t * LK;
+    const long long eight = 8ll * p.width;
+    const int ranks = p.rank - r0 - g;   // row 8 j is one as long as 8 j is less
     const X* xr[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
         const int m = tile_row(p.plan, tile, 8 * i + g);
-        xr[i] = m < 0 ? nullptr : static_cast<const X*>(p.x) + m * p.ldx;
-    }
-    const W* wr[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int r = r0 + 8 * j + g;
-        wr[j] = r < p.rank ? w + (long long)r * p.width : nullptr;
+        xr[i] = m < 0 ? nullptr : static_cast<const X*>(p.x) + m * p.ldx + t * LK;
     }
     float acc[MT][NT][4] = {};
-    constexpr bool SAME = !is_f32<X> && __is_same(X, W);   // both of one 16-bit type: no conversion at all
-    constexpr int LK = SAME ? 8 : 4;                       // consecutive elements a lane takes
-    constexpr int CHUNK = 4 * LK;
-    const int chunks = (p.width + CHUNK - 1) / CHUNK, workers = WARPS * p.splits;
-#pragma unroll 2
-    for (int c = blockIdx.y * WARPS + warp; c < chunks; c += workers) {
-        const int k = c * CHUNK + t * LK, live = p.width - k;
-        if constexpr (SAME) {
-            uint4 a[2 * MT], b[NT];
+    const int chunks = (p.width + CHUNK - 1) / CHUNK, workers = WARPS * p.splits, first = blockIdx.y * WARPS + warp;
+    if constexpr (VEC) {
+        const unsigned mine = shared_address(smem) + threadIdx.x * 16;
+        auto issue = [&](int c, int stage) {
+            if (c < chunks) {
+                const unsigned to = mine + stage * S::STAGE;
+                const bool live = c * CHUNK + t * LK < p.width;   // a width of whole eights: all of the lane's elements, or none
+                int q = 0;
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) a[i] = load_raw<X, VEC>(xr[i] + k, xr[i] ? live : 0);
+                for (int i = 0; i < 2 * MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) b[j] = load_raw<W, VEC>(wr[j] + k, wr[j] ? live : 0);
+                    for (int e = 0; e < S::XP; ++e, ++q)
+                        copy16(to + q * THREADS * 16, live && xr[i] ? xr[i] + c * CHUNK + e * (LK / S::XP) : static_cast<const X*>(p.x), live && xr[i]);
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < S::WP; ++e, ++q)
+                        copy16(to + q * THREADS * 16, live && 8 * j < ranks ? w + j * eight + c * CHUNK + e * (LK / S::WP) : static_cast<const W*>(p.w),
+                               live && 8 * j < ranks);
+            }
+            copies_end();
+        };
+        int stage = 0, ahead = S::STAGES - 1;
+#pragma unroll
+        for (int i = 0; i < S::STAGES - 1; ++i) issue(first + i * workers, i);
+        for (int c = first; c < chunks; c += workers) {
+            copies_wait<S::STAGES - 2>();
+            const unsigned from = mine + stage * S::STAGE;
+            issue(c + (S::STAGES - 1) * workers, ahead);
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+            ahead = ahead + 1 == S::STAGES ? 0 : ahead + 1;
+            uint4 a[2 * MT][S::XP];
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+                for (int e = 0; e < S::XP; ++e) a[i][e] = slot(from + (i * S::XP + e) * THREADS * 16);
+            if constexpr (S::SAME) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    mma_16bit<X>(acc[i][j], a[2 * i].x, a[2 * i + 1].x, a[2 * i].y, a[2 * i + 1].y, b[j].x, b[j].y);
-                    mma_16bit<X>(acc[i][j], a[2 * i].z, a[2 * i + 1].z, a[2 * i].w, a[2 * i + 1].w, b[j].z, b[j].w);
-                }
-        } else {
-            float a[2 * MT][4], b[NT][4];
-#pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) load<X, 4, VEC>(xr[i] + k, xr[i] ? live : 0, a[i]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) load<W, 4, VEC>(wr[j] + k, wr[j] ? live : 0, b[j]);
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-                unsigned ah[MT][4], al[MT][4];
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    split(a[2 * i][e], ah[i][0], al[i][0]);
-                    split(a[2 * i + 1][e], ah[i][1], al[i][1]);
-                    split(a[2 * i][e + 1], ah[i][2], al[i][2]);
-                    split(a[2 * i + 1][e + 1], ah[i][3], al[i][3]);
-                }
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    unsigned b0, b1, l0, l1;
-                    split(b[j][e], b0, l0);
-                    split(b[j][e + 1], b1, l1);
+                    const uint4 k = slot(from + (2 * MT + j) * THREADS * 16);
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        mma_tf32(acc[i][j], ah[i], b0, b1);
-                        if (is_f32<X>) mma_tf32(acc[i][j], al[i], b0, b1);
-                        if (is_f32<W>) mma_tf32(acc[i][j], ah[i], l0, l1);
+                        const uint4 &u = a[2 * i][0], &v = a[2 * i + 1][0];
+                        mma_16bit<X>(acc[i][j], u.x, v.x, u.y, v.y, k.x, k.y);
+                        mma_16bit<X>(acc[i][j], u.z, v.z, u.w, v.w, k.z, k.w);
                     }
                 }
+            } else {
+                float af[2 * MT][LK], bf[NT][LK];
+#pragma unroll
+                for (int i = 0; i < 2 * MT; ++i) widen_pieces<X>(a[i], af[i]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    uint4 b[S::WP];
+#pragma unroll
+                    for (int e = 0; e < S::WP; ++e) b[e] = slot(from + (2 * MT * S::XP + j * S::WP + e) * THREADS * 16);
+                    widen_pieces<W>(b, bf[j]);
+                }
+                down_step<X, W, MT, NT, LK>(acc, af, bf);
             }
+        }
+        copies_wait<0>();
+    } else {
+        for (int c = first; c < chunks; c += workers) {
+            const int k = c * CHUNK, live = p.width - k - t * LK;
+            float af[2 * MT][LK], bf[NT][LK];
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) load<X, LK, false>(xr[i] + k, xr[i] ? live : 0, af[i]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) load<W, LK, false>(w + j * eight + k, 8 * j < ranks ? live : 0, bf[j]);
+            down_step<X, W, MT, NT, LK>(acc, af, bf);
         }
     }
     constexpr int ROWS = 16 * MT, COLS = 8 * NT;
+    float* red = reinterpret_cast<float*>(smem);   // [WARPS][ROWS][COLS]
+    __syncthreads();   // the queue's memory is free
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -295,134 +392,230 @@ __global__ void __launch_bounds__(THREADS) down_kernel(const Args p)
     }
 }
 
-// Two consecutive values of h, summed over the splits in their order and scaled.
-__device__ __forceinline__ float2 load_h(const Args& p, int m, int r, float scale)
+// A value of h, summed over the splits in their order and scaled.
+__device__ __forceinline__ float load_h(const Args& p, int m, int r, float scale)
 {
-    float2 s = make_float2(0.f, 0.f);
-    if (m >= 0) {
-        for (int q = 0; q < p.splits; ++q) {
-            const float2 v = *reinterpret_cast<const float2*>(p.h + ((long long)q * p.rows + m) * p.rank8 + r);
-            s.x += v.x, s.y += v.y;
-        }
-        s.x *= scale, s.y *= scale;
-    }
-    return s;
+    float s = 0.f;
+    for (int q = 0; q < p.splits; ++q) s += p.h[((long long)q * p.rows + m) * p.rank8 + r];
+    return s * scale;
 }
 
 // One tile of 16 MT rows, 64 columns a warp: lane (g, t) loads eight consecutive columns 8 g .. of ranks 2t and 2t + 1, which are
-// the elements of eight instructions, and ends up with the sixteen consecutive columns 16 t .. of rows g and g + 8.
+// the elements of eight instructions, and ends up with the sixteen consecutive columns 16 t .. of rows g and g + 8.  The tile's h,
+// scaled and split, lies in shared memory for all warps in the order in which the instructions read it; base is on its way meanwhile.
 template <class X, class W, int MT, bool VEC>
-__global__ void __launch_bounds__(THREADS) up_kernel(const Args p)
+__global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 {
+    constexpr int BP = 16 * sizeof(X) / 16;   // pieces of a lane's columns of one row
+    extern __shared__ __align__(16) unsigned char smem[];
     if (int(blockIdx.x) >= p.plan.head[0]) return;
     const int4 tile = p.plan.tiles[blockIdx.x];
     const bool none = tile.x >= p.count;
     if (none && p.base == p.out) return;   // in place: these rows are there already
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int n0 = (blockIdx.y * WARPS + warp) * 64;
-    if (n0 >= p.width) return;
     int row[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) row[i] = tile_row(p.plan, tile, 8 * i + g);
+    const unsigned mine = shared_address(smem) + p.rank8 * 16 * MT * 8 + threadIdx.x * 16;
+    if (VEC && p.base) {
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+            for (int e = 0; e < BP; ++e) {
+                const int n = n0 + 16 * t + e * (16 / BP);
+                const bool live = row[i] >= 0 && n < p.width;
+                copy16(mine + (i * BP + e) * THREADS * 16, static_cast<const X*>(p.base) + (live ? row[i] * p.ldbase + n : 0), live);
+            }
+        copies_end();
+    }
     float acc[MT][8][4] = {};
     if (!none) {
         const float scale = p.scale ? p.scale[tile.x] : 1.f;
+        float4* h = reinterpret_cast<float4*>(smem);   // [rank8 / 8][MT][hi, lo][32 lanes]
+        for (int i = threadIdx.x; i < 16 * MT * p.rank8; i += THREADS) {
+            const int at = i / p.rank8, r = i - at * p.rank8, m = tile_row(p.plan, tile, at);
+            unsigned hi = 0, lo = 0;
+            if (m >= 0) split(load_h(p, m, r, scale), hi, lo);
+            // element of the lane that holds row at % 8 and rank pair r % 8 / 2: rows by 8, then the pair's second
+            const int frag = ((r / 8 * MT + at / 16) * 2 * 32 + at % 8 * 4 + r % 8 / 2) * 4 + (at / 8 & 1) + 2 * (r & 1);
+            reinterpret_cast<unsigned*>(h)[frag] = hi;
+            reinterpret_cast<unsigned*>(h)[frag + 128] = lo;
+        }
+        __syncthreads();
         const W* w = static_cast<const W*>(p.w) + (long long)tile.x * p.rank * p.width + n0 + 8 * g;
         const int live = p.width - n0 - 8 * g;
-#pragma unroll 2
+        float next[2][8];
+        auto fetch = [&](int r) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) load<W, 8, VEC>(w + (long long)(r + 2 * t + e) * p.width, r + 2 * t + e < p.rank ? live : 0, next[e]);
+        };
+        fetch(0);
         for (int r = 0; r < p.rank8; r += 8) {
-            const int ra = r + 2 * t;
-            float b0[8], b1[8];
-            load<W, 8, VEC>(w + (long long)ra * p.width, ra < p.rank ? live : 0, b0);
-            load<W, 8, VEC>(w + (long long)(ra + 1) * p.width, ra + 1 < p.rank ? live : 0, b1);
+            float b[2][8];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) b[e >> 3][e & 7] = next[e >> 3][e & 7];
+            if (r + 8 < p.rank8) fetch(r + 8);
             unsigned ah[MT][4], al[MT][4];
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const float2 u = load_h(p, row[2 * i], ra, scale), v = load_h(p, row[2 * i + 1], ra, scale);
-                split(u.x, ah[i][0], al[i][0]);
-                split(v.x, ah[i][1], al[i][1]);
-                split(u.y, ah[i][2], al[i][2]);
-                split(v.y, ah[i][3], al[i][3]);
+                const uint4 u = slot(shared_address(h + ((r / 8 * MT + i) * 2) * 32 + lane)), v = slot(shared_address(h + ((r / 8 * MT + i) * 2 + 1) * 32 + lane));
+                ah[i][0] = u.x, ah[i][1] = u.y, ah[i][2] = u.z, ah[i][3] = u.w;
+                al[i][0] = v.x, al[i][1] = v.y, al[i][2] = v.z, al[i][3] = v.w;
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 unsigned h0, h1, l0, l1;
-                split(b0[j], h0, l0);
-                split(b1[j], h1, l1);
+                parts<!is_f32<W>>(b[0][j], h0, l0);
+                parts<!is_f32<W>>(b[1][j], h1, l1);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    mma_tf32(acc[i][j], ah[i], h0, h1);
-                    mma_tf32(acc[i][j], al[i], h0, h1);
-                    if (is_f32<W>) mma_tf32(acc[i][j], ah[i], l0, l1);
+                    // fp32 results: as in down_step
+                    float s[4] = {};
+                    float(&d)[4] = is_f32<X> ? s : acc[i][j];
+                    mma_tf32(d, al[i], h0, h1);
+                    if (is_f32<W>) mma_tf32(d, ah[i], l0, l1);
+                    mma_tf32(d, ah[i], h0, h1);
+                    if (is_f32<X>) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] += s[e];
+                    }
                 }
             }
         }
     }
     // column 8 c + j of the warp's 64 sits in element c of instruction j: c = 2t and 2t + 1 are this lane's
+    if (VEC) copies_wait<0>();
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
         if (row[i] < 0) continue;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int n = n0 + 16 * t + 8 * c, live = p.width - n;
-            float v[8];
-            if (p.base) load<X, 8, VEC>(static_cast<const X*>(p.base) + row[i] * p.ldbase + n, live, v);
+            float v[8] = {};
+            if (p.base) {
+                if constexpr (VEC) {
+                    uint4 q[BP / 2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = acc[i >> 1][j][(i & 1) * 2 + c];
-                v[j] = p.base ? v[j] + d : d;
+                    for (int e = 0; e < BP / 2; ++e) q[e] = slot(mine + (i * BP + c * (BP / 2) + e) * THREADS * 16);
+                    widen_pieces<X>(q, v);
+                } else load<X, 8, VEC>(static_cast<const X*>(p.base) + row[i] * p.ldbase + n, live, v);
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += acc[i >> 1][j][(i & 1) * 2 + c];
             store<X, 8, VEC>(static_cast<X*>(p.out) + row[i] * p.ldout + n, live, v);
         }
     }
 }
 
-// dw[a][r0 .. r0 + 16 RT)[n0 .. n0 + 8 NJ) over all rows of adapter a, which the warps share out: eight sorted rows an instruction.
-template <class X, class W, int RT, int NJ, bool VEC>
-__global__ void __launch_bounds__(THREADS) grad_kernel(const Args p)
+constexpr int GRAD_STAGES = 3;
+template <class X>
+constexpr int grad_pieces = 8 * sizeof(X) / 16 * 2;   // of a lane's eight columns of two rows
+
+// dw[a][r0 .. r0 + 16 RT)[n0 .. n0 + 64) over all rows of adapter a, eight sorted rows an instruction: the warps of the `gridDim.z` CTAs of
+// a cluster share the rows out, and the CTAs add up their sums over distributed shared memory, in their order.
+template <class X, class W, int RT, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
 {
-    extern __shared__ float red[];   // [WARPS][16 RT][8 NJ]
+    constexpr int NJ = 8, ROWS = 16 * RT, COLS = 8 * NJ, XP = grad_pieces<X> / 2, STAGE = THREADS * 16 * grad_pieces<X>;
+    extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int a = blockIdx.y, n0 = blockIdx.x * 8 * NJ, r0 = blockIdx.z * 16 * RT;
-    const int first = p.plan.offsets[a], last = p.plan.offsets[a + 1];
+    const int blocks = (p.rank + ROWS - 1) / ROWS;
+    const int a = blockIdx.x / blocks, n0 = blockIdx.y * COLS, r0 = blockIdx.x % blocks * ROWS;
+    const int shares = gridDim.z, share = blockIdx.z, step = 8 * WARPS * shares;
+    const int begin = p.plan.offsets[a] + 8 * (share * WARPS + warp), end = p.plan.offsets[a + 1];
     const float scale = p.scale ? p.scale[a] : 1.f;
     const int n = n0 + NJ * g, live = p.width - n;
     float acc[RT][NJ][4] = {};
-#pragma unroll 2
-    for (int at = first + 8 * warp; at < last; at += 8 * WARPS) {
-        int m[2];
-        float b[2][NJ];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int pos = at + 2 * t + e;
-            m[e] = pos < last ? p.plan.order[pos] : -1;
-            load<X, NJ, VEC>(static_cast<const X*>(p.x) + (long long)max(m[e], 0) * p.ldx + n, m[e] >= 0 ? live : 0, b[e]);
-        }
+    auto row_at = [&](int at, int e) { return at + 2 * t + e < end ? p.plan.order[at + 2 * t + e] : -1; };
+    auto products = [&](const float (&b)[2][NJ], const float (&h)[RT][4]) {
         unsigned ah[RT][4], al[RT][4];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split(h[i][e] * scale, ah[i][e], al[i][e]);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            unsigned h0, h1, l0, l1;
+            parts<!is_f32<X>>(b[0][j], h0, l0);
+            parts<!is_f32<X>>(b[1][j], h1, l1);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                float s[4] = {};   // as in down_step
+                float(&d)[4] = is_f32<W> ? s : acc[i][j];
+                mma_tf32(d, al[i], h0, h1);
+                if (is_f32<X>) mma_tf32(d, ah[i], l0, l1);
+                mma_tf32(d, ah[i], h0, h1);
+                if (is_f32<W>) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] += s[e];
+                }
+            }
+        }
+    };
+    // h of ranks g and g + 8 of both rows: elements of the instruction's first operand
+    auto load_rows_h = [&](const int (&m)[2], float (&h)[RT][4]) {
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = r0 + 16 * i + g + 8 * (e & 1), row = m[e >> 1];
-                float v = 0.f;
-                if (row >= 0 && r < p.rank)
-                    for (int q = 0; q < p.splits; ++q) v += p.h[((long long)q * p.rows + row) * p.rank8 + r];
-                split(v * scale, ah[i][e], al[i][e]);
+                h[i][e] = row >= 0 && r < p.rank ? load_h(p, row, r, 1.f) : 0.f;
             }
+    };
+    if constexpr (VEC) {
+        const unsigned mine = shared_address(smem) + threadIdx.x * 16;
+        auto issue = [&](const int (&m)[2], int stage) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            unsigned h0, h1, l0, l1;
-            split(b[0][j], h0, l0);
-            split(b[1][j], h1, l1);
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                mma_tf32(acc[i][j], ah[i], h0, h1);
-                mma_tf32(acc[i][j], al[i], h0, h1);
-                if (is_f32<X>) mma_tf32(acc[i][j], ah[i], l0, l1);
-            }
+                for (int q = 0; q < XP; ++q) {
+                    const bool in = m[e] >= 0 && live > 0;
+                    copy16(mine + stage * STAGE + (e * XP + q) * THREADS * 16,
+                           static_cast<const X*>(p.x) + (in ? m[e] * p.ldx + n + q * (NJ / XP) : 0), in);
+                }
+            copies_end();
+        };
+        // rows of the steps on their way: their indexes are read one step before their copies begin
+        int rows[GRAD_STAGES][2];
+#pragma unroll
+        for (int i = 0; i < GRAD_STAGES; ++i) rows[i][0] = row_at(begin + i * step, 0), rows[i][1] = row_at(begin + i * step, 1);
+#pragma unroll
+        for (int i = 0; i < GRAD_STAGES - 1; ++i) issue(rows[i], i);
+        int stage = 0, ahead = GRAD_STAGES - 1;
+        for (int at = begin; at < end; at += step) {
+            float h[RT][4];
+            load_rows_h(rows[0], h);
+            copies_wait<GRAD_STAGES - 2>();
+            uint4 q[2][XP];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int c = 0; c < XP; ++c) q[e][c] = slot(mine + stage * STAGE + (e * XP + c) * THREADS * 16);
+            issue(rows[GRAD_STAGES - 1], ahead);
+            stage = stage + 1 == GRAD_STAGES ? 0 : stage + 1;
+            ahead = ahead + 1 == GRAD_STAGES ? 0 : ahead + 1;
+#pragma unroll
+            for (int i = 0; i < GRAD_STAGES - 1; ++i) rows[i][0] = rows[i + 1][0], rows[i][1] = rows[i + 1][1];
+            rows[GRAD_STAGES - 1][0] = row_at(at + GRAD_STAGES * step, 0), rows[GRAD_STAGES - 1][1] = row_at(at + GRAD_STAGES * step, 1);
+            float b[2][NJ];
+            widen_pieces<X>(q[0], b[0]);
+            widen_pieces<X>(q[1], b[1]);
+            products(b, h);
+        }
+        copies_wait<0>();
+    } else {
+        for (int at = begin; at < end; at += step) {
+            const int m[2] = {row_at(at, 0), row_at(at, 1)};
+            float h[RT][4], b[2][NJ];
+            load_rows_h(m, h);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) load<X, NJ, false>(static_cast<const X*>(p.x) + (m[e] >= 0 ? m[e] * p.ldx + n : 0), m[e] >= 0 ? live : 0, b[e]);
+            products(b, h);
         }
     }
-    constexpr int ROWS = 16 * RT, COLS = 8 * NJ;
+    float* red = reinterpret_cast<float*>(smem);   // [WARPS][ROWS][COLS]; the CTA's sums end up in the first
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -431,16 +624,40 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(const Args p)
             for (int e = 0; e < 4; ++e)
                 red[(warp * ROWS + 16 * i + g + (e & 2) * 4) * COLS + (2 * t + (e & 1)) * NJ + j] = acc[i][j][e];
     __syncthreads();
-    for (int i = threadIdx.x * 8; i < ROWS * COLS; i += THREADS * 8) {
+    if (shares > 1) {
+        for (int i = threadIdx.x; i < ROWS * COLS; i += THREADS) {
+            float s = 0.f;
+#pragma unroll
+            for (int q = 0; q < WARPS; ++q) s += red[q * ROWS * COLS + i];
+            red[i] = s;   // this thread alone reads and writes element i of each
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    for (int i = (share * THREADS + threadIdx.x) * 8; i < ROWS * COLS; i += shares * THREADS * 8) {
         const int r = r0 + i / COLS, at = n0 + i % COLS;
         if (r >= p.rank || at >= p.width) continue;
         float s[8] = {};
+        if (shares == 1) {
 #pragma unroll
-        for (int q = 0; q < WARPS; ++q)
+            for (int q = 0; q < WARPS; ++q)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] += red[q * ROWS * COLS + i + e];
+                for (int e = 0; e < 8; ++e) s[e] += red[q * ROWS * COLS + i + e];
+        } else {
+            for (int q = 0; q < shares; ++q) {
+                unsigned from;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(shared_address(red + i)), "r"(q));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float v;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(from + 4 * e) : "memory");
+                    s[e] += v;
+                }
+            }
+        }
         store<W, 8, VEC>(static_cast<W*>(p.out) + ((long long)a * p.rank + r) * p.width + at, p.width - at, s);
     }
+    // nobody leaves while its sums are being read
+    if (shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 }  // namespace adapters

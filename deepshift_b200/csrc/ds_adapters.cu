@@ -206,23 +206,41 @@ int launch_up(const Args& a, cudaStream_t st)
 }
 
 template <class X, class W>
-int up(const Args& a, bool vec, cudaStream_t st)
+int launch_up_stream(const Args& a, cudaStream_t st)
 {
-    if (plan_tile_rows(a.rows) == 32) return vec ? launch_up<X, W, 2, true>(a, st) : launch_up<X, W, 2, false>(a, st);
-    return vec ? launch_up<X, W, 1, true>(a, st) : launch_up<X, W, 1, false>(a, st);
+    using S = Stream<X, W>;
+    static_assert(S::smem(S::MOST_RANK) <= 227 * 1024, "shared memory of an SM");
+    if (!allow_smem<up_stream_kernel<X, W>>(S::smem(S::MOST_RANK))) return DS_ERR_CUDA;
+    const int columns = (a.width + S::COLS - 1) / S::COLS, per_sm = S::smem(a.rank8) <= 113 * 1024 ? 2 : 1;
+    const long long tiles = plan_tiles(a.rows, a.count);
+    long long runs = 148 * per_sm / columns;   // one wave
+    runs = runs < 1 ? 1 : runs > tiles ? tiles : runs;
+    up_stream_kernel<X, W><<<dim3(unsigned(runs), columns), THREADS, S::smem(a.rank8), st>>>(a);
+    return finish();
 }
 
-template <class X, class W, int RT, bool VEC>
+template <class X, class W>
+int up(const Args& a, bool vec, cudaStream_t st)
+{
+    const bool wide = plan_tile_rows(a.rows) == 32;
+    if (!vec) return wide ? launch_up<X, W, 2, false>(a, st) : launch_up<X, W, 1, false>(a, st);
+    if (!wide) return launch_up<X, W, 1, true>(a, st);
+    if (a.rank8 <= Stream<X, W>::MOST_RANK) return launch_up_stream<X, W>(a, st);
+    return launch_up<X, W, 2, true>(a, st);
+}
+
+template <class X, class W, int RT, int CW, bool VEC>
 int launch_grad(const Args& a, cudaStream_t st)
 {
-    constexpr int sums = WARPS * 16 * RT * 64 * 4, queue = VEC ? GRAD_STAGES * THREADS * 16 * grad_pieces<X> : 0;
-    constexpr int smem = sums > queue ? sums : queue;
-    if (!allow_smem<grad_kernel<X, W, RT, VEC>>(smem)) return DS_ERR_CUDA;
-    const int columns = (a.width + 63) / 64, blocks = (a.rank + 16 * RT - 1) / (16 * RT);
-    // CTAs that share an adapter's rows: until two for each SM are at work, as long as each warp has two steps of rows, were the
+    constexpr int RW = WARPS / CW, block = RW == 8 ? 64 : 32;
+    constexpr int sums = RW * 16 * RT * 64 * CW * 4, work = 2 * block * 16 * RT * 8 + (VEC ? GRAD_STAGES * THREADS * 16 * grad_pieces<X> : 0);
+    constexpr int smem = sums > work ? sums : work;
+    if (!allow_smem<grad_kernel<X, W, RT, CW, VEC>>(smem)) return DS_ERR_CUDA;
+    const int columns = (a.width + 64 * CW - 1) / (64 * CW), blocks = (a.rank + 16 * RT - 1) / (16 * RT);
+    // CTAs that share an adapter's rows: until two for each SM are at work, as long as each has two blocks of rows, were the
     // rows spread evenly
     int shares = 1;
-    while (shares < 8 && (long long)columns * a.count * blocks * shares * 2 <= 296 && a.rows / a.count >= 2 * shares * 2 * WARPS * 8) shares *= 2;
+    while (shares < 8 && (long long)columns * a.count * blocks * shares < 296 && a.rows / a.count >= 2 * shares * 2 * block) shares *= 2;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(a.count * blocks, columns, shares);
     c.blockDim = dim3(THREADS);
@@ -233,15 +251,23 @@ int launch_grad(const Args& a, cudaStream_t st)
     cluster.val.clusterDim = {1, 1, unsigned(shares)};
     c.attrs = &cluster;
     c.numAttrs = 1;
-    if (cudaLaunchKernelEx(&c, grad_kernel<X, W, RT, VEC>, a) != cudaSuccess) return DS_ERR_CUDA;
+    if (cudaLaunchKernelEx(&c, grad_kernel<X, W, RT, CW, VEC>, a) != cudaSuccess) return DS_ERR_CUDA;
     return finish();
+}
+
+template <class X, class W, int RT, bool VEC>
+int grad_columns(const Args& a, cudaStream_t st)
+{
+    if (a.width <= 64) return launch_grad<X, W, RT, 1, VEC>(a, st);
+    if (a.width <= 256) return launch_grad<X, W, RT, 4, VEC>(a, st);
+    return launch_grad<X, W, RT, 8, VEC>(a, st);
 }
 
 template <class X, class W>
 int grad(const Args& a, bool vec, cudaStream_t st)
 {
-    if (!vec) return launch_grad<X, W, 2, false>(a, st);
-    return a.rank <= 16 ? launch_grad<X, W, 1, true>(a, st) : launch_grad<X, W, 2, true>(a, st);
+    if (!vec) return launch_grad<X, W, 2, 4, false>(a, st);
+    return a.rank <= 16 ? grad_columns<X, W, 1, true>(a, st) : grad_columns<X, W, 2, true>(a, st);
 }
 
 // Calls f(X{}, W{}) with the types of a call.

@@ -136,12 +136,13 @@ __device__ __forceinline__ void store(T* p, int live, const float (&v)[N])
         }
         return;
     }
-    if (VEC) return;
+    if constexpr (!VEC) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (i < live) {
-            if constexpr (is_f32<T>) p[i] = v[i];
-            else reinterpret_cast<unsigned short*>(p)[i] = narrow<T>(v[i]);
+        for (int i = 0; i < N; ++i) {
+            if (i < live) {
+                if constexpr (is_f32<T>) p[i] = v[i];
+                else reinterpret_cast<unsigned short*>(p)[i] = narrow<T>(v[i]);
+            }
         }
     }
 }
@@ -392,12 +393,39 @@ __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
     }
 }
 
-// A value of h, summed over the splits in their order and scaled.
-__device__ __forceinline__ float load_h(const Args& p, int m, int r, float scale)
+// Four values of h, summed over the splits in their order and scaled; 0 without a row.
+__device__ __forceinline__ float4 load_h4(const Args& p, int m, int r, float scale)
 {
-    float s = 0.f;
-    for (int q = 0; q < p.splits; ++q) s += p.h[((long long)q * p.rows + m) * p.rank8 + r];
-    return s * scale;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m < 0) return s;
+    const float* h = p.h + (long long)m * p.rank8 + r;
+    for (int q = 0; q < p.splits; ++q) {
+        const float4 v = *reinterpret_cast<const float4*>(h + (long long)q * p.rows * p.rank8);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
+    return s;
+}
+
+// The two parts of v at word `at` of a block of 128 words for hi, 128 for lo.
+__device__ __forceinline__ void put_parts(unsigned* at, float v)
+{
+    unsigned hi, lo;
+    split(v, hi, lo);
+    at[0] = hi;
+    at[128] = lo;
+}
+
+// Values r .. r + 3 (r a multiple of 4) of row `at` of a tile into the order in which the instruction reads its first operand [row][rank]:
+// blocks [rank / 8][halves of 16 rows][hi, lo][lane][4], the lane that holds row at % 8 and rank pair r % 8 / 2, its
+// elements by rows of 8 and then by the pair's second.
+__device__ __forceinline__ void put_h4(unsigned* h, int halves, int at, int r, const float4& v)
+{
+    unsigned* to = h + (r / 8 * halves + at / 16) * 256 + (at % 8 * 4 + r % 8 / 2) * 4 + (at / 8 & 1);
+    put_parts(to, v.x);
+    put_parts(to + 2, v.y);
+    put_parts(to + 4, v.z);
+    put_parts(to + 6, v.w);
 }
 
 // One tile of 16 MT rows, 64 columns a warp: lane (g, t) loads eight consecutive columns 8 g .. of ranks 2t and 2t + 1, which are
@@ -432,16 +460,10 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
     float acc[MT][8][4] = {};
     if (!none) {
         const float scale = p.scale ? p.scale[tile.x] : 1.f;
-        float4* h = reinterpret_cast<float4*>(smem);   // [rank8 / 8][MT][hi, lo][32 lanes]
-        for (int i = threadIdx.x; i < 16 * MT * p.rank8; i += THREADS) {
-            const int at = i / p.rank8, r = i - at * p.rank8, m = tile_row(p.plan, tile, at);
-            unsigned hi = 0, lo = 0;
-            if (m >= 0) split(load_h(p, m, r, scale), hi, lo);
-            // element of the lane that holds row at % 8 and rank pair r % 8 / 2: rows by 8, then the pair's second
-            const int frag = ((r / 8 * MT + at / 16) * 2 * 32 + at % 8 * 4 + r % 8 / 2) * 4 + (at / 8 & 1) + 2 * (r & 1);
-            reinterpret_cast<unsigned*>(h)[frag] = hi;
-            reinterpret_cast<unsigned*>(h)[frag + 128] = lo;
-        }
+        unsigned* h = reinterpret_cast<unsigned*>(smem);
+        constexpr int PER = THREADS / (16 * MT);   // threads a row
+        const int at = threadIdx.x / PER, m = tile_row(p.plan, tile, at);
+        for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(h, MT, at, r, load_h4(p, m, r, scale));
         __syncthreads();
         const W* w = static_cast<const W*>(p.w) + (long long)tile.x * p.rank * p.width + n0 + 8 * g;
         const int live = p.width - n0 - 8 * g;
@@ -459,7 +481,8 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
             unsigned ah[MT][4], al[MT][4];
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const uint4 u = slot(shared_address(h + ((r / 8 * MT + i) * 2) * 32 + lane)), v = slot(shared_address(h + ((r / 8 * MT + i) * 2 + 1) * 32 + lane));
+                const unsigned here = shared_address(h + (r / 8 * MT + i) * 256 + lane * 4);
+                const uint4 u = slot(here), v = slot(here + 512);
                 ah[i][0] = u.x, ah[i][1] = u.y, ah[i][2] = u.z, ah[i][3] = u.w;
                 al[i][0] = v.x, al[i][1] = v.y, al[i][2] = v.z, al[i][3] = v.w;
             }
@@ -508,32 +531,210 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
     }
 }
 
-constexpr int GRAD_STAGES = 3;
+// Many rows: up_kernel's product for 256 columns and a run of consecutive tiles of 32 rows.  The adapter's part of `w` stays in shared memory
+// until a tile of another adapter comes (up_kernel reads it from L2 for every tile, and waits for it), and the next tile's
+// base and h are on their way during a tile's products.  Four warps side by side, two above one another.
+template <class X, class W>
+struct Stream {
+    static constexpr int COLS = 256, ROWS = 32;
+    static constexpr int BP = 16 * sizeof(X) / 16, BASE = THREADS * 16 * 2 * BP;   // base of a tile: two rows of sixteen columns a lane
+    static constexpr int WROW = COLS * int(sizeof(W)) + 16;   // a row of w: rows 2t of the lanes t fall on different banks
+    static constexpr int MOST_RANK = 64;
+    __host__ __device__ static constexpr int h_bytes(int rank8) { return ROWS * rank8 * 8; }
+    static constexpr int smem(int rank8) { return 2 * BASE + 2 * h_bytes(rank8) + rank8 * WROW; }
+};
+
+template <class X, class W>
+__global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
+{
+    using S = Stream<X, W>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int total = p.plan.head[0], first = int((long long)total * blockIdx.x / gridDim.x), last = int((long long)total * (blockIdx.x + 1) / gridDim.x);
+    if (first == last) return;
+    const int c0 = blockIdx.y * S::COLS, in_block = (warp & 3) * 64, n0 = c0 + in_block, half = warp >> 2;
+    const unsigned base_at = shared_address(smem) + threadIdx.x * 16, h_at = shared_address(smem) + 2 * S::BASE, w_at = h_at + 2 * S::h_bytes(p.rank8);
+    constexpr int PER = THREADS / S::ROWS, HV = S::MOST_RANK / 4 / PER;   // threads a row, and fours of its h that each brings in
+    const int h_row = threadIdx.x / PER, h_rank = threadIdx.x % PER * 4;
+    float4 hv[HV];
+    auto row_of = [&](const int4& tile, int e) { return tile_row(p.plan, tile, 16 * half + 8 * e + g); };
+    auto issue_base = [&](const int4& tile, const int (&row)[2], int buf) {
+        if (p.base) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < S::BP; ++e) {
+                    const int n = n0 + 16 * t + e * (16 / S::BP);
+                    const bool live = row[i] >= 0 && n < p.width;
+                    copy16(base_at + buf * S::BASE + (i * S::BP + e) * THREADS * 16, static_cast<const X*>(p.base) + (live ? row[i] * p.ldbase + n : 0), live);
+                }
+        }
+        copies_end();
+    };
+    auto fetch_h = [&](const int4& tile) {
+        const bool none = tile.x >= p.count;
+        const float scale = p.scale && !none ? p.scale[tile.x] : 1.f;
+        const int m = none ? -1 : tile_row(p.plan, tile, h_row);
+#pragma unroll
+        for (int q = 0; q < HV; ++q)
+            if (h_rank + q * PER * 4 < p.rank8) hv[q] = load_h4(p, m, h_rank + q * PER * 4, scale);
+    };
+    auto put_h = [&](int buf) {
+        unsigned* h = reinterpret_cast<unsigned*>(smem + 2 * S::BASE + buf * S::h_bytes(p.rank8));
+#pragma unroll
+        for (int q = 0; q < HV; ++q)
+            if (h_rank + q * PER * 4 < p.rank8) put_h4(h, 2, h_row, h_rank + q * PER * 4, hv[q]);
+    };
+    auto load_w = [&](int adapter) {
+        constexpr int PER = 16 / sizeof(W), PIECES = S::COLS / PER;
+        const W* w = static_cast<const W*>(p.w) + (long long)adapter * p.rank * p.width + c0;
+        for (int i = threadIdx.x; i < p.rank8 * PIECES; i += THREADS) {
+            const int r = i / PIECES, c = i % PIECES * PER;
+            const bool live = r < p.rank && c0 + c < p.width;
+            copy16(w_at + r * S::WROW + c * int(sizeof(W)), live ? w + (long long)r * p.width + c : static_cast<const W*>(p.w), live);
+        }
+        copies_end();
+    };
+    int4 tile = p.plan.tiles[first];
+    int row[2] = {row_of(tile, 0), row_of(tile, 1)};
+    issue_base(tile, row, 0);
+    int held = -1;   // whose w is in shared memory
+    if (tile.x < p.count) load_w(held = tile.x);
+    fetch_h(tile);
+    put_h(0);
+    copies_wait<0>();
+    __syncthreads();
+    for (int at = first, buf = 0; at < last; ++at, buf ^= 1) {
+        const int4 next = at + 1 < last ? p.plan.tiles[at + 1] : make_int4(p.count, 0, 0, 0);
+        const int next_row[2] = {row_of(next, 0), row_of(next, 1)};
+        issue_base(next, next_row, buf ^ 1);
+        fetch_h(next);
+        float acc[8][4] = {};
+        if (tile.x < p.count) {
+            const unsigned h = h_at + buf * S::h_bytes(p.rank8) + half * 1024 + lane * 16;
+            const unsigned w = w_at + 2 * t * S::WROW + (in_block + 8 * g) * int(sizeof(W));
+            for (int r = 0; r < p.rank8; r += 8) {
+                constexpr int WP = 8 * sizeof(W) / 16;
+                uint4 q[2][WP];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int c = 0; c < WP; ++c) q[e][c] = slot(w + (r + e) * S::WROW + c * 16);
+                const uint4 u = slot(h + r / 8 * 2048), v = slot(h + r / 8 * 2048 + 512);
+                const unsigned ah[4] = {u.x, u.y, u.z, u.w}, al[4] = {v.x, v.y, v.z, v.w};
+                float b[2][8];
+                widen_pieces<W>(q[0], b[0]);
+                widen_pieces<W>(q[1], b[1]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    unsigned h0, h1, l0, l1;
+                    parts<!is_f32<W>>(b[0][j], h0, l0);
+                    parts<!is_f32<W>>(b[1][j], h1, l1);
+                    float s[4] = {};   // fp32 results: as in down_step
+                    float(&d)[4] = is_f32<X> ? s : acc[j];
+                    mma_tf32(d, al, h0, h1);
+                    if (is_f32<W>) mma_tf32(d, ah, l0, l1);
+                    mma_tf32(d, ah, h0, h1);
+                    if (is_f32<X>) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[j][e] += s[e];
+                    }
+                }
+            }
+        }
+        copies_wait<1>();
+        if (!(tile.x >= p.count && p.base == p.out)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (row[i] < 0) continue;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int n = n0 + 16 * t + 8 * c;
+                    float v[8] = {};
+                    if (p.base) {
+                        uint4 q[S::BP / 2];
+#pragma unroll
+                        for (int e = 0; e < S::BP / 2; ++e) q[e] = slot(base_at + buf * S::BASE + (i * S::BP + c * (S::BP / 2) + e) * THREADS * 16);
+                        widen_pieces<X>(q, v);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += acc[j][i * 2 + c];
+                    store<X, 8, true>(static_cast<X*>(p.out) + row[i] * p.ldout + n, p.width - n, v);
+                }
+            }
+        }
+        put_h(buf ^ 1);
+        if (next.x < p.count && next.x != held) {
+            __syncthreads();   // everybody is done with the held one
+            load_w(held = next.x);
+            copies_wait<0>();
+        }
+        __syncthreads();
+        tile = next, row[0] = next_row[0], row[1] = next_row[1];
+    }
+    copies_wait<0>();
+}
+
+constexpr int GRAD_STAGES = 4;
 template <class X>
 constexpr int grad_pieces = 8 * sizeof(X) / 16 * 2;   // of a lane's eight columns of two rows
 
-// dw[a][r0 .. r0 + 16 RT)[n0 .. n0 + 64) over all rows of adapter a, eight sorted rows an instruction: the warps of the `gridDim.z` CTAs of
-// a cluster share the rows out, and the CTAs add up their sums over distributed shared memory, in their order.
-template <class X, class W, int RT, bool VEC>
+// dw[a][r0 .. r0 + 16 RT)[n0 .. n0 + 64 CW) over all rows of adapter a.  CW warps side by side, 8 / CW above one another, share a block of rows
+// whose h, scaled and split, lies in shared memory in the order in which the instructions read it; the next block's is on its way meanwhile, and
+// each lane's rows are several steps ahead.  The `gridDim.z` CTAs of a cluster take one part of the rows each and add up their
+// sums over distributed shared memory, in their order.
+template <class X, class W, int RT, int CW, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
 {
-    constexpr int NJ = 8, ROWS = 16 * RT, COLS = 8 * NJ, XP = grad_pieces<X> / 2, STAGE = THREADS * 16 * grad_pieces<X>;
-    extern __shared__ __align__(16) unsigned char smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int blocks = (p.rank + ROWS - 1) / ROWS;
-    const int a = blockIdx.x / blocks, n0 = blockIdx.y * COLS, r0 = blockIdx.x % blocks * ROWS;
-    const int shares = gridDim.z, share = blockIdx.z, step = 8 * WARPS * shares;
-    const int begin = p.plan.offsets[a] + 8 * (share * WARPS + warp), end = p.plan.offsets[a + 1];
+    constexpr int NJ = 8, RANKS = 16 * RT, COLS = 8 * NJ * CW, XP = grad_pieces<X> / 2, STAGE = THREADS * 16 * grad_pieces<X>;
+    constexpr int RW = WARPS / CW, BLOCK = RW == 8 ? 64 : 32, STEPS = BLOCK / 8 / RW;   // rows of a block, steps of a warp in it
+    constexpr int HV = (BLOCK * RANKS / 4 + THREADS - 1) / THREADS, H_BYTES = BLOCK * RANKS * 8;
+    extern __shared__ __align__(16) unsigned char smem[];   // h of two blocks, then the queue
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, cw = warp % CW, rw = warp / CW;
+    const int blocks = (p.rank + RANKS - 1) / RANKS;
+    const int a = blockIdx.x / blocks, n0 = blockIdx.y * COLS + 64 * cw, r0 = blockIdx.x % blocks * RANKS;
+    const int shares = gridDim.z, share = blockIdx.z;
+    // whole blocks of rows for each CTA
+    const int from = p.plan.offsets[a], all = p.plan.offsets[a + 1] - from, part = ((all + shares - 1) / shares + BLOCK - 1) / BLOCK * BLOCK;
+    const int begin = from + min(all, share * part), end = from + min(all, (share + 1) * part);
     const float scale = p.scale ? p.scale[a] : 1.f;
     const int n = n0 + NJ * g, live = p.width - n;
+    const int count = (end - begin + BLOCK - 1) / BLOCK;
     float acc[RT][NJ][4] = {};
-    auto row_at = [&](int at, int e) { return at + 2 * t + e < end ? p.plan.order[at + 2 * t + e] : -1; };
-    auto products = [&](const float (&b)[2][NJ], const float (&h)[RT][4]) {
+    // step i of this warp: rows 8 (i % STEPS RW + rw) ... of block i / STEPS
+    auto row_at = [&](int i, int e) {
+        const int at = begin + i / STEPS * BLOCK + (i % STEPS * RW + rw) * 8 + 2 * t + e;
+        return at < end ? p.plan.order[at] : -1;
+    };
+    float4 hv[HV];
+    auto fetch_h = [&](int block) {
+#pragma unroll
+        for (int q = 0; q < HV; ++q) {
+            const int i = threadIdx.x + q * THREADS, r = r0 + i % (RANKS / 4) * 4, at = begin + block * BLOCK + i / (RANKS / 4);
+            if (i < BLOCK * RANKS / 4) hv[q] = load_h4(p, at < end && r < p.rank8 ? p.plan.order[at] : -1, r, scale);
+        }
+    };
+    auto put_h = [&](int buf) {   // as put_h4, but of an operand [rank][row]: blocks [row / 8][RT][hi, lo][lane][4]
+        unsigned* h = reinterpret_cast<unsigned*>(smem + buf * H_BYTES);
+#pragma unroll
+        for (int q = 0; q < HV; ++q) {
+            const int i = threadIdx.x + q * THREADS, r = i % (RANKS / 4) * 4, at = i / (RANKS / 4);
+            if (i >= BLOCK * RANKS / 4) continue;
+            unsigned* to = h + (at / 8 * RT + r / 16) * 256 + (r % 8 * 4 + at % 8 / 2) * 4 + (r / 8 & 1) + 2 * (at & 1);
+            put_parts(to, hv[q].x);
+            put_parts(to + 16, hv[q].y);
+            put_parts(to + 32, hv[q].z);
+            put_parts(to + 48, hv[q].w);
+        }
+    };
+    auto products = [&](const float (&b)[2][NJ], unsigned h) {
         unsigned ah[RT][4], al[RT][4];
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split(h[i][e] * scale, ah[i][e], al[i][e]);
+        for (int i = 0; i < RT; ++i) {
+            const uint4 u = slot(h + i * 1024), v = slot(h + i * 1024 + 512);
+            ah[i][0] = u.x, ah[i][1] = u.y, ah[i][2] = u.z, ah[i][3] = u.w;
+            al[i][0] = v.x, al[i][1] = v.y, al[i][2] = v.z, al[i][3] = v.w;
+        }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             unsigned h0, h1, l0, l1;
@@ -553,68 +754,64 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
             }
         }
     };
-    // h of ranks g and g + 8 of both rows: elements of the instruction's first operand
-    auto load_rows_h = [&](const int (&m)[2], float (&h)[RT][4]) {
+    const unsigned mine = shared_address(smem) + 2 * H_BYTES + threadIdx.x * 16;
+    auto issue = [&](const int (&m)[2], int stage) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = r0 + 16 * i + g + 8 * (e & 1), row = m[e >> 1];
-                h[i][e] = row >= 0 && r < p.rank ? load_h(p, row, r, 1.f) : 0.f;
+            for (int q = 0; q < XP; ++q) {
+                const bool in = m[e] >= 0 && live > 0;
+                copy16(mine + stage * STAGE + (e * XP + q) * THREADS * 16,
+                       static_cast<const X*>(p.x) + (in ? m[e] * p.ldx + n + q * (NJ / XP) : 0), in);
             }
+        copies_end();
     };
+    int rows[2], stage = 0, ahead = GRAD_STAGES - 1;   // the rows of the step whose copies begin next
     if constexpr (VEC) {
-        const unsigned mine = shared_address(smem) + threadIdx.x * 16;
-        auto issue = [&](const int (&m)[2], int stage) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int q = 0; q < XP; ++q) {
-                    const bool in = m[e] >= 0 && live > 0;
-                    copy16(mine + stage * STAGE + (e * XP + q) * THREADS * 16,
-                           static_cast<const X*>(p.x) + (in ? m[e] * p.ldx + n + q * (NJ / XP) : 0), in);
-                }
-            copies_end();
-        };
-        // rows of the steps on their way: their indexes are read one step before their copies begin
-        int rows[GRAD_STAGES][2];
-#pragma unroll
-        for (int i = 0; i < GRAD_STAGES; ++i) rows[i][0] = row_at(begin + i * step, 0), rows[i][1] = row_at(begin + i * step, 1);
-#pragma unroll
-        for (int i = 0; i < GRAD_STAGES - 1; ++i) issue(rows[i], i);
-        int stage = 0, ahead = GRAD_STAGES - 1;
-        for (int at = begin; at < end; at += step) {
-            float h[RT][4];
-            load_rows_h(rows[0], h);
-            copies_wait<GRAD_STAGES - 2>();
-            uint4 q[2][XP];
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int c = 0; c < XP; ++c) q[e][c] = slot(mine + stage * STAGE + (e * XP + c) * THREADS * 16);
-            issue(rows[GRAD_STAGES - 1], ahead);
-            stage = stage + 1 == GRAD_STAGES ? 0 : stage + 1;
-            ahead = ahead + 1 == GRAD_STAGES ? 0 : ahead + 1;
-#pragma unroll
-            for (int i = 0; i < GRAD_STAGES - 1; ++i) rows[i][0] = rows[i + 1][0], rows[i][1] = rows[i + 1][1];
-            rows[GRAD_STAGES - 1][0] = row_at(at + GRAD_STAGES * step, 0), rows[GRAD_STAGES - 1][1] = row_at(at + GRAD_STAGES * step, 1);
-            float b[2][NJ];
-            widen_pieces<X>(q[0], b[0]);
-            widen_pieces<X>(q[1], b[1]);
-            products(b, h);
+        for (int i = 0; i < GRAD_STAGES - 1; ++i) {
+            const int m[2] = {row_at(i, 0), row_at(i, 1)};
+            issue(m, i);
         }
-        copies_wait<0>();
-    } else {
-        for (int at = begin; at < end; at += step) {
-            const int m[2] = {row_at(at, 0), row_at(at, 1)};
-            float h[RT][4], b[2][NJ];
-            load_rows_h(m, h);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) load<X, NJ, false>(static_cast<const X*>(p.x) + (m[e] >= 0 ? m[e] * p.ldx + n : 0), m[e] >= 0 ? live : 0, b[e]);
-            products(b, h);
-        }
+        rows[0] = row_at(GRAD_STAGES - 1, 0), rows[1] = row_at(GRAD_STAGES - 1, 1);
     }
-    float* red = reinterpret_cast<float*>(smem);   // [WARPS][ROWS][COLS]; the CTA's sums end up in the first
+    fetch_h(0);
+    put_h(0);
+    __syncthreads();
+    for (int block = 0; block < count; ++block) {
+        fetch_h(block + 1);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int i = block * STEPS + s;
+            const unsigned h = shared_address(smem) + (block & 1) * H_BYTES + (s * RW + rw) * RT * 1024 + lane * 16;
+            float b[2][NJ];
+            if constexpr (VEC) {
+                copies_wait<GRAD_STAGES - 2>();
+                uint4 q[2][XP];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int c = 0; c < XP; ++c) q[e][c] = slot(mine + stage * STAGE + (e * XP + c) * THREADS * 16);
+                issue(rows, ahead);
+                rows[0] = row_at(i + GRAD_STAGES, 0), rows[1] = row_at(i + GRAD_STAGES, 1);
+                stage = stage + 1 == GRAD_STAGES ? 0 : stage + 1;
+                ahead = ahead + 1 == GRAD_STAGES ? 0 : ahead + 1;
+                widen_pieces<X>(q[0], b[0]);
+                widen_pieces<X>(q[1], b[1]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int m = row_at(i, e);
+                    load<X, NJ, false>(static_cast<const X*>(p.x) + (m >= 0 ? m * p.ldx + n : 0), m >= 0 ? live : 0, b[e]);
+                }
+            }
+            products(b, h);
+        }
+        put_h(block + 1 & 1);
+        __syncthreads();
+    }
+    if (VEC) copies_wait<0>();
+    float* red = reinterpret_cast<float*>(smem);   // [RW][RANKS][COLS]; the CTA's sums end up in the first
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -622,35 +819,40 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                red[(warp * ROWS + 16 * i + g + (e & 2) * 4) * COLS + (2 * t + (e & 1)) * NJ + j] = acc[i][j][e];
+                red[(rw * RANKS + 16 * i + g + (e & 2) * 4) * COLS + 64 * cw + (2 * t + (e & 1)) * NJ + j] = acc[i][j][e];
     __syncthreads();
     if (shares > 1) {
-        for (int i = threadIdx.x; i < ROWS * COLS; i += THREADS) {
-            float s = 0.f;
+        if (RW > 1)
+            for (int i = threadIdx.x; i < RANKS * COLS; i += THREADS) {
+                float s = 0.f;
 #pragma unroll
-            for (int q = 0; q < WARPS; ++q) s += red[q * ROWS * COLS + i];
-            red[i] = s;   // this thread alone reads and writes element i of each
-        }
+                for (int q = 0; q < RW; ++q) s += red[q * RANKS * COLS + i];
+                red[i] = s;   // this thread alone reads and writes element i of each
+            }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    for (int i = (share * THREADS + threadIdx.x) * 8; i < ROWS * COLS; i += shares * THREADS * 8) {
-        const int r = r0 + i / COLS, at = n0 + i % COLS;
+    for (int i = (share * THREADS + threadIdx.x) * 8; i < RANKS * COLS; i += shares * THREADS * 8) {
+        const int r = r0 + i / COLS, at = blockIdx.y * COLS + i % COLS;
         if (r >= p.rank || at >= p.width) continue;
         float s[8] = {};
         if (shares == 1) {
 #pragma unroll
-            for (int q = 0; q < WARPS; ++q)
+            for (int q = 0; q < RW; ++q)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] += red[q * ROWS * COLS + i + e];
+                for (int e = 0; e < 8; ++e) s[e] += red[q * RANKS * COLS + i + e];
         } else {
             for (int q = 0; q < shares; ++q) {
-                unsigned from;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(shared_address(red + i)), "r"(q));
+                unsigned at_q;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_q) : "r"(shared_address(red + i)), "r"(q));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float v;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(from + 4 * e) : "memory");
-                    s[e] += v;
+                for (int e = 0; e < 8; e += 4) {
+                    float v[4];
+                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                                 : "r"(at_q + 4 * e)
+                                 : "memory");
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[e + c] += v[c];
                 }
             }
         }

@@ -20,7 +20,6 @@ import torch
 import torch.nn as nn
 
 from . import _ffi
-from .kernels import _stream_ptr
 
 TYPES = {torch.float32: _ffi.T_F32, torch.bfloat16: _ffi.T_BF16, torch.float16: _ffi.T_F16}
 
@@ -61,8 +60,7 @@ def plan_rows(ids, count, device=None):
     ids = (ids if ids.dtype == torch.int32 else ids.clamp(-2, MAX_COUNT).to(torch.int32)).contiguous()
     n = _ffi.lib().ds_rows_plan_bytes(ids.numel(), count)
     data = torch.empty(n // 4, dtype=torch.int32, device=ids.device)
-    with torch.cuda.device(ids.device):
-        _ffi.check(_ffi.lib().ds_rows_plan(ids.data_ptr(), ids.numel(), count, data.data_ptr(), n, _stream_ptr(ids.device)), "plan_rows")
+    _ffi.run("ds_rows_plan", ids.get_device(), ids.data_ptr(), ids.numel(), count, data.data_ptr(), n)
     return RowPlan(ids.numel(), count, data)
 
 
@@ -71,82 +69,78 @@ def _h_bytes(rows, width, rank, count, act, weight):
     return _ffi.lib().ds_adapters_h_bytes(rows, width, rank, count, act, weight)
 
 
-def _rows(t, name, width, like):
+def _rows(t, name, width, dtype, device):
     """A tensor as [rows, width] with consecutive elements in a row: itself where it is one, or its leading dimensions folded."""
-    if t.dim() < 1 or t.size(-1) != width:
-        raise RuntimeError("%s must have %d elements a row, got %s" % (name, width, tuple(t.shape)))
-    if t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError("%s must be %s on %s, got %s on %s" % (name, like.dtype, like.device, t.dtype, t.device))
-    if t.dim() != 2:
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        raise RuntimeError("%s must have %d elements a row, got %s" % (name, width, tuple(shape)))
+    if t.dtype is not dtype or t.get_device() != device:
+        raise RuntimeError("%s must be %s on cuda:%d, got %s on %s" % (name, dtype, device, t.dtype, t.device))
+    if len(shape) != 2:
         if not t.is_contiguous():
             raise RuntimeError("%s must be contiguous, or two-dimensional" % name)
-        t = t.view(-1, width)
+        return t.view(-1, width)
     if width > 1 and t.stride(1) != 1:
         raise RuntimeError("the elements of a row of %s must be contiguous" % name)
     return t
 
 
 def _check(x, down, up, scale, plan):
-    if not x.is_cuda:
+    """Sizes of a call whose arguments fit one another: count, rank, k, n, the two types and the device's index."""
+    device = x.get_device() if x.is_cuda else -1
+    if device < 0:
         raise RuntimeError("x must be a CUDA tensor")
-    if x.dtype not in TYPES or down.dtype not in TYPES:
+    act, weight = TYPES.get(x.dtype), TYPES.get(down.dtype)
+    if act is None or weight is None:
         raise RuntimeError("x and the adapters must be float32, bfloat16 or float16, got %s and %s" % (x.dtype, down.dtype))
-    if x.dtype != down.dtype and torch.float32 not in (x.dtype, down.dtype):
+    if act != weight and act and weight:   # float32 is 0
         raise RuntimeError("x is %s and the adapters %s: one of two types has to be float32" % (x.dtype, down.dtype))
-    for t, name in ((down, "down"), (up, "up")):
-        if t.dim() != 3 or not t.is_contiguous():
-            raise RuntimeError("%s must be contiguous, [count, rank, width]" % name)
-        if t.device != x.device or t.dtype != down.dtype:
-            raise RuntimeError("down and up must be of one type, on the device of x")
+    if down.dim() != 3 or up.dim() != 3 or not down.is_contiguous() or not up.is_contiguous():
+        raise RuntimeError("down and up must be contiguous, [count, rank, width]")
+    if up.dtype is not down.dtype or down.get_device() != device or up.get_device() != device:
+        raise RuntimeError("down and up must be of one type, on the device of x")
     count, rank, k = down.shape
-    if up.shape[:2] != down.shape[:2]:
+    count_up, rank_up, n = up.shape
+    if count_up != count or rank_up != rank:
         raise RuntimeError("down is %s and up %s: count and rank must agree" % (tuple(down.shape), tuple(up.shape)))
-    n = up.shape[2]
-    if not 1 <= rank <= MAX_RANK or not 1 <= k <= MAX_WIDTH or not 1 <= n <= MAX_WIDTH:
+    if not (1 <= rank <= MAX_RANK and 1 <= k <= MAX_WIDTH and 1 <= n <= MAX_WIDTH):
         raise RuntimeError("ranks are 1 .. %d and widths 1 .. %d, got %d, %d and %d" % (MAX_RANK, MAX_WIDTH, rank, k, n))
-    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (count,) or not scale.is_contiguous() or
-                              scale.device != x.device):
+    if scale is not None and (scale.dtype is not torch.float32 or scale.dim() != 1 or scale.numel() != count or not scale.is_contiguous() or
+                              scale.get_device() != device):
         raise RuntimeError("scale must be float32 [%d], contiguous, on the device of x" % count)
-    if plan.count != count or plan.device != x.device:
+    if plan.count != count or plan.device.index != device:
         raise RuntimeError("the plan is for %d adapters on %s, not for %d on %s" % (plan.count, plan.device, count, x.device))
-    return count, rank, k, n
-
-
-def _struct(plan, down, up, scale, rank, k, n, act, weight):
-    a = _ffi.Adapters()
-    a.rows, a.k, a.n, a.rank, a.count = plan.rows, k, n, rank, plan.count
-    a.act_type, a.weight_type = act, weight
-    a.plan, a.down, a.up = plan.data.data_ptr(), down.data_ptr(), up.data_ptr()
-    a.scale = scale.data_ptr() if scale is not None else None
-    return a
+    return count, rank, k, n, act, weight, device
 
 
 def _forward(x, down, up, scale, plan, base, out):
-    count, rank, k, n = _check(x, down, up, scale, plan)
-    shape = x.shape[:-1] + (n,)
-    rows = _rows(x, "x", k, x)
-    if rows.size(0) != plan.rows:
-        raise RuntimeError("x has %d rows, the plan is for %d" % (rows.size(0), plan.rows))
+    count, rank, k, n, act, weight, device = _check(x, down, up, scale, plan)
+    rows = _rows(x, "x", k, x.dtype, device)
+    m = plan.rows
+    if rows.shape[0] != m:
+        raise RuntimeError("x has %d rows, the plan is for %d" % (rows.shape[0], m))
+    shape = (m, n) if rows is x else x.shape[:-1] + (n,)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif out.shape != shape:
-        raise RuntimeError("out must be %s, got %s" % (tuple(shape), tuple(out.shape)))
-    to = _rows(out, "out", n, x)
-    act, weight = TYPES[x.dtype], TYPES[down.dtype]
-    a = _struct(plan, down, up, scale, rank, k, n, act, weight)
-    a.x, a.x_stride, a.out, a.out_stride = rows.data_ptr(), rows.stride(0), to.data_ptr(), to.stride(0)
+        to = out = x.new_empty(shape)
+        to_stride = n
+    else:
+        if out.shape != shape:
+            raise RuntimeError("out must be %s, got %s" % (tuple(shape), tuple(out.shape)))
+        to = _rows(out, "out", n, x.dtype, device)
+        to_stride = to.stride(0)
+    base_at = base_stride = 0
     if base is not None:
         if base.shape != shape:
             raise RuntimeError("base must be %s, got %s" % (tuple(shape), tuple(base.shape)))
-        add = _rows(base, "base", n, x)
-        if add.data_ptr() == to.data_ptr() and add.stride(0) != to.stride(0):
+        add = _rows(base, "base", n, x.dtype, device)
+        base_at, base_stride = add.data_ptr(), add.stride(0)
+        if base_at == to.data_ptr() and base_stride != to_stride:
             raise RuntimeError("base and out overlap")
-        a.base, a.base_stride = add.data_ptr(), add.stride(0)
-    nbytes = _h_bytes(plan.rows, k, rank, count, act, weight)
-    h = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
-    a.h, a.h_bytes = h.data_ptr(), nbytes
-    with torch.cuda.device(x.device):
-        _ffi.check(_ffi.lib().ds_adapters_apply(a, _stream_ptr(x.device)), "adapters.apply")
+    nbytes = _h_bytes(m, k, rank, count, act, weight)
+    h = x.new_empty(nbytes // 4, dtype=torch.float32)
+    _ffi.run("ds_adapters_apply", device, _ffi.pack_adapters(
+        m, k, n, rank, count, act, weight, plan.data.data_ptr(), down.data_ptr(), up.data_ptr(), scale.data_ptr() if scale is not None else 0,
+        rows.data_ptr(), rows.stride(0), base_at, base_stride, to.data_ptr(), to_stride, h.data_ptr(), nbytes, 0, 0, 0, 0, 0, 0, 0, 0))
     return out, h
 
 
@@ -162,34 +156,25 @@ class _Apply(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         x, down, up, scale, h = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if not any(need[:3]):
-            return None, None, None, None, None, grad if need[5] else None
-        plan, (count, rank, k), n = ctx.plan, down.shape, up.shape[2]
-        rows = _rows(x, "x", k, x)
-        g = grad.reshape(-1, n)
-        if n > 1 and g.stride(1) != 1:
-            g = g.contiguous()
-        act, weight = TYPES[x.dtype], TYPES[down.dtype]
-        a = _struct(plan, down, up, scale, rank, k, n, act, weight)
-        a.x, a.x_stride, a.grad, a.grad_stride = rows.data_ptr(), rows.stride(0), g.data_ptr(), g.stride(0)
+        need_x, need_down, need_up, _, _, need_base = ctx.needs_input_grad
         dx = ddown = dup = None
-        if need[0]:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            a.dx, a.dx_stride = dx.data_ptr(), k
-        if need[1]:
-            ddown = torch.empty_like(down)
-            a.ddown = ddown.data_ptr()
-        if need[2]:
-            dup = torch.empty_like(up)
-            a.dup = dup.data_ptr()
-        a.h, a.h_bytes = h.data_ptr(), 4 * h.numel()
-        nbytes = _h_bytes(plan.rows, n, rank, count, act, weight)
-        dh = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
-        a.dh, a.dh_bytes = dh.data_ptr(), nbytes
-        with torch.cuda.device(x.device):
-            _ffi.check(_ffi.lib().ds_adapters_backward(a, _stream_ptr(x.device)), "adapters.apply (backward)")
-        return dx, ddown, dup, None, None, grad if need[5] else None
+        if need_x or need_down or need_up:
+            plan, (count, rank, k), n, device = ctx.plan, down.shape, up.shape[2], x.get_device()
+            act, weight, m = TYPES[x.dtype], TYPES[down.dtype], ctx.plan.rows
+            rows = _rows(x, "x", k, x.dtype, device)
+            g = grad if grad.dim() == 2 else grad.reshape(-1, n)
+            if n > 1 and g.stride(1) != 1:
+                g = g.contiguous()
+            dx = x.new_empty(x.shape) if need_x else None
+            ddown = torch.empty_like(down) if need_down else None
+            dup = torch.empty_like(up) if need_up else None
+            nbytes = _h_bytes(m, n, rank, count, act, weight)
+            dh = h.new_empty(nbytes // 4)
+            _ffi.run("ds_adapters_backward", device, _ffi.pack_adapters(
+                m, k, n, rank, count, act, weight, plan.data.data_ptr(), down.data_ptr(), up.data_ptr(), scale.data_ptr() if scale is not None else 0,
+                rows.data_ptr(), rows.stride(0), 0, 0, 0, 0, h.data_ptr(), 4 * h.numel(), g.data_ptr(), g.stride(0),
+                dx.data_ptr() if need_x else 0, k, ddown.data_ptr() if need_down else 0, dup.data_ptr() if need_up else 0, dh.data_ptr(), nbytes))
+        return dx, ddown, dup, None, None, grad if need_base else None
 
 
 def apply(x, down, up, scale, plan, base=None, out=None):

@@ -557,8 +557,21 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
     constexpr int PER = THREADS / S::ROWS, HV = S::MOST_RANK / 4 / PER;   // threads a row, and fours of its h that each brings in
     const int h_row = threadIdx.x / PER, h_rank = threadIdx.x % PER * 4;
     float4 hv[HV];
-    auto row_of = [&](const int4& tile, int e) { return tile_row(p.plan, tile, 16 * half + 8 * e + g); };
-    auto issue_base = [&](const int4& tile, const int (&row)[2], int buf) {
+    // what is known of a tile ahead of time: its rows of this lane, the one whose h this thread brings in, and its scale
+    struct Ahead {
+        int4 tile;
+        int row[2], h_m;
+        float scale;
+    };
+    auto tile_of = [&](int i) { return i < last ? p.plan.tiles[i] : make_int4(p.count, 0, 0, 0); };
+    auto rows_of = [&](Ahead& n) {
+        n.row[0] = tile_row(p.plan, n.tile, 16 * half + g);
+        n.row[1] = tile_row(p.plan, n.tile, 16 * half + 8 + g);
+        const bool none = n.tile.x >= p.count;
+        n.h_m = none ? -1 : tile_row(p.plan, n.tile, h_row);
+        n.scale = p.scale && !none ? p.scale[n.tile.x] : 1.f;
+    };
+    auto issue_base = [&](const int (&row)[2], int buf) {
         if (p.base) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -571,13 +584,10 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
         }
         copies_end();
     };
-    auto fetch_h = [&](const int4& tile) {
-        const bool none = tile.x >= p.count;
-        const float scale = p.scale && !none ? p.scale[tile.x] : 1.f;
-        const int m = none ? -1 : tile_row(p.plan, tile, h_row);
+    auto fetch_h = [&](const Ahead& n) {
 #pragma unroll
         for (int q = 0; q < HV; ++q)
-            if (h_rank + q * PER * 4 < p.rank8) hv[q] = load_h4(p, m, h_rank + q * PER * 4, scale);
+            if (h_rank + q * PER * 4 < p.rank8) hv[q] = load_h4(p, n.h_m, h_rank + q * PER * 4, n.scale);
     };
     auto put_h = [&](int buf) {
         unsigned* h = reinterpret_cast<unsigned*>(smem + 2 * S::BASE + buf * S::h_bytes(p.rank8));
@@ -595,20 +605,25 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
         }
         copies_end();
     };
-    int4 tile = p.plan.tiles[first];
-    int row[2] = {row_of(tile, 0), row_of(tile, 1)};
-    issue_base(tile, row, 0);
+    Ahead now, next;
+    now.tile = tile_of(first);
+    next.tile = tile_of(first + 1);
+    rows_of(now);
+    rows_of(next);
+    issue_base(now.row, 0);
     int held = -1;   // whose w is in shared memory
-    if (tile.x < p.count) load_w(held = tile.x);
-    fetch_h(tile);
+    if (now.tile.x < p.count) load_w(held = now.tile.x);
+    fetch_h(now);
     put_h(0);
     copies_wait<0>();
     __syncthreads();
     for (int at = first, buf = 0; at < last; ++at, buf ^= 1) {
-        const int4 next = at + 1 < last ? p.plan.tiles[at + 1] : make_int4(p.count, 0, 0, 0);
-        const int next_row[2] = {row_of(next, 0), row_of(next, 1)};
-        issue_base(next, next_row, buf ^ 1);
+        issue_base(next.row, buf ^ 1);
         fetch_h(next);
+        Ahead then;
+        then.tile = tile_of(at + 2);
+        const int4 tile = now.tile;
+        const int(&row)[2] = now.row;
         float acc[8][4] = {};
         if (tile.x < p.count) {
             const unsigned h = h_at + buf * S::h_bytes(p.rank8) + half * 1024 + lane * 16;
@@ -663,14 +678,15 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
                 }
             }
         }
+        rows_of(then);
         put_h(buf ^ 1);
-        if (next.x < p.count && next.x != held) {
+        if (next.tile.x < p.count && next.tile.x != held) {
             __syncthreads();   // everybody is done with the held one
-            load_w(held = next.x);
+            load_w(held = next.tile.x);
             copies_wait<0>();
         }
         __syncthreads();
-        tile = next, row[0] = next_row[0], row[1] = next_row[1];
+        now = next, next = then;
     }
     copies_wait<0>();
 }
@@ -707,12 +723,17 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
         return at < end ? p.plan.order[at] : -1;
     };
     float4 hv[HV];
-    auto fetch_h = [&](int block) {
+    int h_m[HV];   // rows of the block whose h is brought in next, read a block before
+    auto fetch_rows = [&](int block) {
 #pragma unroll
         for (int q = 0; q < HV; ++q) {
             const int i = threadIdx.x + q * THREADS, r = r0 + i % (RANKS / 4) * 4, at = begin + block * BLOCK + i / (RANKS / 4);
-            if (i < BLOCK * RANKS / 4) hv[q] = load_h4(p, at < end && r < p.rank8 ? p.plan.order[at] : -1, r, scale);
+            h_m[q] = i < BLOCK * RANKS / 4 && at < end && r < p.rank8 ? p.plan.order[at] : -1;
         }
+    };
+    auto fetch_h = [&] {
+#pragma unroll
+        for (int q = 0; q < HV; ++q) hv[q] = load_h4(p, h_m[q], r0 + (threadIdx.x + q * THREADS) % (RANKS / 4) * 4, scale);
     };
     auto put_h = [&](int buf) {   // as put_h4, but of an operand [rank][row]: blocks [row / 8][RT][hi, lo][lane][4]
         unsigned* h = reinterpret_cast<unsigned*>(smem + buf * H_BYTES);
@@ -775,11 +796,14 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
         }
         rows[0] = row_at(GRAD_STAGES - 1, 0), rows[1] = row_at(GRAD_STAGES - 1, 1);
     }
-    fetch_h(0);
+    fetch_rows(0);
+    fetch_h();
+    fetch_rows(1);
     put_h(0);
     __syncthreads();
     for (int block = 0; block < count; ++block) {
-        fetch_h(block + 1);
+        fetch_h();
+        fetch_rows(block + 2);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int i = block * STEPS + s;

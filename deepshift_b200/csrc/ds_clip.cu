@@ -15,9 +15,8 @@ namespace ds {
 namespace {
 
 constexpr int CLIP_THREADS = 256;
-constexpr int CLIP_UNITS = 4;                                  // units of 8 elements a thread has in flight
-constexpr int CLIP_CHUNK = CLIP_THREADS * CLIP_UNITS * 8;      // elements
-constexpr int CLIP_CTAS = 148 * 6;                             // most CTAs, and partial sums, of a launch
+constexpr int CLIP_STEP = CLIP_THREADS * 16;   // bytes that a CTA's threads take in pieces of 16
+constexpr int CLIP_CTAS = 148 * 8;             // most CTAs, and partial sums, of a launch
 
 // Tensors of one launch, passed by value: nothing to copy to the device, nothing that a captured graph could outlive.
 template <int CAP>
@@ -28,7 +27,11 @@ struct ClipTable {
     int first[CAP + 1];      // first chunk of each tensor
     unsigned char kind[CAP]; // type of src, type of dst << 2, 16-byte aligned << 4
     int count;
+    int steps;               // a chunk: this many steps of U pieces a thread
 };
+
+// Elements of a 16-byte piece of a type.
+__device__ __forceinline__ int per_piece(int kind) { return kind == DS_T_F32 ? 4 : 8; }
 
 __device__ __forceinline__ float2 unpack(unsigned v, int kind)
 {
@@ -36,31 +39,36 @@ __device__ __forceinline__ float2 unpack(unsigned v, int kind)
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-// Eight elements from element `at` of a tensor of n; those beyond n are 0.
-__device__ __forceinline__ void load8(const void* p, int kind, bool vec, long long at, long long n, float (&v)[8])
+// The piece from element `at` of a tensor of n, zeros behind its end.
+__device__ __forceinline__ uint4 load_piece(const void* p, int kind, bool vec, long long at, long long n)
 {
-    if (vec && at + 8 <= n) {
+    const int per = per_piece(kind);
+    if (vec && at + per <= n) return *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at * (16 / per));
+    unsigned w[4] = {0, 0, 0, 0};
+    if (at < n) {
         if (kind == DS_T_F32) {
-            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-            const float4 a = q[0], b = q[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (at + i < n) w[i] = static_cast<const unsigned*>(p)[at + i];
         } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + at);
-            const unsigned w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = unpack(w[i], kind);
-                v[2 * i] = f.x, v[2 * i + 1] = f.y;
-            }
+            for (int i = 0; i < 8; ++i)
+                if (at + i < n) w[i >> 1] |= unsigned(static_cast<const unsigned short*>(p)[at + i]) << (16 * (i & 1));
         }
-        return;
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Values of a piece; fp32 has four, and zeros.
+__device__ __forceinline__ void widen(const uint4& q, int kind, float (&v)[8])
+{
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = 0.f;
-        if (at + i < n) {
-            if (kind == DS_T_F32) v[i] = static_cast<const float*>(p)[at + i];
-            else v[i] = unpack(static_cast<const unsigned short*>(p)[at + i], kind).x;
+    for (int i = 0; i < 4; ++i) {
+        if (kind == DS_T_F32) v[i] = __uint_as_float(w[i]), v[4 + i] = 0.f;
+        else {
+            const float2 f = unpack(w[i], kind);
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
         }
     }
 }
@@ -70,24 +78,27 @@ __device__ __forceinline__ unsigned short narrow(float f, int kind)
     return kind == DS_T_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
 }
 
-__device__ __forceinline__ void store8(void* p, int kind, bool vec, long long at, long long n, const float (&v)[8])
+__device__ __forceinline__ unsigned narrow2(float a, float b, int kind) { return narrow(a, kind) | unsigned(narrow(b, kind)) << 16; }
+
+// The `per` (4 or 8) values of a piece to element `at`.  Nothing reads them soon: the stores give way to what the sums left in L2.
+__device__ __forceinline__ void store_piece(void* p, int kind, bool vec, long long at, long long n, int per, const float (&v)[8])
 {
-    if (vec && at + 8 <= n) {
+    if (vec && at + per <= n) {
         if (kind == DS_T_F32) {
             float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-            q[0] = make_float4(v[0], v[1], v[2], v[3]);
-            q[1] = make_float4(v[4], v[5], v[6], v[7]);
+            __stcs(q, make_float4(v[0], v[1], v[2], v[3]));
+            if (per == 8) __stcs(q + 1, make_float4(v[4], v[5], v[6], v[7]));
         } else {
-            unsigned w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = narrow(v[2 * i], kind) | unsigned(narrow(v[2 * i + 1], kind)) << 16;
-            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            char* q = static_cast<char*>(p) + at * 2;
+            const uint2 a = make_uint2(narrow2(v[0], v[1], kind), narrow2(v[2], v[3], kind));
+            if (per == 8) __stcs(reinterpret_cast<uint4*>(q), make_uint4(a.x, a.y, narrow2(v[4], v[5], kind), narrow2(v[6], v[7], kind)));
+            else __stcs(reinterpret_cast<uint2*>(q), a);
         }
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        if (at + i < n) {
+        if (i < per && at + i < n) {
             if (kind == DS_T_F32) static_cast<float*>(p)[at + i] = v[i];
             else static_cast<unsigned short*>(p)[at + i] = narrow(v[i], kind);
         }
@@ -120,32 +131,53 @@ __device__ __forceinline__ double cta_sum(double v)
     return s;
 }
 
-// Squares are added up in fp32 by eights, which rounds each sum by some 1e-7 of itself at random, and the sums in double.
-// Eight whose sum leaves the range where fp32 can hold it (values beyond 1e18, or all so small that their squares vanish)
-// are squared in double instead.
-template <int CAP>
+// Squares are added up in fp32 by eights (two pieces of fp32, one of 16 bits), which rounds each sum by some 1e-7 of itself at
+// random, and the sums in double: one conversion for eight values, where one for each took twice as long as the reading.
+// Where a sum leaves the range that fp32 can hold (values beyond 1e18, or all so small that their squares vanish) the warp squares in
+// double instead, save for pieces that are 0 altogether.
+template <int CAP, int U>
 __global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* __restrict__ partial)
 {
     double acc = 0.0;
     for (int chunk = blockIdx.x; chunk < t.first[t.count]; chunk += gridDim.x) {
         const int i = tensor_of(t, chunk);
-        const int kind = t.kind[i] & 3;
+        const int kind = t.kind[i] & 3, per = per_piece(kind);
         const bool vec = t.kind[i] & 16;
         const void* p = t.src[i];
         const long long n = t.n[i];
-        const long long at = (long long)(chunk - t.first[i]) * CLIP_CHUNK + threadIdx.x * 8;
-        float v[CLIP_UNITS][8];
+        long long at = ((long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS + threadIdx.x) * per;
+        for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
+            uint4 q[U];
 #pragma unroll
-        for (int u = 0; u < CLIP_UNITS; ++u) load8(p, kind, vec, at + u * (CLIP_THREADS * 8), n, v[u]);
+            for (int u = 0; u < U; ++u) q[u] = load_piece(p, kind, vec, at + u * CLIP_THREADS * per, n);
+            float s[U / 2];
+            bool fits = true;
 #pragma unroll
-        for (int u = 0; u < CLIP_UNITS; ++u) {
-            float s = 0.f;
+            for (int u = 0; u < U; u += 2) {
+                float a = 0.f, b = 0.f, v[8];
+                widen(q[u], kind, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = fmaf(v[u][e], v[u][e], s);
-            if (s > 1e-30f && s < 1e37f) acc += s;
-            else {
+                for (int e = 0; e < 8; ++e) a = fmaf(v[e], v[e], a);
+                widen(q[u + 1], kind, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc += double(v[u][e]) * v[u][e];
+                for (int e = 0; e < 8; ++e) b = fmaf(v[e], v[e], b);
+                s[u / 2] = a + b;
+                fits = fits && a > 1e-30f && b > 1e-30f && a + b < 1e37f;
+            }
+            if (__all_sync(0xFFFFFFFFu, fits)) {
+#pragma unroll
+                for (int u = 0; u < U / 2; ++u) acc += s[u];
+            } else {
+                const unsigned size = kind == DS_T_F32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+#pragma unroll 1
+                for (int u = 0; u < U; ++u) {
+                    const uint4 w = load_piece(p, kind, vec, at + u * CLIP_THREADS * per, n);
+                    if (((w.x | w.y | w.z | w.w) & size) == 0) continue;
+                    float v[8];
+                    widen(w, kind, v);
+#pragma unroll 1
+                    for (int e = 0; e < 8; ++e) acc += double(v[e]) * v[e];
+                }
             }
         }
     }
@@ -160,7 +192,7 @@ __device__ __forceinline__ float total_norm(const double* __restrict__ partial, 
     return float(sqrt(cta_sum(s)));
 }
 
-template <int CAP>
+template <int CAP, int U>
 __global__ void __launch_bounds__(CLIP_THREADS) scale_kernel(const __grid_constant__ ClipTable<CAP> t, const double* __restrict__ partial,
                                                              int partials, float max_norm, float* __restrict__ norm)
 {
@@ -172,17 +204,22 @@ __global__ void __launch_bounds__(CLIP_THREADS) scale_kernel(const __grid_consta
         const int chunk = t.first[t.count] - 1 - c;
         const int i = tensor_of(t, chunk);
         if (f == 1.f && t.src[i] == t.dst[i]) continue;
+        const int kind = t.kind[i] & 3, per = per_piece(kind), to = t.kind[i] >> 2 & 3;
         const bool vec = t.kind[i] & 16;
         const long long n = t.n[i];
-        const long long at = (long long)(chunk - t.first[i]) * CLIP_CHUNK + threadIdx.x * 8;
-        float v[CLIP_UNITS][8];
+        long long at = ((long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS + threadIdx.x) * per;
+        for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
+            uint4 q[U];
 #pragma unroll
-        for (int u = 0; u < CLIP_UNITS; ++u) load8(t.src[i], t.kind[i] & 3, vec, at + u * (CLIP_THREADS * 8), n, v[u]);
+            for (int u = 0; u < U; ++u) q[u] = load_piece(t.src[i], kind, vec, at + u * CLIP_THREADS * per, n);
 #pragma unroll
-        for (int u = 0; u < CLIP_UNITS; ++u) {
+            for (int u = 0; u < U; ++u) {
+                float v[8];
+                widen(q[u], kind, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[u][e] *= f;
-            store8(t.dst[i], t.kind[i] >> 2 & 3, vec, at + u * (CLIP_THREADS * 8), n, v[u]);
+                for (int e = 0; e < 8; ++e) v[e] *= f;
+                store_piece(t.dst[i], to, vec, at + u * CLIP_THREADS * per, n, per, v);
+            }
         }
     }
 }
@@ -193,12 +230,18 @@ __global__ void __launch_bounds__(CLIP_THREADS) norm_only_kernel(const double* _
     if (threadIdx.x == 0) *norm = all;
 }
 
+int type_bytes(int type) { return type == DS_T_F32 ? 4 : 2; }
+
+// Chunks of a tensor whose chunks take `bytes`.
+long long chunks_of(const ds_tensor_t& a, long long bytes) { return (a.n * type_bytes(a.src_type) + bytes - 1) / bytes; }
+
 // Fills a table from tensors[0 .. count) and returns its chunks.
 template <int CAP>
-int fill(ClipTable<CAP>& t, const ds_tensor_t* tensors, int count)
+int fill(ClipTable<CAP>& t, const ds_tensor_t* tensors, int count, int steps, int bytes)
 {
     t.count = 0;
     t.first[0] = 0;
+    t.steps = steps;
     for (int i = 0; i < count; ++i) {
         const ds_tensor_t& a = tensors[i];
         if (a.n == 0) continue;
@@ -208,30 +251,30 @@ int fill(ClipTable<CAP>& t, const ds_tensor_t* tensors, int count)
         t.n[k] = a.n;
         const bool vec = ((reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst)) & 15) == 0;
         t.kind[k] = (unsigned char)(a.src_type | a.dst_type << 2 | (vec ? 16 : 0));
-        t.first[k + 1] = t.first[k] + int((a.n + CLIP_CHUNK - 1) / CLIP_CHUNK);
+        t.first[k + 1] = t.first[k] + int(chunks_of(a, bytes));
     }
     return t.first[t.count];
 }
 
 int ctas(int chunks) { return chunks < CLIP_CTAS ? chunks : CLIP_CTAS; }
 
-template <int CAP>
-int run(const ds_tensor_t* tensors, int count, float max_norm, float* norm, double* partial, cudaStream_t st, bool scale)
+template <int CAP, int U>
+int run(const ds_tensor_t* tensors, int count, int steps, float max_norm, float* norm, double* partial, cudaStream_t st, bool scale)
 {
     ClipTable<CAP> t;
-    int partials = 0;
+    int partials = 0, chunks = 0;
     for (int at = 0; at < count; at += CAP) {
-        const int chunks = fill(t, tensors + at, count - at < CAP ? count - at : CAP);
+        chunks = fill(t, tensors + at, count - at < CAP ? count - at : CAP, steps, steps * U * CLIP_STEP);
         if (!chunks) continue;
-        norm_kernel<CAP><<<ctas(chunks), CLIP_THREADS, 0, st>>>(t, partial + partials);
+        norm_kernel<CAP, U><<<ctas(chunks), CLIP_THREADS, 0, st>>>(t, partial + partials);
         note_launch();
         partials += ctas(chunks);
     }
     bool written = false;
     for (int at = 0; scale && at < count; at += CAP) {
-        const int chunks = fill(t, tensors + at, count - at < CAP ? count - at : CAP);
+        if (count > CAP) chunks = fill(t, tensors + at, count - at < CAP ? count - at : CAP, steps, steps * U * CLIP_STEP);
         if (!chunks) continue;
-        scale_kernel<CAP><<<ctas(chunks), CLIP_THREADS, 0, st>>>(t, partial, partials, max_norm, written ? nullptr : norm);
+        scale_kernel<CAP, U><<<ctas(chunks), CLIP_THREADS, 0, st>>>(t, partial, partials, max_norm, written ? nullptr : norm);
         note_launch();
         written = true;
     }
@@ -240,6 +283,15 @@ int run(const ds_tensor_t* tensors, int count, float max_norm, float* norm, doub
         note_launch();
     }
     return cudaGetLastError() == cudaSuccess ? DS_OK : DS_ERR_CUDA;
+}
+
+// Four pieces a thread and small chunks where all gradients together would not give every SM a few of the larger ones; then eight pieces, and
+// chunks of up to four such steps, so that finding a chunk's tensor (a search in the table) stays small.
+template <int CAP>
+int run(const ds_tensor_t* tensors, int count, long long bytes, float max_norm, float* norm, double* partial, cudaStream_t st, bool scale)
+{
+    if (bytes < 148ll * 4 * 8 * CLIP_STEP) return run<CAP, 4>(tensors, count, 1, max_norm, norm, partial, st, scale);
+    return run<CAP, 8>(tensors, count, bytes < 148ll * 64 * 8 * CLIP_STEP ? 1 : 4, max_norm, norm, partial, st, scale);
 }
 
 constexpr int CAP_FEW = 32, CAP_MANY = 512;
@@ -261,20 +313,21 @@ extern "C" int ds_clip_norm(const ds_tensor_t* tensors, int count, float max_nor
     if (scratch_bytes < ds_clip_bytes(count)) return DS_ERR_SCRATCH;
     if (reinterpret_cast<uintptr_t>(scratch) & 7) return DS_ERR_ALIGN;
     int with = 0, without = 0;   // tensors that have somewhere to go, and that have not: all or none
-    long long chunks = 0;
+    long long bytes = 0, chunks = 0;
     for (int i = 0; i < count; ++i) {
         const ds_tensor_t& a = tensors[i];
         if (a.n < 0 || (a.n && !a.src)) return DS_ERR_BAD_ARG;
         if (a.src_type < 0 || a.src_type > DS_T_F16 || a.dst_type < 0 || a.dst_type > DS_T_F16) return DS_ERR_UNSUPPORTED;
         if (a.n > 1ll << 42) return DS_ERR_RANGE;
         if (a.n) ++(a.dst ? with : without);
-        chunks += (a.n + ds::CLIP_CHUNK - 1) / ds::CLIP_CHUNK;
+        bytes += a.n * ds::type_bytes(a.src_type);
+        chunks += ds::chunks_of(a, 4 * ds::CLIP_STEP);
     }
     if (with && without) return DS_ERR_BAD_ARG;
     if (chunks >= 1ll << 30) return DS_ERR_RANGE;   // chunks are counted in 32 bits
     const bool scale = with > 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     double* partial = static_cast<double*>(scratch);
-    return count <= ds::CAP_FEW ? ds::run<ds::CAP_FEW>(tensors, count, max_norm, norm, partial, st, scale)
-                                : ds::run<ds::CAP_MANY>(tensors, count, max_norm, norm, partial, st, scale);
+    return count <= ds::CAP_FEW ? ds::run<ds::CAP_FEW>(tensors, count, bytes, max_norm, norm, partial, st, scale)
+                                : ds::run<ds::CAP_MANY>(tensors, count, bytes, max_norm, norm, partial, st, scale);
 }

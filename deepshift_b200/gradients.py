@@ -5,14 +5,18 @@
 ``torch.nn.utils.clip_grad_norm_`` with the 2-norm.  Two kernels for up to 512 tensors.  The sums are formed in a fixed order:
 the same gradients give the same norm, bit for bit.  No counterpart in the reference.
 """
-import ctypes
 import math
+from array import array
 
 import torch
 
 from . import _ffi
 from .adapters import TYPES
-from .kernels import _stream_ptr
+
+
+def _on(index):
+    """A test for dense tensors on the GPU of that index."""
+    return lambda t: t.get_device() == index and t.layout is torch.strided
 
 
 def _flat(t):
@@ -27,43 +31,47 @@ def _flat(t):
     return True
 
 
-def _run(tensors, to, max_norm, what):
-    """One call of the library; ``to``: None for the norm alone."""
-    device = tensors[0].device
-    if device.type != "cuda":
+def _run(tensors, to, max_norm):
+    """One call of the library; ``to``: None for the norm alone.  Properties are read a list at a time: there may be hundreds of
+    tensors, and each microsecond a tensor would count."""
+    device = tensors[0].get_device() if tensors[0].is_cuda else -1
+    if device < 0:
         raise RuntimeError("gradients must be CUDA tensors")
-    table, places = [], set()
-    for i, t in enumerate(tensors):
-        if t.layout is not torch.strided or t.dtype not in TYPES:
-            raise RuntimeError("gradients must be dense, float32, bfloat16 or float16, got %s" % t.dtype)
-        if t.device != device:
-            raise RuntimeError("all gradients must be on one device")
-        if not _flat(t):
-            raise RuntimeError("a gradient must fill its memory without gaps")
-        n, kind = t.numel(), TYPES[t.dtype]
-        if to is None:
-            table += (t.data_ptr(), 0, n, kind)
-            continue
-        o = to[i]
-        if o is not t:
-            if o.dtype not in TYPES or o.device != device:
+    if not all(map(_on(device), tensors)):
+        raise RuntimeError("all gradients must be dense and on one GPU")
+    count = len(tensors)
+    kinds = [TYPES.get(t.dtype, -1) for t in tensors]
+    if -1 in kinds:
+        raise RuntimeError("gradients must be float32, bfloat16 or float16")
+    whole = all(map(torch.Tensor.is_contiguous, tensors))
+    if not whole and not all(map(_flat, tensors)):
+        raise RuntimeError("a gradient must fill its memory without gaps")
+    table = array("q", bytes(32 * count))   # ds_tensor_t: source, place, elements, and both types in one word
+    at = list(map(torch.Tensor.data_ptr, tensors))
+    n = list(map(torch.Tensor.numel, tensors))
+    table[0::4], table[2::4] = array("q", at), array("q", n)
+    if to is not None:
+        if to is not tensors:
+            if not all(map(_on(device), to)) or not all(o.dtype in TYPES for o in to):
                 raise RuntimeError("out must be float32, bfloat16 or float16, on the gradients' device")
-            if o.shape != t.shape or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous())):
+            if [o.shape for o in to] != [t.shape for t in tensors] or not (
+                    whole and all(map(torch.Tensor.is_contiguous, to)) or [o.stride() for o in to] == [t.stride() for t in tensors]):
                 raise RuntimeError("out must have the shapes and layouts of the gradients")
-        at = o.data_ptr()
-        if n:
-            if at in places:
+            at = list(map(torch.Tensor.data_ptr, to))
+            kinds = [k | TYPES[o.dtype] << 32 for k, o in zip(kinds, to)]
+        else:
+            kinds = [k | k << 32 for k in kinds]
+        table[1::4] = array("q", at)
+        # every place is written by itself; empty tensors have none
+        if len(set(at)) < count:
+            places = [p for p, e in zip(at, n) if e]
+            if len(set(places)) < len(places):
                 raise RuntimeError("the same memory twice among the places that are written")
-            places.add(at)
-        table += (t.data_ptr(), at, n, kind | TYPES[o.dtype] << 32)
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    lib = _ffi.lib()
-    nbytes = lib.ds_clip_bytes(len(tensors))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    with torch.cuda.device(device):
-        # an entry of ds_tensor_t is four words: the last holds both types
-        _ffi.check(lib.ds_clip_norm((ctypes.c_int64 * len(table))(*table), len(tensors), max_norm, norm.data_ptr(),
-                                    scratch.data_ptr(), nbytes, _stream_ptr(device)), what)
+    table[3::4] = array("q", kinds)
+    norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+    nbytes = _ffi.lib().ds_clip_bytes(count)
+    scratch = norm.new_empty(nbytes, dtype=torch.uint8)
+    _ffi.run("ds_clip_norm", device, table.buffer_info()[0], count, max_norm, norm.data_ptr(), scratch.data_ptr(), nbytes)
     return norm
 
 
@@ -81,13 +89,13 @@ def clip_norm(tensors, max_norm, out=None):
     to = tensors if out is None else list(out)
     if len(to) != len(tensors):
         raise RuntimeError("%d tensors and %d places for them" % (len(tensors), len(to)))
-    return _run(tensors, to, max_norm, "clip_norm") if tensors else torch.zeros(())
+    return _run(tensors, to, max_norm) if tensors else torch.zeros(())
 
 
 def global_norm(tensors):
     """The norm of all ``tensors`` together, as ``clip_norm`` forms it; changes nothing."""
     tensors = list(tensors)
-    return _run(tensors, None, math.inf, "global_norm") if tensors else torch.zeros(())
+    return _run(tensors, None, math.inf) if tensors else torch.zeros(())
 
 
 def clip_grad_norm_(parameters, max_norm):

@@ -9,7 +9,6 @@ No counterpart in the reference.
 import torch
 
 from . import _ffi
-from .kernels import _stream_ptr
 
 _TYPES = {torch.bfloat16: _ffi.T_BF16, torch.float16: _ffi.T_F16}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -22,70 +21,59 @@ def _check(hidden, weight, target, reduction):
         raise ValueError("reduction must be none, mean or sum, got %r" % (reduction,))
     if not hidden.is_cuda:
         raise RuntimeError("hidden must be a CUDA tensor")
-    if hidden.dtype not in _TYPES or weight.dtype != hidden.dtype:
+    if hidden.dtype not in _TYPES or weight.dtype is not hidden.dtype:
         raise RuntimeError("hidden and weight must both be bfloat16 or float16, got %s and %s" % (hidden.dtype, weight.dtype))
-    if hidden.dim() < 1 or weight.dim() != 2 or hidden.size(-1) != weight.size(1):
-        raise RuntimeError("hidden must be [..., d] and weight [v, d], got %s and %s" % (tuple(hidden.shape), tuple(weight.shape)))
-    if target.shape != hidden.shape[:-1] or target.dtype not in (torch.int64, torch.int32):
-        raise RuntimeError("target must be int64 %s, got %s of %s" % (tuple(hidden.shape[:-1]), target.dtype, tuple(target.shape)))
-    if weight.device != hidden.device or target.device != hidden.device:
+    shape = hidden.shape
+    if not shape or weight.dim() != 2 or shape[-1] != weight.shape[1]:
+        raise RuntimeError("hidden must be [..., d] and weight [v, d], got %s and %s" % (tuple(shape), tuple(weight.shape)))
+    if target.shape != shape[:-1] or target.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError("target must be int64 %s, got %s of %s" % (tuple(shape[:-1]), target.dtype, tuple(target.shape)))
+    device = hidden.get_device()
+    if weight.get_device() != device or target.get_device() != device:
         raise RuntimeError("hidden, weight and target must be on one device")
-    v, d = weight.shape
-    if target.numel() > MAX_ROWS or not 1 <= d <= MAX_WIDTH or not 1 <= v <= MAX_VOCABULARY:
+    (v, d), n = weight.shape, target.numel()
+    if n > MAX_ROWS or not 1 <= d <= MAX_WIDTH or not 1 <= v <= MAX_VOCABULARY:
         raise RuntimeError("at most %d rows of 1 .. %d and a vocabulary of 1 .. %d, got %d, %d and %d"
-                           % (MAX_ROWS, MAX_WIDTH, MAX_VOCABULARY, target.numel(), d, v))
+                           % (MAX_ROWS, MAX_WIDTH, MAX_VOCABULARY, n, d, v))
 
 
-def _call(hidden, weight, target, ignore_index, reduction, backward):
-    """The structure of a call, and its scratch."""
-    a = _ffi.Loss()
-    a.rows, a.d, a.v = hidden.size(0), weight.size(1), weight.size(0)
-    a.type, a.reduction, a.ignore_index = _TYPES[hidden.dtype], reduction, ignore_index
-    a.hidden, a.weight, a.target = hidden.data_ptr(), weight.data_ptr(), target.data_ptr()
-    n = _ffi.lib().ds_loss_bytes(a.rows, a.d, a.v, backward, int(bool((a.hidden or 0) & 15 or a.weight & 15)))
-    scratch = torch.empty(n, dtype=torch.uint8, device=hidden.device)
-    a.scratch, a.scratch_bytes = scratch.data_ptr(), n
-    return a, scratch
+def _call(name, hidden, weight, target, ignore_index, reduction, each=0, lse=0, loss=0, count=0, grad=0, dhidden=0, dweight=0):
+    """One call of the library, with its scratch."""
+    rows, (v, d), at_h, at_w, device = hidden.shape[0], weight.shape, hidden.data_ptr(), weight.data_ptr(), hidden.get_device()
+    n = _ffi.lib().ds_loss_bytes(rows, d, v, name == "ds_loss_backward", int((at_h | at_w) & 15 != 0))
+    scratch = hidden.new_empty(n, dtype=torch.uint8)
+    _ffi.run(name, device, _ffi.pack_loss(rows, d, v, _TYPES[hidden.dtype], reduction, at_h, at_w, target.data_ptr(), ignore_index, each, lse, loss, count,
+                                          grad, dhidden, dweight, scratch.data_ptr(), n))
 
 
 def _forward(hidden, weight, target, ignore_index, reduction):
-    a, scratch = _call(hidden, weight, target, ignore_index, reduction, 0)
-    each, lse = torch.empty((2, a.rows), dtype=torch.float32, device=hidden.device).unbind()
-    whole = torch.empty(2, dtype=torch.float32, device=hidden.device) if reduction else None
-    a.each, a.lse = each.data_ptr(), lse.data_ptr()
-    if reduction:
-        a.loss, a.count = whole.data_ptr(), whole.data_ptr() + 4
-    with torch.cuda.device(hidden.device):
-        _ffi.check(_ffi.lib().ds_loss_forward(a, _stream_ptr(hidden.device)), "linear_cross_entropy")
-    return each, lse, whole
+    """Losses and log-sum-exps of the rows [2, rows], and their sum or mean and the number that it is over."""
+    rows = hidden.shape[0]
+    out = hidden.new_empty(2 * rows + 2, dtype=torch.float32)
+    at = out.data_ptr()
+    _call("ds_loss_forward", hidden, weight, target, ignore_index, reduction, at, at + 4 * rows, at + 8 * rows, at + 8 * rows + 4)
+    return out
 
 
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        each, lse, whole = _forward(hidden, weight, target, ignore_index, reduction)
-        ctx.save_for_backward(hidden, weight, target, lse, whole)
+        out = _forward(hidden, weight, target, ignore_index, reduction)
+        rows = hidden.shape[0]
+        ctx.save_for_backward(hidden, weight, target, out)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        return whole[0] if reduction else each.clone()
+        return out[2 * rows].clone() if reduction else out[:rows].clone()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, target, lse, whole = ctx.saved_tensors
+        hidden, weight, target, out = ctx.saved_tensors
         grad = grad.contiguous()
-        a, scratch = _call(hidden, weight, target, ctx.ignore_index, ctx.reduction, 1)
-        a.lse, a.grad = lse.data_ptr(), grad.data_ptr()
-        if ctx.reduction:
-            a.count = whole.data_ptr() + 4
-        dhidden = dweight = None
-        if ctx.needs_input_grad[0]:
-            dhidden = torch.empty_like(hidden)
-            a.dhidden = dhidden.data_ptr()
-        if ctx.needs_input_grad[1]:
-            dweight = torch.empty_like(weight)
-            a.dweight = dweight.data_ptr()
-        with torch.cuda.device(hidden.device):
-            _ffi.check(_ffi.lib().ds_loss_backward(a, _stream_ptr(hidden.device)), "linear_cross_entropy (backward)")
+        rows, at = hidden.shape[0], out.data_ptr()
+        dhidden = torch.empty_like(hidden) if ctx.needs_input_grad[0] else None
+        dweight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        _call("ds_loss_backward", hidden, weight, target, ctx.ignore_index, ctx.reduction, lse=at + 4 * rows, count=at + 8 * rows + 4,
+              grad=grad.data_ptr(), dhidden=dhidden.data_ptr() if dhidden is not None else 0, dweight=dweight.data_ptr() if dweight is not None else 0)
         return dhidden, dweight, None, None, None
 
 
@@ -100,12 +88,12 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     _check(hidden, weight, target, reduction)
     code = _REDUCTIONS[reduction]
     shape = target.shape
-    rows = hidden.reshape(-1, hidden.size(-1)).contiguous()
-    weight = weight.contiguous()
-    flat = target.reshape(-1).to(torch.int64).contiguous()
+    rows = hidden if hidden.dim() == 2 and hidden.is_contiguous() else hidden.reshape(-1, hidden.size(-1)).contiguous()
+    weight = weight if weight.is_contiguous() else weight.contiguous()
+    flat = target if target.dtype is torch.int64 and target.dim() == 1 and target.is_contiguous() else target.reshape(-1).to(torch.int64).contiguous()
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         loss = _Loss.apply(rows, weight, flat, int(ignore_index), code)
     else:
-        each, _, whole = _forward(rows, weight, flat, int(ignore_index), code)
-        loss = whole[0] if code else each
-    return loss if code else loss.view(shape)
+        out, n = _forward(rows, weight, flat, int(ignore_index), code), rows.shape[0]
+        loss = out[2 * n] if code else out[:n]
+    return loss if code or shape == loss.shape else loss.view(shape)

@@ -13,7 +13,6 @@ Rows are sorted by adapter once a batch (``plan_rows``), on the GPU and without 
 layer and both directions.  All calls run on torch's current stream of their tensors' device; scratch comes from torch's
 allocator.  No counterpart in the reference.
 """
-import functools
 import math
 
 import torch
@@ -62,11 +61,6 @@ def plan_rows(ids, count, device=None):
     data = torch.empty(n // 4, dtype=torch.int32, device=ids.device)
     _ffi.run("ds_rows_plan", ids.get_device(), ids.data_ptr(), ids.numel(), count, data.data_ptr(), n)
     return RowPlan(ids.numel(), count, data)
-
-
-@functools.lru_cache(maxsize=4096)
-def _h_bytes(rows, width, rank, count, act, weight):
-    return _ffi.lib().ds_adapters_h_bytes(rows, width, rank, count, act, weight)
 
 
 def _rows(t, name, width, dtype, device):
@@ -136,7 +130,7 @@ def _forward(x, down, up, scale, plan, base, out):
         base_at, base_stride = add.data_ptr(), add.stride(0)
         if base_at == to.data_ptr() and base_stride != to_stride:
             raise RuntimeError("base and out overlap")
-    nbytes = _h_bytes(m, k, rank, count, act, weight)
+    nbytes = 4 * m * ((rank + 7) // 8 * 8)   # ds_adapters_h_bytes
     h = x.new_empty(nbytes // 4, dtype=torch.float32)
     _ffi.run("ds_adapters_apply", device, _ffi.pack_adapters(
         m, k, n, rank, count, act, weight, plan.data.data_ptr(), down.data_ptr(), up.data_ptr(), scale.data_ptr() if scale is not None else 0,
@@ -168,11 +162,11 @@ class _Apply(torch.autograd.Function):
             dx = x.new_empty(x.shape) if need_x else None
             ddown = torch.empty_like(down) if need_down else None
             dup = torch.empty_like(up) if need_up else None
-            nbytes = _h_bytes(m, n, rank, count, act, weight)
-            dh = h.new_empty(nbytes // 4)
+            nbytes = 4 * h.numel()
+            dh = torch.empty_like(h)
             _ffi.run("ds_adapters_backward", device, _ffi.pack_adapters(
                 m, k, n, rank, count, act, weight, plan.data.data_ptr(), down.data_ptr(), up.data_ptr(), scale.data_ptr() if scale is not None else 0,
-                rows.data_ptr(), rows.stride(0), 0, 0, 0, 0, h.data_ptr(), 4 * h.numel(), g.data_ptr(), g.stride(0),
+                rows.data_ptr(), rows.stride(0), 0, 0, 0, 0, h.data_ptr(), nbytes, g.data_ptr(), g.stride(0),
                 dx.data_ptr() if need_x else 0, k, ddown.data_ptr() if need_down else 0, dup.data_ptr() if need_up else 0, dh.data_ptr(), nbytes))
         return dx, ddown, dup, None, None, grad if need_base else None
 

@@ -136,13 +136,12 @@ bool aligned(const void* p, long long stride, int type)
 }
 
 // CTAs a tile's sums are shared by: until there are two for each SM, as long as every warp keeps a piece of its own.
-int splits_of(int rows, int width, int rank, int count, bool same16)
+int splits_of(const Args& a, int rank_blocks, int pieces)
 {
-    const long long tiles = plan_tiles(rows, count) * (same16 ? (rank + 63) / 64 : (rank + 31) / 32);
-    const int pieces = (width + (same16 ? 31 : 15)) / (same16 ? 32 : 16) / WARPS;
-    long long s = 296 / (tiles < 1 ? 1 : tiles);   // no rows, no tiles
-    if (s > pieces) s = pieces;
-    return s < 1 ? 1 : s > 16 ? 16 : int(s);
+    const long long ctas = plan_tiles(a.rows, a.count) * rank_blocks;
+    int s = 1;
+    while (s < 8 && ctas * s * 2 <= 296 && pieces >= 2 * s * WARPS) s *= 2;
+    return s;
 }
 
 int finish()
@@ -164,15 +163,31 @@ bool allow_smem(int bytes)
     return true;
 }
 
+template <auto KERNEL>
+int launch_cluster(dim3 grid, dim3 cluster, int smem, const Args& a, cudaStream_t st)
+{
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim = {cluster.x, cluster.y, cluster.z};
+    c.attrs = &attribute;
+    c.numAttrs = 1;
+    if (cudaLaunchKernelEx(&c, KERNEL, a) != cudaSuccess) return DS_ERR_CUDA;
+    return finish();
+}
+
 template <class X, class W, int MT, int NT, bool VEC>
 int launch_down(const Args& a, cudaStream_t st)
 {
     constexpr int smem = Down<X, W, MT, NT>::smem(VEC);
     static_assert(smem <= 227 * 1024, "shared memory of an SM");
     if (!allow_smem<down_kernel<X, W, MT, NT, VEC>>(smem)) return DS_ERR_CUDA;
-    const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), a.splits, (a.rank8 + 8 * NT - 1) / (8 * NT));
-    down_kernel<X, W, MT, NT, VEC><<<grid, THREADS, smem, st>>>(a);
-    return finish();
+    const int blocks = (a.rank8 + 8 * NT - 1) / (8 * NT), chunk = 4 * Down<X, W, MT, NT>::LK, shares = splits_of(a, blocks, (a.width + chunk - 1) / chunk);
+    return launch_cluster<down_kernel<X, W, MT, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), smem, a, st);
 }
 
 // Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere, where 64 would not fit the
@@ -241,18 +256,7 @@ int launch_grad(const Args& a, cudaStream_t st)
     // rows spread evenly
     int shares = 1;
     while (shares < 8 && (long long)columns * a.count * blocks * shares < 296 && a.rows / a.count >= 2 * shares * 2 * block) shares *= 2;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(a.count * blocks, columns, shares);
-    c.blockDim = dim3(THREADS);
-    c.dynamicSmemBytes = smem;
-    c.stream = st;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim = {1, 1, unsigned(shares)};
-    c.attrs = &cluster;
-    c.numAttrs = 1;
-    if (cudaLaunchKernelEx(&c, grad_kernel<X, W, RT, CW, VEC>, a) != cudaSuccess) return DS_ERR_CUDA;
-    return finish();
+    return launch_cluster<grad_kernel<X, W, RT, CW, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), smem, a, st);
 }
 
 template <class X, class W, int RT, bool VEC>
@@ -300,8 +304,8 @@ int check(const ds_adapters_t* a, bool backward)
     if (backward ? (a->rows && (!a->grad || !a->dh)) : (a->rows && !a->out)) return DS_ERR_BAD_ARG;
     if (reinterpret_cast<uintptr_t>(a->plan) & 15 || reinterpret_cast<uintptr_t>(a->h) & 15 || reinterpret_cast<uintptr_t>(a->dh) & 15)
         return DS_ERR_ALIGN;
-    if (a->h_bytes < ds_adapters_h_bytes(a->rows, a->k, a->rank, a->count, a->act_type, a->weight_type)) return DS_ERR_SCRATCH;
-    if (backward && a->dh_bytes < ds_adapters_h_bytes(a->rows, a->n, a->rank, a->count, a->act_type, a->weight_type)) return DS_ERR_SCRATCH;
+    const long long need = ds_adapters_h_bytes(a->rows, a->rank);
+    if (a->h_bytes < need || (backward && a->dh_bytes < need)) return DS_ERR_SCRATCH;
     return DS_OK;
 }
 
@@ -319,7 +323,6 @@ Args down_args(const ds_adapters_t* a, const void* x, long long ldx, const void*
 {
     Args p = common(a);
     p.x = x, p.ldx = ldx, p.w = w, p.width = width, p.h = h;
-    p.splits = splits_of(a->rows, width, a->rank, a->count, a->act_type != DS_T_F32 && a->act_type == a->weight_type);
     return p;
 }
 
@@ -346,11 +349,10 @@ extern "C" int ds_rows_plan(const int32_t* ids, int rows, int count, int32_t* pl
     return finish();
 }
 
-extern "C" long long ds_adapters_h_bytes(int rows, int width, int rank, int count, int act_type, int weight_type)
+extern "C" long long ds_adapters_h_bytes(int rows, int rank)
 {
-    using namespace ds::adapters;
-    if (rows < 0 || width < 1 || rank < 1 || count < 1) return -1;
-    return (long long)splits_of(rows, width, rank, count, act_type != DS_T_F32 && act_type == weight_type) * rows * rank8(rank) * 4;
+    if (rows < 0 || rank < 1) return -1;
+    return (long long)rows * ds::adapters::rank8(rank) * 4;
 }
 
 extern "C" int ds_adapters_apply(const ds_adapters_t* a, void* stream)
@@ -397,8 +399,8 @@ extern "C" int ds_adapters_backward(const ds_adapters_t* a, void* stream)
             if (const int e = grad<X, W>(p, vec_k && aligned(a->ddown, a->k, a->weight_type), st)) return e;
         }
         if (a->dup) {
-            Args p = down_args(a, a->grad, a->grad_stride, nullptr, a->k, a->h);   // the forward's h, its splits those of k
-            p.width = a->n, p.out = a->dup;
+            Args p = down_args(a, a->grad, a->grad_stride, nullptr, a->n, a->h);   // the forward's h
+            p.out = a->dup;
             if (const int e = grad<X, W>(p, vec_n && aligned(a->dup, a->n, a->weight_type), st)) return e;
         }
         return int(DS_OK);

@@ -54,12 +54,12 @@ struct Args {
     long long ldx;
     const void* w;        // [count][rank][width]
     const float* scale;   // [count] or null
-    float* h;             // [splits][rows][rank8], rank8 = rank to the next multiple of 8, zeros behind rank
+    float* h;             // [rows][rank8], rank8 = rank to the next multiple of 8, zeros behind rank
     const void* base;     // [rows][ldbase] or null
     long long ldbase;
     void* out;            // [rows][ldout], or a gradient [count][rank][width]
     long long ldout;
-    int rows, width, rank, rank8, count, splits;
+    int rows, width, rank, rank8, count;
 };
 
 using bf16 = __nv_bfloat16;
@@ -274,8 +274,23 @@ __device__ __forceinline__ void down_step(float (&acc)[MT][NT][4], const float (
     }
 }
 
-// h for one tile of 16 MT rows: a CTA's warps share the summed index out among them, and so do `splits` CTAs (blockIdx.y),
-// each of which writes its own partial sums.  blockIdx.z: ranks by 8 NT.
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Four consecutive sums of CTA `rank` of the cluster at the place of `here` in its shared memory.
+__device__ __forceinline__ float4 sums_of(const float* here, int rank)
+{
+    unsigned at;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_address(here)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+// h for one tile of 16 MT rows: a CTA's warps share the summed index out among them, and so do the `gridDim.y` CTAs of a cluster,
+// which add up their sums over distributed shared memory, in their order.  blockIdx.z: ranks by 8 NT.
 template <class X, class W, int MT, int NT, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
 {
@@ -298,7 +313,7 @@ __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
         xr[i] = m < 0 ? nullptr : static_cast<const X*>(p.x) + m * p.ldx + t * LK;
     }
     float acc[MT][NT][4] = {};
-    const int chunks = (p.width + CHUNK - 1) / CHUNK, workers = WARPS * p.splits, first = blockIdx.y * WARPS + warp;
+    const int chunks = (p.width + CHUNK - 1) / CHUNK, workers = WARPS * gridDim.y, first = blockIdx.y * WARPS + warp;
     if constexpr (VEC) {
         const unsigned mine = shared_address(smem) + threadIdx.x * 16;
         auto issue = [&](int c, int stage) {
@@ -382,29 +397,37 @@ __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
             for (int e = 0; e < 4; ++e)
                 red[(warp * ROWS + 16 * i + g + (e & 2) * 4) * COLS + 8 * j + 2 * t + (e & 1)] = acc[i][j][e];
     __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * COLS; i += THREADS) {
+    const int shares = gridDim.y;
+    if (shares > 1) {
+        for (int i = threadIdx.x; i < ROWS * COLS; i += THREADS) {
+            float s = 0.f;
+#pragma unroll
+            for (int q = 0; q < WARPS; ++q) s += red[q * ROWS * COLS + i];
+            red[i] = s;   // this thread alone reads and writes element i of each
+        }
+        cluster_sync();
+    }
+    for (int i = (blockIdx.y * THREADS + threadIdx.x) * 4; i < ROWS * COLS; i += shares * THREADS * 4) {
         const int row = i / COLS, r = r0 + i % COLS;
         const int m = tile_row(p.plan, tile, row);
         if (m < 0 || r >= p.rank8) continue;
-        float s = 0.f;
+        float s[4] = {};
+        for (int q = 0; q < (shares > 1 ? shares : WARPS); ++q) {
+            const float4 v = shares > 1 ? sums_of(red + i, q) : *reinterpret_cast<const float4*>(red + q * ROWS * COLS + i);
+            s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+        }
 #pragma unroll
-        for (int q = 0; q < WARPS; ++q) s += red[q * ROWS * COLS + i];
-        p.h[((long long)blockIdx.y * p.rows + m) * p.rank8 + r] = r < p.rank ? s : 0.f;
+        for (int e = 0; e < 4; ++e)
+            if (r + e >= p.rank) s[e] = 0.f;
+        *reinterpret_cast<float4*>(p.h + (long long)m * p.rank8 + r) = make_float4(s[0], s[1], s[2], s[3]);
     }
+    if (shares > 1) cluster_sync();   // nobody leaves while its sums are being read
 }
 
-// Four values of h, summed over the splits in their order and scaled; 0 without a row.
-__device__ __forceinline__ float4 load_h4(const Args& p, int m, int r, float scale)
+// Four values of h; 0 without a row.
+__device__ __forceinline__ float4 load_h4(const Args& p, int m, int r)
 {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (m < 0) return s;
-    const float* h = p.h + (long long)m * p.rank8 + r;
-    for (int q = 0; q < p.splits; ++q) {
-        const float4 v = *reinterpret_cast<const float4*>(h + (long long)q * p.rows * p.rank8);
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-    }
-    s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
-    return s;
+    return m < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(p.h + (long long)m * p.rank8 + r);
 }
 
 // The two parts of v at word `at` of a block of 128 words for hi, 128 for lo.
@@ -419,13 +442,13 @@ __device__ __forceinline__ void put_parts(unsigned* at, float v)
 // Values r .. r + 3 (r a multiple of 4) of row `at` of a tile into the order in which the instruction reads its first operand [row][rank]:
 // blocks [rank / 8][halves of 16 rows][hi, lo][lane][4], the lane that holds row at % 8 and rank pair r % 8 / 2, its
 // elements by rows of 8 and then by the pair's second.
-__device__ __forceinline__ void put_h4(unsigned* h, int halves, int at, int r, const float4& v)
+__device__ __forceinline__ void put_h4(unsigned* h, int halves, int at, int r, const float4& v, float scale)
 {
     unsigned* to = h + (r / 8 * halves + at / 16) * 256 + (at % 8 * 4 + r % 8 / 2) * 4 + (at / 8 & 1);
-    put_parts(to, v.x);
-    put_parts(to + 2, v.y);
-    put_parts(to + 4, v.z);
-    put_parts(to + 6, v.w);
+    put_parts(to, v.x * scale);
+    put_parts(to + 2, v.y * scale);
+    put_parts(to + 4, v.z * scale);
+    put_parts(to + 6, v.w * scale);
 }
 
 // One tile of 16 MT rows, 64 columns a warp: lane (g, t) loads eight consecutive columns 8 g .. of ranks 2t and 2t + 1, which are
@@ -463,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
         unsigned* h = reinterpret_cast<unsigned*>(smem);
         constexpr int PER = THREADS / (16 * MT);   // threads a row
         const int at = threadIdx.x / PER, m = tile_row(p.plan, tile, at);
-        for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(h, MT, at, r, load_h4(p, m, r, scale));
+        for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(h, MT, at, r, load_h4(p, m, r), scale);
         __syncthreads();
         const W* w = static_cast<const W*>(p.w) + (long long)tile.x * p.rank * p.width + n0 + 8 * g;
         const int live = p.width - n0 - 8 * g;
@@ -587,13 +610,13 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
     auto fetch_h = [&](const Ahead& n) {
 #pragma unroll
         for (int q = 0; q < HV; ++q)
-            if (h_rank + q * PER * 4 < p.rank8) hv[q] = load_h4(p, n.h_m, h_rank + q * PER * 4, n.scale);
+            if (h_rank + q * PER * 4 < p.rank8) hv[q] = load_h4(p, n.h_m, h_rank + q * PER * 4);   // used, and waited for, in put_h
     };
-    auto put_h = [&](int buf) {
+    auto put_h = [&](const Ahead& n, int buf) {
         unsigned* h = reinterpret_cast<unsigned*>(smem + 2 * S::BASE + buf * S::h_bytes(p.rank8));
 #pragma unroll
         for (int q = 0; q < HV; ++q)
-            if (h_rank + q * PER * 4 < p.rank8) put_h4(h, 2, h_row, h_rank + q * PER * 4, hv[q]);
+            if (h_rank + q * PER * 4 < p.rank8) put_h4(h, 2, h_row, h_rank + q * PER * 4, hv[q], n.scale);
     };
     auto load_w = [&](int adapter) {
         constexpr int PER = 16 / sizeof(W), PIECES = S::COLS / PER;
@@ -614,7 +637,7 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
     int held = -1;   // whose w is in shared memory
     if (now.tile.x < p.count) load_w(held = now.tile.x);
     fetch_h(now);
-    put_h(0);
+    put_h(now, 0);
     copies_wait<0>();
     __syncthreads();
     for (int at = first, buf = 0; at < last; ++at, buf ^= 1) {
@@ -679,7 +702,7 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
             }
         }
         rows_of(then);
-        put_h(buf ^ 1);
+        put_h(next, buf ^ 1);
         if (next.tile.x < p.count && next.tile.x != held) {
             __syncthreads();   // everybody is done with the held one
             load_w(held = next.tile.x);
@@ -733,7 +756,7 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
     };
     auto fetch_h = [&] {
 #pragma unroll
-        for (int q = 0; q < HV; ++q) hv[q] = load_h4(p, h_m[q], r0 + (threadIdx.x + q * THREADS) % (RANKS / 4) * 4, scale);
+        for (int q = 0; q < HV; ++q) hv[q] = load_h4(p, h_m[q], r0 + (threadIdx.x + q * THREADS) % (RANKS / 4) * 4);
     };
     auto put_h = [&](int buf) {   // as put_h4, but of an operand [rank][row]: blocks [row / 8][RT][hi, lo][lane][4]
         unsigned* h = reinterpret_cast<unsigned*>(smem + buf * H_BYTES);
@@ -742,10 +765,10 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
             const int i = threadIdx.x + q * THREADS, r = i % (RANKS / 4) * 4, at = i / (RANKS / 4);
             if (i >= BLOCK * RANKS / 4) continue;
             unsigned* to = h + (at / 8 * RT + r / 16) * 256 + (r % 8 * 4 + at % 8 / 2) * 4 + (r / 8 & 1) + 2 * (at & 1);
-            put_parts(to, hv[q].x);
-            put_parts(to + 16, hv[q].y);
-            put_parts(to + 32, hv[q].z);
-            put_parts(to + 48, hv[q].w);
+            put_parts(to, hv[q].x * scale);
+            put_parts(to + 16, hv[q].y * scale);
+            put_parts(to + 32, hv[q].z * scale);
+            put_parts(to + 48, hv[q].w * scale);
         }
     };
     auto products = [&](const float (&b)[2][NJ], unsigned h) {
@@ -853,7 +876,7 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
                 for (int q = 0; q < RW; ++q) s += red[q * RANKS * COLS + i];
                 red[i] = s;   // this thread alone reads and writes element i of each
             }
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_sync();
     }
     for (int i = (share * THREADS + threadIdx.x) * 8; i < RANKS * COLS; i += shares * THREADS * 8) {
         const int r = r0 + i / COLS, at = blockIdx.y * COLS + i % COLS;
@@ -866,24 +889,15 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
                 for (int e = 0; e < 8; ++e) s[e] += red[q * RANKS * COLS + i + e];
         } else {
             for (int q = 0; q < shares; ++q) {
-                unsigned at_q;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_q) : "r"(shared_address(red + i)), "r"(q));
-#pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    float v[4];
-                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-                                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                                 : "r"(at_q + 4 * e)
-                                 : "memory");
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) s[e + c] += v[c];
-                }
+                const float4 u = sums_of(red + i, q), v = sums_of(red + i + 4, q);
+                s[0] += u.x, s[1] += u.y, s[2] += u.z, s[3] += u.w;
+                s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
             }
         }
         store<W, 8, VEC>(static_cast<W*>(p.out) + ((long long)a * p.rank + r) * p.width + at, p.width - at, s);
     }
     // nobody leaves while its sums are being read
-    if (shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (shares > 1) cluster_sync();
 }
 
 }  // namespace adapters

@@ -25,7 +25,7 @@ struct ClipTable {
     void* dst[CAP];
     long long n[CAP];
     int first[CAP + 1];      // first chunk of each tensor
-    unsigned char kind[CAP]; // type of src, type of dst << 2, 16-byte aligned << 4
+    unsigned char kind[CAP]; // type of src, type of dst << 2, src 16-byte aligned << 4, both << 5
     int count;
     int steps;               // a chunk: this many steps of U pieces a thread
 };
@@ -39,7 +39,17 @@ __device__ __forceinline__ float2 unpack(unsigned v, int kind)
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-// The piece from element `at` of a tensor of n, zeros behind its end.
+// The elements of a thread's piece: `per` consecutive ones from `at`, or, in tensors that are not 16-byte aligned, every CLIP_THREADS-th, so
+// that a warp's accesses lie side by side all the same (one by one and 16 bytes apart they took four times as long).
+__device__ __forceinline__ long long element(bool vec, long long at, int i) { return at + (vec ? i : i * CLIP_THREADS); }
+
+// Where a thread's piece u of a step that begins at element `start` begins.
+__device__ __forceinline__ long long piece_at(bool vec, long long start, int u, int per)
+{
+    return start + (long long)u * CLIP_THREADS * per + (vec ? threadIdx.x * per : threadIdx.x);
+}
+
+// The piece at element `at` of a tensor of n, zeros behind its end.
 __device__ __forceinline__ uint4 load_piece(const void* p, int kind, bool vec, long long at, long long n)
 {
     const int per = per_piece(kind);
@@ -49,11 +59,11 @@ __device__ __forceinline__ uint4 load_piece(const void* p, int kind, bool vec, l
         if (kind == DS_T_F32) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (at + i < n) w[i] = static_cast<const unsigned*>(p)[at + i];
+                if (element(vec, at, i) < n) w[i] = static_cast<const unsigned*>(p)[element(vec, at, i)];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (at + i < n) w[i >> 1] |= unsigned(static_cast<const unsigned short*>(p)[at + i]) << (16 * (i & 1));
+                if (element(vec, at, i) < n) w[i >> 1] |= unsigned(static_cast<const unsigned short*>(p)[element(vec, at, i)]) << (16 * (i & 1));
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
@@ -98,9 +108,10 @@ __device__ __forceinline__ void store_piece(void* p, int kind, bool vec, long lo
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        if (i < per && at + i < n) {
-            if (kind == DS_T_F32) static_cast<float*>(p)[at + i] = v[i];
-            else static_cast<unsigned short*>(p)[at + i] = narrow(v[i], kind);
+        const long long to = element(vec, at, i);
+        if (i < per && to < n) {
+            if (kind == DS_T_F32) static_cast<float*>(p)[to] = v[i];
+            else static_cast<unsigned short*>(p)[to] = narrow(v[i], kind);
         }
     }
 }
@@ -145,11 +156,11 @@ __global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constan
         const bool vec = t.kind[i] & 16;
         const void* p = t.src[i];
         const long long n = t.n[i];
-        long long at = ((long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS + threadIdx.x) * per;
+        long long at = (long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS * per;
         for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
             uint4 q[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = load_piece(p, kind, vec, at + u * CLIP_THREADS * per, n);
+            for (int u = 0; u < U; ++u) q[u] = load_piece(p, kind, vec, piece_at(vec, at, u, per), n);
             float s[U / 2];
             bool fits = true;
 #pragma unroll
@@ -171,7 +182,7 @@ __global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constan
                 const unsigned size = kind == DS_T_F32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
 #pragma unroll 1
                 for (int u = 0; u < U; ++u) {
-                    const uint4 w = load_piece(p, kind, vec, at + u * CLIP_THREADS * per, n);
+                    const uint4 w = load_piece(p, kind, vec, piece_at(vec, at, u, per), n);
                     if (((w.x | w.y | w.z | w.w) & size) == 0) continue;
                     float v[8];
                     widen(w, kind, v);
@@ -205,20 +216,20 @@ __global__ void __launch_bounds__(CLIP_THREADS) scale_kernel(const __grid_consta
         const int i = tensor_of(t, chunk);
         if (f == 1.f && t.src[i] == t.dst[i]) continue;
         const int kind = t.kind[i] & 3, per = per_piece(kind), to = t.kind[i] >> 2 & 3;
-        const bool vec = t.kind[i] & 16;
+        const bool vec = t.kind[i] & 32;
         const long long n = t.n[i];
-        long long at = ((long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS + threadIdx.x) * per;
+        long long at = (long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS * per;
         for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
             uint4 q[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = load_piece(t.src[i], kind, vec, at + u * CLIP_THREADS * per, n);
+            for (int u = 0; u < U; ++u) q[u] = load_piece(t.src[i], kind, vec, piece_at(vec, at, u, per), n);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float v[8];
                 widen(q[u], kind, v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= f;
-                store_piece(t.dst[i], to, vec, at + u * CLIP_THREADS * per, n, per, v);
+                store_piece(t.dst[i], to, vec, piece_at(vec, at, u, per), n, per, v);
             }
         }
     }
@@ -249,8 +260,8 @@ int fill(ClipTable<CAP>& t, const ds_tensor_t* tensors, int count, int steps, in
         t.src[k] = a.src;
         t.dst[k] = a.dst;
         t.n[k] = a.n;
-        const bool vec = ((reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst)) & 15) == 0;
-        t.kind[k] = (unsigned char)(a.src_type | a.dst_type << 2 | (vec ? 16 : 0));
+        const uintptr_t src = reinterpret_cast<uintptr_t>(a.src), dst = reinterpret_cast<uintptr_t>(a.dst);
+        t.kind[k] = (unsigned char)(a.src_type | a.dst_type << 2 | (src & 15 ? 0 : 16) | ((src | dst) & 15 ? 0 : 32));
         t.first[k + 1] = t.first[k] + int(chunks_of(a, bytes));
     }
     return t.first[t.count];

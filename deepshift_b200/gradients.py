@@ -7,6 +7,7 @@ the same gradients give the same norm, bit for bit.  No counterpart in the refer
 """
 import math
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -14,9 +15,7 @@ from . import _ffi
 from .adapters import TYPES
 
 
-def _on(index):
-    """A test for dense tensors on the GPU of that index."""
-    return lambda t: t.get_device() == index and t.layout is torch.strided
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
 
 
 def _flat(t):
@@ -37,12 +36,12 @@ def _run(tensors, to, max_norm):
     device = tensors[0].get_device() if tensors[0].is_cuda else -1
     if device < 0:
         raise RuntimeError("gradients must be CUDA tensors")
-    if not all(map(_on(device), tensors)):
-        raise RuntimeError("all gradients must be dense and on one GPU")
+    if set(map(torch.Tensor.get_device, tensors)) != {device}:
+        raise RuntimeError("all gradients must be on one GPU")
     count = len(tensors)
-    kinds = [TYPES.get(t.dtype, -1) for t in tensors]
-    if -1 in kinds:
-        raise RuntimeError("gradients must be float32, bfloat16 or float16")
+    kinds = list(map(TYPES.get, map(_dtype, tensors)))
+    if None in kinds or any(map(attrgetter("is_sparse"), tensors)):
+        raise RuntimeError("gradients must be dense, float32, bfloat16 or float16")
     whole = all(map(torch.Tensor.is_contiguous, tensors))
     if not whole and not all(map(_flat, tensors)):
         raise RuntimeError("a gradient must fill its memory without gaps")
@@ -52,13 +51,14 @@ def _run(tensors, to, max_norm):
     table[0::4], table[2::4] = array("q", at), array("q", n)
     if to is not None:
         if to is not tensors:
-            if not all(map(_on(device), to)) or not all(o.dtype in TYPES for o in to):
+            places = list(map(TYPES.get, map(_dtype, to)))
+            if set(map(torch.Tensor.get_device, to)) != {device} or None in places:
                 raise RuntimeError("out must be float32, bfloat16 or float16, on the gradients' device")
-            if [o.shape for o in to] != [t.shape for t in tensors] or not (
+            if list(map(_shape, to)) != list(map(_shape, tensors)) or not (
                     whole and all(map(torch.Tensor.is_contiguous, to)) or [o.stride() for o in to] == [t.stride() for t in tensors]):
                 raise RuntimeError("out must have the shapes and layouts of the gradients")
             at = list(map(torch.Tensor.data_ptr, to))
-            kinds = [k | TYPES[o.dtype] << 32 for k, o in zip(kinds, to)]
+            kinds = [k | o << 32 for k, o in zip(kinds, places)]
         else:
             kinds = [k | k << 32 for k in kinds]
         table[1::4] = array("q", at)

@@ -460,20 +460,20 @@ typedef struct {
     long long base_stride;
     void *out;                         /* [rows][n]                                                        */
     long long out_stride;
-    float *h;                          /* ds_adapters_h_bytes(rows, k, ...): written by _apply, read by _backward */
+    float *h;                          /* ds_adapters_h_bytes: written by _apply, read by _backward */
     long long h_bytes;
     const void *grad;                  /* _backward only: gradient of out [rows][n]                        */
     long long grad_stride;
     void *dx;                          /* [rows][k] or NULL                                                */
     long long dx_stride;
     void *ddown, *dup;                 /* gradients of down and up, whole, in weight_type, or NULL         */
-    float *dh;                         /* ds_adapters_h_bytes(rows, n, ...)                                */
+    float *dh;                         /* scratch of the same size                                         */
     long long dh_bytes;
 } ds_adapters_t;
 
 long long ds_rows_plan_bytes(int rows, int count);
 int ds_rows_plan(const int32_t *ids, int rows, int count, int32_t *plan, long long plan_bytes, void *stream);
-long long ds_adapters_h_bytes(int rows, int width, int rank, int count, int act_type, int weight_type);
+long long ds_adapters_h_bytes(int rows, int rank);
 int ds_adapters_apply(const ds_adapters_t *a, void *stream);
 int ds_adapters_backward(const ds_adapters_t *a, void *stream);
 

@@ -163,8 +163,8 @@ bool allow_smem(int bytes)
     return true;
 }
 
-template <auto KERNEL>
-int launch_cluster(dim3 grid, dim3 cluster, int smem, const Args& a, cudaStream_t st)
+template <auto KERNEL, class... A>
+int launch_cluster(dim3 grid, dim3 cluster, int smem, cudaStream_t st, const A&... a)
 {
     cudaLaunchConfig_t c = {};
     c.gridDim = grid;
@@ -176,7 +176,7 @@ int launch_cluster(dim3 grid, dim3 cluster, int smem, const Args& a, cudaStream_
     attribute.val.clusterDim = {cluster.x, cluster.y, cluster.z};
     c.attrs = &attribute;
     c.numAttrs = 1;
-    if (cudaLaunchKernelEx(&c, KERNEL, a) != cudaSuccess) return DS_ERR_CUDA;
+    if (cudaLaunchKernelEx(&c, KERNEL, a...) != cudaSuccess) return DS_ERR_CUDA;
     return finish();
 }
 
@@ -187,7 +187,7 @@ int launch_down(const Args& a, cudaStream_t st)
     static_assert(smem <= 227 * 1024, "shared memory of an SM");
     if (!allow_smem<down_kernel<X, W, MT, NT, VEC>>(smem)) return DS_ERR_CUDA;
     const int blocks = (a.rank8 + 8 * NT - 1) / (8 * NT), chunk = 4 * Down<X, W, MT, NT>::LK, shares = splits_of(a, blocks, (a.width + chunk - 1) / chunk);
-    return launch_cluster<down_kernel<X, W, MT, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), smem, a, st);
+    return launch_cluster<down_kernel<X, W, MT, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), smem, st, a);
 }
 
 // Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere, where 64 would not fit the
@@ -213,8 +213,9 @@ template <class X, class W, int MT, bool VEC>
 int launch_up(const Args& a, cudaStream_t st)
 {
     // h of the tile in two parts, and the base's columns
-    const int smem = a.rank8 * 16 * MT * 8 + (VEC ? THREADS * 16 * 2 * MT * int(sizeof(X)) : 0);
-    if (!allow_smem<up_kernel<X, W, MT, VEC>>(MAX_RANK * 16 * MT * 8 + (VEC ? THREADS * 16 * 2 * MT * int(sizeof(X)) : 0))) return DS_ERR_CUDA;
+    constexpr int rows = VEC ? MT * base_bytes<X> : WARPS * 16 * 65 * 4;
+    const int smem = a.rank8 * 16 * MT * 8 + rows;
+    if (!allow_smem<up_kernel<X, W, MT, VEC>>(MAX_RANK * 16 * MT * 8 + rows)) return DS_ERR_CUDA;
     const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS));
     up_kernel<X, W, MT, VEC><<<grid, THREADS, smem, st>>>(a);
     return finish();
@@ -256,7 +257,7 @@ int launch_grad(const Args& a, cudaStream_t st)
     // rows spread evenly
     int shares = 1;
     while (shares < 8 && (long long)columns * a.count * blocks * shares < 296 && a.rows / a.count >= 2 * shares * 2 * block) shares *= 2;
-    return launch_cluster<grad_kernel<X, W, RT, CW, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), smem, a, st);
+    return launch_cluster<grad_kernel<X, W, RT, CW, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), smem, st, a);
 }
 
 template <class X, class W, int RT, bool VEC>
@@ -272,6 +273,36 @@ int grad(const Args& a, bool vec, cudaStream_t st)
 {
     if (!vec) return launch_grad<X, W, 2, 4, false>(a, st);
     return a.rank <= 16 ? grad_columns<X, W, 1, true>(a, st) : grad_columns<X, W, 2, true>(a, st);
+}
+
+template <class X, class W, int NT, bool VEC>
+int launch_both(const Args& d, const Args& u, cudaStream_t st)
+{
+    constexpr int smem = both_smem<X, W, NT>(VEC);
+    static_assert(smem <= 227 * 1024, "shared memory of an SM");
+    if (!allow_smem<both_kernel<X, W, NT, VEC>>(smem)) return DS_ERR_CUDA;
+    // CTAs a tile: until there are two for each SM, as long as each has 64 columns or a step of every warp's
+    const int steps = (d.width + 4 * Down<X, W, 1, NT>::LK * WARPS - 1) / (4 * Down<X, W, 1, NT>::LK * WARPS), columns = (u.width + 63) / 64;
+    const long long tiles = plan_tiles(d.rows, d.count);
+    int shares = 1;
+    while (shares < 8 && tiles * shares * 2 <= 296 && shares < (steps > columns ? steps : columns)) shares *= 2;
+    return launch_cluster<both_kernel<X, W, NT, VEC>>(dim3(unsigned(tiles), shares), dim3(1, shares, 1), smem, st, d, u);
+}
+
+// h = x down^T and out = base + s h up.  One launch for up to 512 rows, whose tiles are of 16 rows, and up to 64 ranks; two otherwise.
+template <class X, class W>
+int both(const Args& d, bool vec_d, const Args& u, bool vec_u, cudaStream_t st)
+{
+    if (plan_tile_rows(d.rows) == 16 && d.rank8 <= 64) {
+        const bool vec = vec_d && vec_u;
+        if (!vec) return d.rank8 <= 8 ? launch_both<X, W, 1, false>(d, u, st) : launch_both<X, W, 8, false>(d, u, st);
+        if (d.rank8 <= 8) return launch_both<X, W, 1, true>(d, u, st);
+        if (d.rank8 <= 16) return launch_both<X, W, 2, true>(d, u, st);
+        if (d.rank8 <= 32) return launch_both<X, W, 4, true>(d, u, st);
+        return launch_both<X, W, 8, true>(d, u, st);
+    }
+    if (const int e = down<X, W>(d, vec_d, st)) return e;
+    return up<X, W>(u, vec_u, st);
 }
 
 // Calls f(X{}, W{}) with the types of a call.
@@ -364,14 +395,13 @@ extern "C" int ds_adapters_apply(const ds_adapters_t* a, void* stream)
         using X = decltype(x);
         using W = decltype(w);
         if (a->rows == 0) return int(DS_OK);
-        Args p = down_args(a, a->x, a->x_stride, a->down, a->k, a->h);
-        if (const int e = down<X, W>(p, a->k % 8 == 0 && aligned(a->x, a->x_stride, a->act_type) && aligned(a->down, a->k, a->weight_type), st))
-            return e;
-        p.w = a->up, p.width = a->n;
-        p.base = a->base, p.ldbase = a->base_stride, p.out = a->out, p.ldout = a->out_stride;
+        const Args d = down_args(a, a->x, a->x_stride, a->down, a->k, a->h);
+        Args u = d;
+        u.w = a->up, u.width = a->n;
+        u.base = a->base, u.ldbase = a->base_stride, u.out = a->out, u.ldout = a->out_stride;
         const bool vec = a->n % 8 == 0 && aligned(a->up, a->n, a->weight_type) && aligned(a->out, a->out_stride, a->act_type) &&
                          (!a->base || aligned(a->base, a->base_stride, a->act_type));
-        return up<X, W>(p, vec, st);
+        return both<X, W>(d, a->k % 8 == 0 && aligned(a->x, a->x_stride, a->act_type) && aligned(a->down, a->k, a->weight_type), u, vec, st);
     });
 }
 
@@ -386,12 +416,12 @@ extern "C" int ds_adapters_backward(const ds_adapters_t* a, void* stream)
         const bool vec_k = a->k % 8 == 0 && aligned(a->x, a->x_stride, a->act_type) && aligned(a->down, a->k, a->weight_type);
         const bool vec_n = a->n % 8 == 0 && aligned(a->grad, a->grad_stride, a->act_type) && aligned(a->up, a->n, a->weight_type);
         const Args dh = down_args(a, a->grad, a->grad_stride, a->up, a->n, a->dh);
-        if ((a->dx || a->ddown) && a->rows)
-            if (const int e = down<X, W>(dh, vec_n, st)) return e;
         if (a->dx && a->rows) {
             Args p = dh;
             p.w = a->down, p.width = a->k, p.out = a->dx, p.ldout = a->dx_stride;
-            if (const int e = up<X, W>(p, vec_k && aligned(a->dx, a->dx_stride, a->act_type), st)) return e;
+            if (const int e = both<X, W>(dh, vec_n, p, vec_k && aligned(a->dx, a->dx_stride, a->act_type), st)) return e;
+        } else if (a->ddown && a->rows) {
+            if (const int e = down<X, W>(dh, vec_n, st)) return e;
         }
         if (a->ddown) {
             Args p = dh;

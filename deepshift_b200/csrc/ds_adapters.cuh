@@ -75,6 +75,13 @@ template <> __device__ __forceinline__ unsigned short narrow<bf16>(float v) { re
 template <> __device__ __forceinline__ unsigned short narrow<f16>(float v) { return __half_as_ushort(__float2half_rn(v)); }
 template <> __device__ __forceinline__ unsigned short narrow<float>(float) { return 0; }
 
+template <class T>
+__device__ __forceinline__ float one(const T* p)
+{
+    if constexpr (is_f32<T>) return *p;
+    else return widen<T>(*reinterpret_cast<const unsigned short*>(p));
+}
+
 // N consecutive elements (N * sizeof(T) a multiple of 8 or 16 bytes) as fp32; of them `live` are in range, the rest are 0.
 // VEC: all or none are in range, and the address is aligned.
 template <class T, int N, bool VEC>
@@ -198,6 +205,12 @@ __device__ __forceinline__ void copy16(unsigned to, const void* from, bool live)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
+template <int BYTES>
+__device__ __forceinline__ void copy_bytes(unsigned to, const void* from, bool live)
+{
+    if constexpr (BYTES == 16) copy16(to, from, live);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(live ? 8 : 0) : "memory");
+}
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -206,6 +219,13 @@ __device__ __forceinline__ uint4 slot(unsigned at)
 {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint2 slot8(unsigned at)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
     return v;
 }
 
@@ -238,7 +258,7 @@ struct Down {
     static constexpr int PIECES = 2 * MT * XP + NT * WP, STAGE = THREADS * 16 * PIECES;
     static constexpr int FIT = 98304 / STAGE, STAGES = FIT < 2 ? 2 : FIT > 6 ? 6 : FIT;
     static constexpr int SUMS = WARPS * 16 * MT * 8 * NT * 4;
-    static constexpr int smem(bool vec) { return vec && STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS; }
+    __host__ __device__ static constexpr int smem(bool vec) { return vec && STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS; }
 };
 
 // One step's products.  fp32 sums of a few products begin at zero and are added to the running ones by the adder, which rounds; the
@@ -258,18 +278,22 @@ __device__ __forceinline__ void down_step(float (&acc)[MT][NT][4], const float (
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            unsigned h0, h1, l0, l1;
-            parts<!is_f32<W>>(b[j][e], h0, l0);
-            parts<!is_f32<W>>(b[j][e + 1], h1, l1);
+            unsigned h[2], l[2];
+            parts<!is_f32<W>>(b[j][e], h[0], l[0]);
+            parts<!is_f32<W>>(b[j][e + 1], h[1], l[1]);
+            float t[MT][4] = {};
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                float t[4] = {};
-                if (is_f32<X>) mma_tf32(t, al[i], h0, h1);
-                if (is_f32<W>) mma_tf32(t, ah[i], l0, l1);
-                mma_tf32(t, ah[i], h0, h1);
+            for (int i = 0; i < MT; ++i)
+                if (is_f32<X>) mma_tf32(t[i], al[i], h[0], h[1]);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) acc[i][j][q] += t[q];
-            }
+            for (int i = 0; i < MT; ++i)
+                if (is_f32<W>) mma_tf32(t[i], ah[i], l[0], l[1]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) mma_tf32(t[i], ah[i], h[0], h[1]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[i][j][q] += t[i][q];
         }
     }
 }
@@ -289,49 +313,65 @@ __device__ __forceinline__ float4 sums_of(const float* here, int rank)
     return v;
 }
 
-// h for one tile of 16 MT rows: a CTA's warps share the summed index out among them, and so do the `gridDim.y` CTAs of a cluster,
-// which add up their sums over distributed shared memory, in their order.  blockIdx.z: ranks by 8 NT.
+// A lane's elements of one step of a row, `left` of which are left: the copies of them, and plain loads.  HALVES: four elements from `row`,
+// four more 16 elements on.
+template <class T, bool HALVES>
+__device__ __forceinline__ void copy_step(unsigned to, const T* row, bool live, const void* other, int left)
+{
+    if constexpr (HALVES) {
+        constexpr int BYTES = 4 * sizeof(T), PER = 16 / BYTES;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const bool in = live && left > 16 * e;
+            copy_bytes<BYTES>(to + e / PER * THREADS * 16 + e % PER * BYTES, in ? static_cast<const void*>(row + 16 * e) : other, in);
+        }
+    } else {
+        const bool in = live && left > 0;   // a width of whole eights: all of the lane's elements, or none
+        copy_bytes<16>(to, in ? static_cast<const void*>(row) : other, in);
+    }
+}
+
+template <class T, int LK, bool HALVES>
+__device__ __forceinline__ void fetch_step(const T* row, int left, float (&v)[LK])
+{
+    constexpr int RUN = HALVES ? 4 : LK;
+#pragma unroll
+    for (int e = 0; e < LK; ++e) {
+        const int k = e / RUN * 16 + e % RUN;
+        v[e] = k < left ? one(row + k) : 0.f;
+    }
+}
+
+// The sums of one warp for a tile of 16 MT rows and 8 NT ranks from r0: every `workers`-th step from `first`.
 template <class X, class W, int MT, int NT, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
+__device__ __forceinline__ void down_sums(const Args& p, const int4& tile, int r0, unsigned char* smem, int first, int workers, float (&acc)[MT][NT][4])
 {
     using S = Down<X, W, MT, NT>;
     constexpr int LK = S::LK, CHUNK = 4 * LK;
-    extern __shared__ __align__(16) unsigned char smem[];
-    if (int(blockIdx.x) >= p.plan.head[0]) return;
-    const int4 tile = p.plan.tiles[blockIdx.x];
-    if (tile.x >= p.count) return;   // rows without an adapter: nothing reads their h
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int r0 = blockIdx.z * 8 * NT;
-    // rows g, 8 + g, ... of this CTA's ranks, and where this lane's elements begin
-    const W* w = static_cast<const W*>(p.w) + ((long long)tile.x * p.rank + r0 + g) * p.width + t * LK;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // rows g, 8 + g, ... of this CTA's ranks, and where this lane's elements begin: consecutive ones, save that of eight fp32 beside
+    // eight 16-bit elements each half lies in its half of the step, so that four lanes' copies fill whole sectors
+    constexpr bool HALVES = S::XP == 2 || S::WP == 2;
+    const int at = HALVES ? 4 * t : LK * t;
+    const W* w = static_cast<const W*>(p.w) + ((long long)tile.x * p.rank + r0 + g) * p.width + at;
     const long long eight = 8ll * p.width;
     const int ranks = p.rank - r0 - g;   // row 8 j is one as long as 8 j is less
     const X* xr[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
         const int m = tile_row(p.plan, tile, 8 * i + g);
-        xr[i] = m < 0 ? nullptr : static_cast<const X*>(p.x) + m * p.ldx + t * LK;
+        xr[i] = m < 0 ? nullptr : static_cast<const X*>(p.x) + m * p.ldx + at;
     }
-    float acc[MT][NT][4] = {};
-    const int chunks = (p.width + CHUNK - 1) / CHUNK, workers = WARPS * gridDim.y, first = blockIdx.y * WARPS + warp;
+    const int chunks = (p.width + CHUNK - 1) / CHUNK;
     if constexpr (VEC) {
         const unsigned mine = shared_address(smem) + threadIdx.x * 16;
         auto issue = [&](int c, int stage) {
             if (c < chunks) {
                 const unsigned to = mine + stage * S::STAGE;
-                const bool live = c * CHUNK + t * LK < p.width;   // a width of whole eights: all of the lane's elements, or none
-                int q = 0;
 #pragma unroll
-                for (int i = 0; i < 2 * MT; ++i)
+                for (int i = 0; i < 2 * MT; ++i) copy_step<X, HALVES>(to + i * S::XP * THREADS * 16, xr[i] + c * CHUNK, xr[i] != nullptr, p.x, p.width - c * CHUNK - at);
 #pragma unroll
-                    for (int e = 0; e < S::XP; ++e, ++q)
-                        copy16(to + q * THREADS * 16, live && xr[i] ? xr[i] + c * CHUNK + e * (LK / S::XP) : static_cast<const X*>(p.x), live && xr[i]);
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < S::WP; ++e, ++q)
-                        copy16(to + q * THREADS * 16, live && 8 * j < ranks ? w + j * eight + c * CHUNK + e * (LK / S::WP) : static_cast<const W*>(p.w),
-                               live && 8 * j < ranks);
+                for (int j = 0; j < NT; ++j) copy_step<W, HALVES>(to + (2 * MT * S::XP + j * S::WP) * THREADS * 16, w + j * eight + c * CHUNK, 8 * j < ranks, p.w, p.width - c * CHUNK - at);
             }
             copies_end();
         };
@@ -377,17 +417,23 @@ __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
         copies_wait<0>();
     } else {
         for (int c = first; c < chunks; c += workers) {
-            const int k = c * CHUNK, live = p.width - k - t * LK;
             float af[2 * MT][LK], bf[NT][LK];
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) load<X, LK, false>(xr[i] + k, xr[i] ? live : 0, af[i]);
+            for (int i = 0; i < 2 * MT; ++i) fetch_step<X, LK, HALVES>(xr[i] + c * CHUNK, xr[i] ? p.width - c * CHUNK - at : 0, af[i]);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) load<W, LK, false>(w + j * eight + k, 8 * j < ranks ? live : 0, bf[j]);
+            for (int j = 0; j < NT; ++j) fetch_step<W, LK, HALVES>(w + j * eight + c * CHUNK, 8 * j < ranks ? p.width - c * CHUNK - at : 0, bf[j]);
             down_step<X, W, MT, NT, LK>(acc, af, bf);
         }
     }
+}
+
+// The warps' sums in shared memory, [WARPS][16 MT][8 NT]; with `whole` added up in the first.
+template <int MT, int NT>
+__device__ __forceinline__ float* gather_sums(unsigned char* smem, const float (&acc)[MT][NT][4], bool whole)
+{
     constexpr int ROWS = 16 * MT, COLS = 8 * NT;
-    float* red = reinterpret_cast<float*>(smem);   // [WARPS][ROWS][COLS]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    float* red = reinterpret_cast<float*>(smem);
     __syncthreads();   // the queue's memory is free
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -397,16 +443,31 @@ __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
             for (int e = 0; e < 4; ++e)
                 red[(warp * ROWS + 16 * i + g + (e & 2) * 4) * COLS + 8 * j + 2 * t + (e & 1)] = acc[i][j][e];
     __syncthreads();
-    const int shares = gridDim.y;
-    if (shares > 1) {
+    if (whole)
         for (int i = threadIdx.x; i < ROWS * COLS; i += THREADS) {
             float s = 0.f;
 #pragma unroll
             for (int q = 0; q < WARPS; ++q) s += red[q * ROWS * COLS + i];
             red[i] = s;   // this thread alone reads and writes element i of each
         }
-        cluster_sync();
-    }
+    return red;
+}
+
+// h for one tile of 16 MT rows: a CTA's warps share the summed index out among them, and so do the `gridDim.y` CTAs of a cluster,
+// which add up their sums over distributed shared memory, in their order.  blockIdx.z: ranks by 8 NT.
+template <class X, class W, int MT, int NT, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
+{
+    constexpr int ROWS = 16 * MT, COLS = 8 * NT;
+    extern __shared__ __align__(16) unsigned char smem[];
+    if (int(blockIdx.x) >= p.plan.head[0]) return;
+    const int4 tile = p.plan.tiles[blockIdx.x];
+    if (tile.x >= p.count) return;   // rows without an adapter: nothing reads their h
+    const int r0 = blockIdx.z * COLS, shares = gridDim.y;
+    float acc[MT][NT][4] = {};
+    down_sums<X, W, MT, NT, VEC>(p, tile, r0, smem, blockIdx.y * WARPS + (threadIdx.x >> 5), WARPS * shares, acc);
+    const float* red = gather_sums(smem, acc, shares > 1);
+    if (shares > 1) cluster_sync();
     for (int i = (blockIdx.y * THREADS + threadIdx.x) * 4; i < ROWS * COLS; i += shares * THREADS * 4) {
         const int row = i / COLS, r = r0 + i % COLS;
         const int m = tile_row(p.plan, tile, row);
@@ -451,108 +512,315 @@ __device__ __forceinline__ void put_h4(unsigned* h, int halves, int at, int r, c
     put_parts(to + 6, v.w * scale);
 }
 
-// One tile of 16 MT rows, 64 columns a warp: lane (g, t) loads eight consecutive columns 8 g .. of ranks 2t and 2t + 1, which are
-// the elements of eight instructions, and ends up with the sixteen consecutive columns 16 t .. of rows g and g + 8.  The tile's h,
-// scaled and split, lies in shared memory for all warps in the order in which the instructions read it; base is on its way meanwhile.
+// ---- the up projection: 16 rows x 64 columns a warp ----
+// Which column of the 64 is element c (0 .. 7) of instruction j (0 .. 7) is free.  With 16-bit results it is 8 c + j, with fp32 32 (j / 4) +
+// 4 c + j % 4: lane g then loads its columns of a row of w in runs of 16 bytes beside its neighbours', and
+// lane t, whose elements are c = 2t and 2t + 1, ends up with units of 32 consecutive bytes of rows g and g + 8.
+template <class X>
+struct Columns {
+    static constexpr int RUNS = is_f32<X> ? 2 : 1, RUN = 8 / RUNS;      // of w: run q begins at 32 q + RUN g
+    static constexpr int UNITS = is_f32<X> ? 2 : 1, UNIT = 32 / sizeof(X);
+    __device__ static int unit(int u, int t) { return 32 * u + UNIT * t; }
+    // the values of unit u of the row's half (0: g, 1: g + 8)
+    __device__ static void values(const float (&acc)[8][4], int u, int half, float (&v)[UNIT])
+    {
+        if constexpr (is_f32<X>) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = acc[4 * u + e % 4][half * 2 + e / 4];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = acc[e % 8][half * 2 + e / 8];
+        }
+    }
+};
+
+// Two lanes' units are copied and stored half and half, both lanes in one unit at a time: an access of 32 bytes side by side
+// is a whole sector, where 16 bytes each of two sectors would move both twice.
+// Address of the half that this lane deals with of the unit of lane `2 (t / 2) + e` of its pair.
+template <class X>
+__device__ __forceinline__ int half_unit(int u, int t, int e)
+{
+    return Columns<X>::unit(u, (t & ~1) | e) + (t & 1) * (16 / int(sizeof(X)));
+}
+
+// base of rows `row` (a lane's two), 64 columns from n0, to the lanes' slots: [row][unit][half][thread].
+template <class X>
+__device__ __forceinline__ void issue_base(const Args& p, const int (&row)[2], int n0, unsigned slots)
+{
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < Columns<X>::UNITS; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int n = n0 + half_unit<X>(u, t, e), owner = (threadIdx.x & ~3) | (t & ~1) | e;
+                const bool live = row[i] >= 0 && n < p.width;
+                copy16(slots + (((i * Columns<X>::UNITS + u) * 2 + (t & 1)) * THREADS + owner) * 16,
+                       static_cast<const X*>(p.base) + (live ? row[i] * p.ldbase + n : 0), live);
+            }
+}
+template <class X>
+constexpr int base_bytes = 2 * Columns<X>::UNITS * 2 * THREADS * 16;   // of 16 rows
+
+// base (its copies have arrived, for the whole warp) plus the sums, to the rows.
+template <class X>
+__device__ __forceinline__ void finish_rows(const Args& p, const int (&row)[2], int n0, unsigned slots, const float (&acc)[8][4])
+{
+    constexpr int UNIT = Columns<X>::UNIT;
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < Columns<X>::UNITS; ++u) {
+            float v[UNIT];
+            Columns<X>::values(acc, u, i, v);
+            if (p.base) {
+                uint4 q[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) q[e] = slot(slots + (((i * Columns<X>::UNITS + u) * 2 + e) * THREADS + threadIdx.x) * 16);
+                float b[UNIT];
+                widen_pieces<X>(q, b);
+#pragma unroll
+                for (int e = 0; e < UNIT; ++e) v[e] += b[e];
+            }
+            unsigned w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (is_f32<X>) w[e] = __float_as_uint(v[e]);
+                else w[e] = narrow<X>(v[2 * e]) | unsigned(narrow<X>(v[2 * e + 1])) << 16;
+            }
+            unsigned got[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) got[e] = __shfl_xor_sync(0xFFFFFFFFu, t & 1 ? w[e] : w[4 + e], 1);
+            if (row[i] < 0) continue;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int n = n0 + half_unit<X>(u, t, e);
+                const bool mine = (t & 1) == e;   // even lanes keep their first half, odd ones their second
+                const uint4 x = mine ? (e ? make_uint4(w[4], w[5], w[6], w[7]) : make_uint4(w[0], w[1], w[2], w[3])) : make_uint4(got[0], got[1], got[2], got[3]);
+                if (n < p.width) *reinterpret_cast<uint4*>(static_cast<X*>(p.out) + row[i] * p.ldout + n) = x;
+            }
+        }
+}
+
+// The same where rows have no alignment: through shared memory (`stage`, 16 x 65 floats of the warp's own), so that lanes side by
+// side read and write elements side by side.
+template <class X>
+__device__ __forceinline__ void finish_unaligned(const Args& p, const int4& tile, int first, int n0, float* stage, const float (&acc)[8][4])
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < Columns<X>::UNITS; ++u) {
+            float v[Columns<X>::UNIT];
+            Columns<X>::values(acc, u, i, v);
+#pragma unroll
+            for (int e = 0; e < Columns<X>::UNIT; ++e) stage[(8 * i + g) * 65 + Columns<X>::unit(u, t) + e] = v[e];
+        }
+    __syncwarp();
+#pragma unroll 4
+    for (int r = 0; r < 16; ++r) {
+        const int m = tile_row(p.plan, tile, first + r);
+        if (m < 0) break;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int n = n0 + lane + 32 * c;
+            if (n >= p.width) continue;
+            float v = stage[r * 65 + lane + 32 * c];
+            if (p.base) v += one(static_cast<const X*>(p.base) + m * p.ldbase + n);
+            X* to = static_cast<X*>(p.out) + m * p.ldout + n;
+            if constexpr (is_f32<X>) *to = v;
+            else *reinterpret_cast<unsigned short*>(to) = narrow<X>(v);
+        }
+    }
+}
+
+// This lane's columns of rank row r of `w` (at element n0 of the adapter's first row), zeros outside.
+template <class X, class W, bool VEC>
+__device__ __forceinline__ void load_w(const Args& p, const W* w, int r, int n0, float (&v)[8])
+{
+    using C = Columns<X>;
+    const int g = (threadIdx.x & 31) >> 2;
+#pragma unroll
+    for (int q = 0; q < C::RUNS; ++q) {
+        const int n = 32 * q + C::RUN * g;
+        float x[C::RUN];
+        load<W, C::RUN, VEC>(w + (long long)r * p.width + n, r < p.rank ? p.width - n0 - n : 0, x);
+#pragma unroll
+        for (int e = 0; e < C::RUN; ++e) v[q * C::RUN + e] = x[e];
+    }
+}
+
+// Products of eight ranks: b = this lane's columns of ranks 2t and 2t + 1, h the address of its elements of the first operand.  fp32 results of up
+// to 32 ranks are one chain of additions (12 of them, cut off at 2^-23 each); flush adds longer ones up in between.
+template <class X, class W>
+__device__ __forceinline__ void up_step(float (&acc)[8][4], unsigned h, const float (&b)[2][8])
+{
+    const uint4 u = slot(h), v = slot(h + 512);
+    const unsigned ah[4] = {u.x, u.y, u.z, u.w}, al[4] = {v.x, v.y, v.z, v.w};
+    unsigned hi[8][2], lo[8][2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) parts<!is_f32<W>>(b[e][j], hi[j][e], lo[j][e]);
+    // one term of all columns after the other: instructions of one column wait for one another
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mma_tf32(acc[j], al, hi[j][0], hi[j][1]);
+    if (is_f32<W>) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mma_tf32(acc[j], ah, lo[j][0], lo[j][1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mma_tf32(acc[j], ah, hi[j][0], hi[j][1]);
+}
+
+__device__ __forceinline__ void flush(float (&total)[8][4], float (&acc)[8][4])
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[j][e] += acc[j][e], acc[j][e] = 0.f;
+}
+
+// All ranks of one warp's 64 columns; `h` = the tile's h in shared memory, `halves` of 16 rows in a block, this being number `half`.  The next
+// ranks' columns are on their way during the products of the present ones.
+template <class X, class W, bool VEC>
+__device__ __forceinline__ void up_products(const Args& p, int adapter, int n0, unsigned h, int halves, int half, float (&acc)[8][4])
+{
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    const W* w = static_cast<const W*>(p.w) + (long long)adapter * p.rank * p.width + n0;
+    float next[2][8], part[8][4] = {};
+    load_w<X, W, VEC>(p, w, 2 * t, n0, next[0]);
+    load_w<X, W, VEC>(p, w, 2 * t + 1, n0, next[1]);
+    for (int r = 0; r < p.rank8; r += 8) {
+        float b[2][8];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) b[e >> 3][e & 7] = next[e >> 3][e & 7];
+        if (r + 8 < p.rank8) {
+            load_w<X, W, VEC>(p, w, r + 8 + 2 * t, n0, next[0]);
+            load_w<X, W, VEC>(p, w, r + 9 + 2 * t, n0, next[1]);
+        }
+        up_step<X, W>(part, h + (r / 8 * halves + half) * 1024 + lane * 16, b);
+        if (r % 32 == 24) flush(acc, part);
+    }
+    flush(acc, part);
+}
+
+// One tile of the plan (MT halves of 16 rows) and 512 columns a CTA.  The tile's h, scaled and split, lies in shared memory for all
+// warps in the order in which the instructions read it; base is on its way meanwhile.
 template <class X, class W, int MT, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 {
-    constexpr int BP = 16 * sizeof(X) / 16;   // pieces of a lane's columns of one row
     extern __shared__ __align__(16) unsigned char smem[];
     if (int(blockIdx.x) >= p.plan.head[0]) return;
     const int4 tile = p.plan.tiles[blockIdx.x];
     const bool none = tile.x >= p.count;
     if (none && p.base == p.out) return;   // in place: these rows are there already
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
     const int n0 = (blockIdx.y * WARPS + warp) * 64;
-    int row[2 * MT];
+    int row[MT][2];
+    const unsigned h = shared_address(smem), slots = h + p.rank8 * 16 * MT * 8;
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) row[i] = tile_row(p.plan, tile, 8 * i + g);
-    const unsigned mine = shared_address(smem) + p.rank8 * 16 * MT * 8 + threadIdx.x * 16;
-    if (VEC && p.base) {
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i)
-#pragma unroll
-            for (int e = 0; e < BP; ++e) {
-                const int n = n0 + 16 * t + e * (16 / BP);
-                const bool live = row[i] >= 0 && n < p.width;
-                copy16(mine + (i * BP + e) * THREADS * 16, static_cast<const X*>(p.base) + (live ? row[i] * p.ldbase + n : 0), live);
-            }
-        copies_end();
+    for (int i = 0; i < MT; ++i) {
+        row[i][0] = tile_row(p.plan, tile, 16 * i + g), row[i][1] = tile_row(p.plan, tile, 16 * i + 8 + g);
+        if (VEC && p.base) issue_base<X>(p, row[i], n0, slots + i * base_bytes<X>);
     }
-    float acc[MT][8][4] = {};
+    if (VEC) copies_end();
     if (!none) {
         const float scale = p.scale ? p.scale[tile.x] : 1.f;
-        unsigned* h = reinterpret_cast<unsigned*>(smem);
         constexpr int PER = THREADS / (16 * MT);   // threads a row
         const int at = threadIdx.x / PER, m = tile_row(p.plan, tile, at);
-        for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(h, MT, at, r, load_h4(p, m, r), scale);
-        __syncthreads();
-        const W* w = static_cast<const W*>(p.w) + (long long)tile.x * p.rank * p.width + n0 + 8 * g;
-        const int live = p.width - n0 - 8 * g;
-        float next[2][8];
-        auto fetch = [&](int r) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) load<W, 8, VEC>(w + (long long)(r + 2 * t + e) * p.width, r + 2 * t + e < p.rank ? live : 0, next[e]);
-        };
-        fetch(0);
-        for (int r = 0; r < p.rank8; r += 8) {
-            float b[2][8];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) b[e >> 3][e & 7] = next[e >> 3][e & 7];
-            if (r + 8 < p.rank8) fetch(r + 8);
-            unsigned ah[MT][4], al[MT][4];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const unsigned here = shared_address(h + (r / 8 * MT + i) * 256 + lane * 4);
-                const uint4 u = slot(here), v = slot(here + 512);
-                ah[i][0] = u.x, ah[i][1] = u.y, ah[i][2] = u.z, ah[i][3] = u.w;
-                al[i][0] = v.x, al[i][1] = v.y, al[i][2] = v.z, al[i][3] = v.w;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                unsigned h0, h1, l0, l1;
-                parts<!is_f32<W>>(b[0][j], h0, l0);
-                parts<!is_f32<W>>(b[1][j], h1, l1);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    // fp32 results: as in down_step
-                    float s[4] = {};
-                    float(&d)[4] = is_f32<X> ? s : acc[i][j];
-                    mma_tf32(d, al[i], h0, h1);
-                    if (is_f32<W>) mma_tf32(d, ah[i], l0, l1);
-                    mma_tf32(d, ah[i], h0, h1);
-                    if (is_f32<X>) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][e] += s[e];
-                    }
-                }
-            }
-        }
+        for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(reinterpret_cast<unsigned*>(smem), MT, at, r, load_h4(p, m, r), scale);
     }
-    // column 8 c + j of the warp's 64 sits in element c of instruction j: c = 2t and 2t + 1 are this lane's
-    if (VEC) copies_wait<0>();
+    __syncthreads();
+    if (n0 >= p.width) return;
+    float* stage = reinterpret_cast<float*>(smem + p.rank8 * 16 * MT * 8) + warp * 16 * 65;
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-        if (row[i] < 0) continue;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int n = n0 + 16 * t + 8 * c, live = p.width - n;
-            float v[8] = {};
-            if (p.base) {
-                if constexpr (VEC) {
-                    uint4 q[BP / 2];
-#pragma unroll
-                    for (int e = 0; e < BP / 2; ++e) q[e] = slot(mine + (i * BP + c * (BP / 2) + e) * THREADS * 16);
-                    widen_pieces<X>(q, v);
-                } else load<X, 8, VEC>(static_cast<const X*>(p.base) + row[i] * p.ldbase + n, live, v);
+    for (int i = 0; i < MT; ++i) {
+        float acc[8][4] = {};
+        if (!none) up_products<X, W, VEC>(p, tile.x, n0, h, MT, i, acc);
+        if constexpr (VEC) {
+            if (i == 0) {
+                copies_wait<0>();
+                __syncwarp();
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += acc[i >> 1][j][(i & 1) * 2 + c];
-            store<X, 8, VEC>(static_cast<X*>(p.out) + row[i] * p.ldout + n, live, v);
-        }
+            finish_rows<X>(p, row[i], n0, slots + i * base_bytes<X>, acc);
+        } else finish_unaligned<X>(p, tile, 16 * i, n0, stage, acc);
     }
 }
+
+// Few rows: both projections of a tile of 16 in one launch (`d`: the down projection's operands, `u`: the up projection's).  The CTAs of
+// a cluster share the summed index out, each adds all their sums up over distributed shared memory, and takes every
+// gridDim.y-th 64 columns of the result, whose part of w and base are fetched while the sums are being formed.
+template <class X, class W, int NT, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Args u)
+{
+    constexpr int COLS = 8 * NT, SUMS = Down<X, W, 1, NT>::smem(VEC);
+    extern __shared__ __align__(16) unsigned char smem[];   // queue and sums, h, base or stage
+    if (int(blockIdx.x) >= d.plan.head[0]) return;
+    const int4 tile = d.plan.tiles[blockIdx.x];
+    const bool none = tile.x >= d.count;
+    if (none && u.base == u.out) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, shares = gridDim.y, share = blockIdx.y;
+    const int row[2] = {tile_row(d.plan, tile, g), tile_row(d.plan, tile, 8 + g)};
+    unsigned* parts_h = reinterpret_cast<unsigned*>(smem + SUMS);
+    const unsigned h = shared_address(parts_h), slots = h + COLS * 16 * 8;
+    float* stage = reinterpret_cast<float*>(smem + SUMS + COLS * 16 * 8) + warp * 16 * 65;
+    if (!none) {
+        const int n0 = (warp * shares + share) * 64;
+        if (n0 < u.width) {
+            const W* w = static_cast<const W*>(u.w) + (long long)tile.x * u.rank * u.width + n0;
+            for (int r = 2 * t; r < u.rank; r += 8)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (r + e < u.rank && n0 + 8 * g < u.width)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(w + (long long)(r + e) * u.width + 8 * g));
+        }
+        float acc[1][NT][4] = {};
+        down_sums<X, W, 1, NT, VEC>(d, tile, 0, smem, share * WARPS + warp, WARPS * shares, acc);
+        const float scale = u.scale ? u.scale[tile.x] : 1.f;
+        const float* red = gather_sums(smem, acc, true);
+        if (shares > 1) cluster_sync();
+        else __syncthreads();
+        for (int i = threadIdx.x * 4; i < 16 * COLS; i += THREADS * 4) {
+            const int at = i / COLS, r = i % COLS;
+            if (r >= d.rank8) continue;
+            float s[4] = {};
+            for (int q = 0; q < shares; ++q) {
+                const float4 v = shares > 1 ? sums_of(red + i, q) : *reinterpret_cast<const float4*>(red + i);
+                s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r + e >= d.rank) s[e] = 0.f;
+            const float4 v = make_float4(s[0], s[1], s[2], s[3]);
+            put_h4(parts_h, 1, at, r, v, scale);
+            const int m = tile_row(d.plan, tile, at);
+            if (d.h && share == 0 && m >= 0) *reinterpret_cast<float4*>(d.h + (long long)m * d.rank8 + r) = v;
+        }
+        if (shares > 1) cluster_sync();   // nobody leaves while its sums are being read
+        else __syncthreads();
+    }
+    for (int n0 = (warp * shares + share) * 64; n0 < u.width; n0 += WARPS * shares * 64) {
+        if (VEC && u.base) {
+            __syncwarp();
+            issue_base<X>(u, row, n0, slots);
+        }
+        if (VEC) copies_end();
+        float acc[8][4] = {};
+        if (!none) up_products<X, W, VEC>(u, tile.x, n0, h, 1, 0, acc);
+        if constexpr (VEC) {
+            copies_wait<0>();
+            __syncwarp();
+            finish_rows<X>(u, row, n0, slots, acc);
+        } else finish_unaligned<X>(u, tile, 0, n0, stage, acc);
+    }
+}
+template <class X, class W, int NT>
+constexpr int both_smem(bool vec) { return Down<X, W, 1, NT>::smem(vec) + 8 * NT * 16 * 8 + (vec ? base_bytes<X> : WARPS * 16 * 65 * 4); }
 
 // Many rows: up_kernel's product for 256 columns and a run of consecutive tiles of 32 rows.  The adapter's part of `w` stays in shared memory
 // until a tile of another adapter comes (up_kernel reads it from L2 for every tile, and waits for it), and the next tile's
@@ -560,23 +828,23 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 template <class X, class W>
 struct Stream {
     static constexpr int COLS = 256, ROWS = 32;
-    static constexpr int BP = 16 * sizeof(X) / 16, BASE = THREADS * 16 * 2 * BP;   // base of a tile: two rows of sixteen columns a lane
     static constexpr int WROW = COLS * int(sizeof(W)) + 16;   // a row of w: rows 2t of the lanes t fall on different banks
     static constexpr int MOST_RANK = 64;
     __host__ __device__ static constexpr int h_bytes(int rank8) { return ROWS * rank8 * 8; }
-    static constexpr int smem(int rank8) { return 2 * BASE + 2 * h_bytes(rank8) + rank8 * WROW; }
+    static constexpr int smem(int rank8) { return 2 * base_bytes<X> + 2 * h_bytes(rank8) + rank8 * WROW; }
 };
 
 template <class X, class W>
 __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
 {
     using S = Stream<X, W>;
+    using C = Columns<X>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int total = p.plan.head[0], first = int((long long)total * blockIdx.x / gridDim.x), last = int((long long)total * (blockIdx.x + 1) / gridDim.x);
     if (first == last) return;
     const int c0 = blockIdx.y * S::COLS, in_block = (warp & 3) * 64, n0 = c0 + in_block, half = warp >> 2;
-    const unsigned base_at = shared_address(smem) + threadIdx.x * 16, h_at = shared_address(smem) + 2 * S::BASE, w_at = h_at + 2 * S::h_bytes(p.rank8);
+    const unsigned base_at = shared_address(smem), h_at = base_at + 2 * base_bytes<X>, w_at = h_at + 2 * S::h_bytes(p.rank8);
     constexpr int PER = THREADS / S::ROWS, HV = S::MOST_RANK / 4 / PER;   // threads a row, and fours of its h that each brings in
     const int h_row = threadIdx.x / PER, h_rank = threadIdx.x % PER * 4;
     float4 hv[HV];
@@ -594,38 +862,29 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
         n.h_m = none ? -1 : tile_row(p.plan, n.tile, h_row);
         n.scale = p.scale && !none ? p.scale[n.tile.x] : 1.f;
     };
-    auto issue_base = [&](const int (&row)[2], int buf) {
-        if (p.base) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < S::BP; ++e) {
-                    const int n = n0 + 16 * t + e * (16 / S::BP);
-                    const bool live = row[i] >= 0 && n < p.width;
-                    copy16(base_at + buf * S::BASE + (i * S::BP + e) * THREADS * 16, static_cast<const X*>(p.base) + (live ? row[i] * p.ldbase + n : 0), live);
-                }
-        }
-        copies_end();
-    };
     auto fetch_h = [&](const Ahead& n) {
 #pragma unroll
         for (int q = 0; q < HV; ++q)
             if (h_rank + q * PER * 4 < p.rank8) hv[q] = load_h4(p, n.h_m, h_rank + q * PER * 4);   // used, and waited for, in put_h
     };
     auto put_h = [&](const Ahead& n, int buf) {
-        unsigned* h = reinterpret_cast<unsigned*>(smem + 2 * S::BASE + buf * S::h_bytes(p.rank8));
+        unsigned* h = reinterpret_cast<unsigned*>(smem + 2 * base_bytes<X> + buf * S::h_bytes(p.rank8));
 #pragma unroll
         for (int q = 0; q < HV; ++q)
             if (h_rank + q * PER * 4 < p.rank8) put_h4(h, 2, h_row, h_rank + q * PER * 4, hv[q], n.scale);
     };
-    auto load_w = [&](int adapter) {
-        constexpr int PER = 16 / sizeof(W), PIECES = S::COLS / PER;
+    auto load_all = [&](int adapter) {
+        constexpr int EACH = 16 / sizeof(W), PIECES = S::COLS / EACH;
         const W* w = static_cast<const W*>(p.w) + (long long)adapter * p.rank * p.width + c0;
         for (int i = threadIdx.x; i < p.rank8 * PIECES; i += THREADS) {
-            const int r = i / PIECES, c = i % PIECES * PER;
+            const int r = i / PIECES, c = i % PIECES * EACH;
             const bool live = r < p.rank && c0 + c < p.width;
             copy16(w_at + r * S::WROW + c * int(sizeof(W)), live ? w + (long long)r * p.width + c : static_cast<const W*>(p.w), live);
         }
+        copies_end();
+    };
+    auto issue = [&](const Ahead& n, int buf) {
+        if (p.base) issue_base<X>(p, n.row, n0, base_at + buf * base_bytes<X>);
         copies_end();
     };
     Ahead now, next;
@@ -633,79 +892,61 @@ __global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
     next.tile = tile_of(first + 1);
     rows_of(now);
     rows_of(next);
-    issue_base(now.row, 0);
+    issue(now, 0);
     int held = -1;   // whose w is in shared memory
-    if (now.tile.x < p.count) load_w(held = now.tile.x);
+    if (now.tile.x < p.count) load_all(held = now.tile.x);
     fetch_h(now);
     put_h(now, 0);
     copies_wait<0>();
     __syncthreads();
     for (int at = first, buf = 0; at < last; ++at, buf ^= 1) {
-        issue_base(next.row, buf ^ 1);
+        issue(next, buf ^ 1);
         fetch_h(next);
         Ahead then;
         then.tile = tile_of(at + 2);
-        const int4 tile = now.tile;
-        const int(&row)[2] = now.row;
         float acc[8][4] = {};
-        if (tile.x < p.count) {
+        if (now.tile.x < p.count) {
             const unsigned h = h_at + buf * S::h_bytes(p.rank8) + half * 1024 + lane * 16;
-            const unsigned w = w_at + 2 * t * S::WROW + (in_block + 8 * g) * int(sizeof(W));
+            const unsigned w = w_at + 2 * t * S::WROW + (in_block + C::RUN * g) * int(sizeof(W));
+            float part[8][4] = {};
             for (int r = 0; r < p.rank8; r += 8) {
-                constexpr int WP = 8 * sizeof(W) / 16;
-                uint4 q[2][WP];
+                float b[2][8];
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int c = 0; c < WP; ++c) q[e][c] = slot(w + (r + e) * S::WROW + c * 16);
-                const uint4 u = slot(h + r / 8 * 2048), v = slot(h + r / 8 * 2048 + 512);
-                const unsigned ah[4] = {u.x, u.y, u.z, u.w}, al[4] = {v.x, v.y, v.z, v.w};
-                float b[2][8];
-                widen_pieces<W>(q[0], b[0]);
-                widen_pieces<W>(q[1], b[1]);
+                    for (int q = 0; q < C::RUNS; ++q) {
+                        const unsigned from = w + (r + e) * S::WROW + 32 * q * int(sizeof(W));
+                        constexpr int BYTES = C::RUN * sizeof(W);
+                        float v[C::RUN];
+                        if constexpr (BYTES == 8) {
+                            const uint2 x = slot8(from);
+                            v[0] = widen<W>((unsigned short)(x.x & 0xFFFFu)), v[1] = widen<W>((unsigned short)(x.x >> 16));
+                            v[2] = widen<W>((unsigned short)(x.y & 0xFFFFu)), v[3] = widen<W>((unsigned short)(x.y >> 16));
+                        } else {
+                            uint4 x[BYTES / 16];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    unsigned h0, h1, l0, l1;
-                    parts<!is_f32<W>>(b[0][j], h0, l0);
-                    parts<!is_f32<W>>(b[1][j], h1, l1);
-                    float s[4] = {};   // fp32 results: as in down_step
-                    float(&d)[4] = is_f32<X> ? s : acc[j];
-                    mma_tf32(d, al, h0, h1);
-                    if (is_f32<W>) mma_tf32(d, ah, l0, l1);
-                    mma_tf32(d, ah, h0, h1);
-                    if (is_f32<X>) {
+                            for (int i = 0; i < BYTES / 16; ++i) x[i] = slot(from + 16 * i);
+                            widen_pieces<W>(x, v);
+                        }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[j][e] += s[e];
+                        for (int i = 0; i < C::RUN; ++i) b[e][q * C::RUN + i] = v[i];
                     }
-                }
+                if constexpr (is_f32<X>) {
+                    up_step<X, W>(part, h + r / 8 * 2048, b);
+                    if (r % 32 == 24) flush(acc, part);
+                } else up_step<X, W>(acc, h + r / 8 * 2048, b);
             }
+            if constexpr (is_f32<X>)
+                if (p.rank8 % 32) flush(acc, part);
         }
         copies_wait<1>();
-        if (!(tile.x >= p.count && p.base == p.out)) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (row[i] < 0) continue;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int n = n0 + 16 * t + 8 * c;
-                    float v[8] = {};
-                    if (p.base) {
-                        uint4 q[S::BP / 2];
-#pragma unroll
-                        for (int e = 0; e < S::BP / 2; ++e) q[e] = slot(base_at + buf * S::BASE + (i * S::BP + c * (S::BP / 2) + e) * THREADS * 16);
-                        widen_pieces<X>(q, v);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] += acc[j][i * 2 + c];
-                    store<X, 8, true>(static_cast<X*>(p.out) + row[i] * p.ldout + n, p.width - n, v);
-                }
-            }
-        }
+        __syncwarp();
+        if (!(now.tile.x >= p.count && p.base == p.out)) finish_rows<X>(p, now.row, n0, base_at + buf * base_bytes<X>, acc);
         rows_of(then);
         put_h(next, buf ^ 1);
         if (next.tile.x < p.count && next.tile.x != held) {
             __syncthreads();   // everybody is done with the held one
-            load_w(held = next.tile.x);
+            load_all(held = next.tile.x);
             copies_wait<0>();
         }
         __syncthreads();
@@ -737,7 +978,6 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
     const int from = p.plan.offsets[a], all = p.plan.offsets[a + 1] - from, part = ((all + shares - 1) / shares + BLOCK - 1) / BLOCK * BLOCK;
     const int begin = from + min(all, share * part), end = from + min(all, (share + 1) * part);
     const float scale = p.scale ? p.scale[a] : 1.f;
-    const int n = n0 + NJ * g, live = p.width - n;
     const int count = (end - begin + BLOCK - 1) / BLOCK;
     float acc[RT][NJ][4] = {};
     // step i of this warp: rows 8 (i % STEPS RW + rw) ... of block i / STEPS
@@ -804,9 +1044,9 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
         for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int q = 0; q < XP; ++q) {
-                const bool in = m[e] >= 0 && live > 0;
-                copy16(mine + stage * STAGE + (e * XP + q) * THREADS * 16,
-                       static_cast<const X*>(p.x) + (in ? m[e] * p.ldx + n + q * (NJ / XP) : 0), in);
+                const int n = n0 + 32 * q + Columns<X>::RUN * g;
+                const bool in = m[e] >= 0 && n < p.width;
+                copy16(mine + stage * STAGE + (e * XP + q) * THREADS * 16, static_cast<const X*>(p.x) + (in ? m[e] * p.ldx + n : 0), in);
             }
         copies_end();
     };
@@ -849,7 +1089,11 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int m = row_at(i, e);
-                    load<X, NJ, false>(static_cast<const X*>(p.x) + (m >= 0 ? m * p.ldx + n : 0), m >= 0 ? live : 0, b[e]);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        const int n = n0 + 32 * (j / Columns<X>::RUN) + Columns<X>::RUN * g + j % Columns<X>::RUN;
+                        b[e][j] = m >= 0 && n < p.width ? one(static_cast<const X*>(p.x) + m * p.ldx + n) : 0.f;
+                    }
                 }
             }
             products(b, h);
@@ -866,7 +1110,7 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                red[(rw * RANKS + 16 * i + g + (e & 2) * 4) * COLS + 64 * cw + (2 * t + (e & 1)) * NJ + j] = acc[i][j][e];
+                red[(rw * RANKS + 16 * i + g + (e & 2) * 4) * COLS + 64 * cw + 32 * (j / Columns<X>::RUN) + Columns<X>::RUN * (2 * t + (e & 1)) + j % Columns<X>::RUN] = acc[i][j][e];
     __syncthreads();
     if (shares > 1) {
         if (RW > 1)

@@ -183,10 +183,10 @@ int launch_cluster(dim3 grid, dim3 cluster, int smem, cudaStream_t st, const A&.
 template <class X, class W, int MT, int NT, bool VEC>
 int launch_down(const Args& a, cudaStream_t st)
 {
-    constexpr int smem = Down<X, W, MT, NT>::smem(VEC);
+    constexpr int smem = Down<X, W, MT, NT, DOWN_BUDGET>::smem(VEC);
     static_assert(smem <= 227 * 1024, "shared memory of an SM");
     if (!allow_smem<down_kernel<X, W, MT, NT, VEC>>(smem)) return DS_ERR_CUDA;
-    const int blocks = (a.rank8 + 8 * NT - 1) / (8 * NT), chunk = 4 * Down<X, W, MT, NT>::LK, shares = splits_of(a, blocks, (a.width + chunk - 1) / chunk);
+    const int blocks = (a.rank8 + 8 * NT - 1) / (8 * NT), chunk = 4 * Down<X, W, MT, NT, DOWN_BUDGET>::LK, shares = splits_of(a, blocks, (a.width + chunk - 1) / chunk);
     return launch_cluster<down_kernel<X, W, MT, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), smem, st, a);
 }
 
@@ -198,7 +198,7 @@ int down_tile(const Args& a, bool vec, cudaStream_t st)
     if (!vec) return a.rank8 <= 8 ? launch_down<X, W, MT, 1, false>(a, st) : launch_down<X, W, MT, 4, false>(a, st);
     if (a.rank8 <= 8) return launch_down<X, W, MT, 1, true>(a, st);
     if (a.rank8 <= 16) return launch_down<X, W, MT, 2, true>(a, st);
-    if constexpr (Down<X, W, MT, 8>::SAME)
+    if constexpr (Down<X, W, MT, 8, DOWN_BUDGET>::SAME)
         if (a.rank8 > 32) return launch_down<X, W, MT, 8, true>(a, st);
     return launch_down<X, W, MT, 4, true>(a, st);
 }
@@ -216,7 +216,7 @@ int launch_up(const Args& a, cudaStream_t st)
     constexpr int rows = VEC ? MT * base_bytes<X> : WARPS * 16 * 65 * 4;
     const int smem = a.rank8 * 16 * MT * 8 + rows;
     if (!allow_smem<up_kernel<X, W, MT, VEC>>(MAX_RANK * 16 * MT * 8 + rows)) return DS_ERR_CUDA;
-    const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS));
+    const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS), VEC ? 1 : MT);
     up_kernel<X, W, MT, VEC><<<grid, THREADS, smem, st>>>(a);
     return finish();
 }
@@ -282,7 +282,7 @@ int launch_both(const Args& d, const Args& u, cudaStream_t st)
     static_assert(smem <= 227 * 1024, "shared memory of an SM");
     if (!allow_smem<both_kernel<X, W, NT, VEC>>(smem)) return DS_ERR_CUDA;
     // CTAs a tile: until there are two for each SM, as long as each has 64 columns or a step of every warp's
-    const int steps = (d.width + 4 * Down<X, W, 1, NT>::LK * WARPS - 1) / (4 * Down<X, W, 1, NT>::LK * WARPS), columns = (u.width + 63) / 64;
+    const int steps = (d.width + 4 * Down<X, W, 1, NT, BOTH_BUDGET>::LK * WARPS - 1) / (4 * Down<X, W, 1, NT, BOTH_BUDGET>::LK * WARPS), columns = (u.width + 63) / 64;
     const long long tiles = plan_tiles(d.rows, d.count);
     int shares = 1;
     while (shares < 8 && tiles * shares * 2 <= 296 && shares < (steps > columns ? steps : columns)) shares *= 2;

@@ -250,16 +250,18 @@ __device__ __forceinline__ void widen_pieces(const uint4 (&p)[N], float (&v)[N *
 }
 
 // Shapes of down_kernel: elements a lane takes of a row at a time (sixteen bytes of the narrower type), the 16-byte pieces of
-// that in both operands, and how many such steps are on their way (96 KB a CTA, so that two fit an SM; two steps at least).
-template <class X, class W, int MT, int NT>
+// that in both operands, and how many such steps are on their way (BUDGET bytes a CTA, so that two fit an SM; two steps at least).
+template <class X, class W, int MT, int NT, int BUDGET>
 struct Down {
     static constexpr bool SAME = !is_f32<X> && __is_same(X, W);   // both of one 16-bit type: no conversion at all
     static constexpr int LK = is_f32<X> && is_f32<W> ? 4 : 8, XP = LK * sizeof(X) / 16, WP = LK * sizeof(W) / 16;
     static constexpr int PIECES = 2 * MT * XP + NT * WP, STAGE = THREADS * 16 * PIECES;
-    static constexpr int FIT = 98304 / STAGE, STAGES = FIT < 2 ? 2 : FIT > 6 ? 6 : FIT;
+    static constexpr int FIT = BUDGET / STAGE, STAGES = FIT < 2 ? 2 : FIT > 6 ? 6 : FIT;
     static constexpr int SUMS = WARPS * 16 * MT * 8 * NT * 4;
     __host__ __device__ static constexpr int smem(bool vec) { return vec && STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS; }
 };
+
+constexpr int DOWN_BUDGET = 98304, BOTH_BUDGET = 49152;
 
 // One step's products.  fp32 sums of a few products begin at zero and are added to the running ones by the adder, which rounds; the
 // tensor core's own additions cut off, and a chain of 200 of them had a relative error of 3e-6.
@@ -343,10 +345,10 @@ __device__ __forceinline__ void fetch_step(const T* row, int left, float (&v)[LK
 }
 
 // The sums of one warp for a tile of 16 MT rows and 8 NT ranks from r0: every `workers`-th step from `first`.
-template <class X, class W, int MT, int NT, bool VEC>
+template <class X, class W, int MT, int NT, int BUDGET, bool VEC>
 __device__ __forceinline__ void down_sums(const Args& p, const int4& tile, int r0, unsigned char* smem, int first, int workers, float (&acc)[MT][NT][4])
 {
-    using S = Down<X, W, MT, NT>;
+    using S = Down<X, W, MT, NT, BUDGET>;
     constexpr int LK = S::LK, CHUNK = 4 * LK;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // rows g, 8 + g, ... of this CTA's ranks, and where this lane's elements begin: consecutive ones, save that of eight fp32 beside
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
     if (tile.x >= p.count) return;   // rows without an adapter: nothing reads their h
     const int r0 = blockIdx.z * COLS, shares = gridDim.y;
     float acc[MT][NT][4] = {};
-    down_sums<X, W, MT, NT, VEC>(p, tile, r0, smem, blockIdx.y * WARPS + (threadIdx.x >> 5), WARPS * shares, acc);
+    down_sums<X, W, MT, NT, DOWN_BUDGET, VEC>(p, tile, r0, smem, blockIdx.y * WARPS + (threadIdx.x >> 5), WARPS * shares, acc);
     const float* red = gather_sums(smem, acc, shares > 1);
     if (shares > 1) cluster_sync();
     for (int i = (blockIdx.y * THREADS + threadIdx.x) * 4; i < ROWS * COLS; i += shares * THREADS * 4) {
@@ -621,19 +623,31 @@ __device__ __forceinline__ void finish_unaligned(const Args& p, const int4& tile
             for (int e = 0; e < Columns<X>::UNIT; ++e) stage[(8 * i + g) * 65 + Columns<X>::unit(u, t) + e] = v[e];
         }
     __syncwarp();
-#pragma unroll 4
-    for (int r = 0; r < 16; ++r) {
-        const int m = tile_row(p.plan, tile, first + r);
-        if (m < 0) break;
+    const int rows = tile_row(p.plan, tile, first + (lane & 15));   // a lane's each
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int n = n0 + lane + 32 * c;
-            if (n >= p.width) continue;
-            float v = stage[r * 65 + lane + 32 * c];
-            if (p.base) v += one(static_cast<const X*>(p.base) + m * p.ldbase + n);
-            X* to = static_cast<X*>(p.out) + m * p.ldout + n;
-            if constexpr (is_f32<X>) *to = v;
-            else *reinterpret_cast<unsigned short*>(to) = narrow<X>(v);
+    for (int r0 = 0; r0 < 16; r0 += 8) {
+        float v[8][2];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int m = __shfl_sync(0xFFFFFFFFu, rows, r0 + r);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int n = n0 + lane + 32 * c;
+                v[r][c] = p.base && m >= 0 && n < p.width ? one(static_cast<const X*>(p.base) + m * p.ldbase + n) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int m = __shfl_sync(0xFFFFFFFFu, rows, r0 + r);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int n = n0 + lane + 32 * c;
+                if (m < 0 || n >= p.width) continue;
+                const float y = v[r][c] + stage[(r0 + r) * 65 + lane + 32 * c];
+                X* to = static_cast<X*>(p.out) + m * p.ldout + n;
+                if constexpr (is_f32<X>) *to = y;
+                else *reinterpret_cast<unsigned short*>(to) = narrow<X>(y);
+            }
         }
     }
 }
@@ -740,6 +754,7 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
     float* stage = reinterpret_cast<float*>(smem + p.rank8 * 16 * MT * 8) + warp * 16 * 65;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
+        if (gridDim.z > 1 && i != int(blockIdx.z)) continue;   // a CTA for each half: there are few tiles, and much to wait for
         float acc[8][4] = {};
         if (!none) up_products<X, W, VEC>(p, tile.x, n0, h, MT, i, acc);
         if constexpr (VEC) {
@@ -758,7 +773,7 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 template <class X, class W, int NT, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Args u)
 {
-    constexpr int COLS = 8 * NT, SUMS = Down<X, W, 1, NT>::smem(VEC);
+    constexpr int COLS = 8 * NT, SUMS = Down<X, W, 1, NT, BOTH_BUDGET>::smem(VEC);
     extern __shared__ __align__(16) unsigned char smem[];   // queue and sums, h, base or stage
     if (int(blockIdx.x) >= d.plan.head[0]) return;
     const int4 tile = d.plan.tiles[blockIdx.x];
@@ -769,8 +784,11 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
     unsigned* parts_h = reinterpret_cast<unsigned*>(smem + SUMS);
     const unsigned h = shared_address(parts_h), slots = h + COLS * 16 * 8;
     float* stage = reinterpret_cast<float*>(smem + SUMS + COLS * 16 * 8) + warp * 16 * 65;
+    const int first_n = (warp * shares + share) * 64;
+    if (VEC && u.base && first_n < u.width) issue_base<X>(u, row, first_n, slots);
+    if (VEC) copies_end();
     if (!none) {
-        const int n0 = (warp * shares + share) * 64;
+        const int n0 = first_n;
         if (n0 < u.width) {
             const W* w = static_cast<const W*>(u.w) + (long long)tile.x * u.rank * u.width + n0;
             for (int r = 2 * t; r < u.rank; r += 8)
@@ -780,7 +798,7 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(w + (long long)(r + e) * u.width + 8 * g));
         }
         float acc[1][NT][4] = {};
-        down_sums<X, W, 1, NT, VEC>(d, tile, 0, smem, share * WARPS + warp, WARPS * shares, acc);
+        down_sums<X, W, 1, NT, BOTH_BUDGET, VEC>(d, tile, 0, smem, share * WARPS + warp, WARPS * shares, acc);
         const float scale = u.scale ? u.scale[tile.x] : 1.f;
         const float* red = gather_sums(smem, acc, true);
         if (shares > 1) cluster_sync();
@@ -804,8 +822,8 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
         if (shares > 1) cluster_sync();   // nobody leaves while its sums are being read
         else __syncthreads();
     }
-    for (int n0 = (warp * shares + share) * 64; n0 < u.width; n0 += WARPS * shares * 64) {
-        if (VEC && u.base) {
+    for (int n0 = first_n; n0 < u.width; n0 += WARPS * shares * 64) {
+        if (VEC && u.base && n0 != first_n) {
             __syncwarp();
             issue_base<X>(u, row, n0, slots);
         }
@@ -820,7 +838,7 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
     }
 }
 template <class X, class W, int NT>
-constexpr int both_smem(bool vec) { return Down<X, W, 1, NT>::smem(vec) + 8 * NT * 16 * 8 + (vec ? base_bytes<X> : WARPS * 16 * 65 * 4); }
+constexpr int both_smem(bool vec) { return Down<X, W, 1, NT, BOTH_BUDGET>::smem(vec) + 8 * NT * 16 * 8 + (vec ? base_bytes<X> : WARPS * 16 * 65 * 4); }
 
 // Many rows: up_kernel's product for 256 columns and a run of consecutive tiles of 32 rows.  The adapter's part of `w` stays in shared memory
 // until a tile of another adapter comes (up_kernel reads it from L2 for every tile, and waits for it), and the next tile's

@@ -24,10 +24,12 @@ __global__ void __launch_bounds__(256) pad_kernel(const unsigned short* __restri
 __device__ __forceinline__ bool counted(long long t, long long ignore) { return t != ignore; }
 
 // loss and log-sum-exp of 32 rows (a lane's each); the warps share the tiles out.  The loss is log(sum) + (max - logit), so that a
-// row that is sure of its target keeps the digits that lse - logit would lose.
+// row that is sure of its target keeps the digits that lse - logit would lose.  The CTA that is done last sums all rows up, in double and
+// in a fixed order, whichever it is.
 __global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ partial, int tiles, const float* __restrict__ at_target,
                                                    const long long* __restrict__ target, long long ignore, int rows, int vocabulary,
-                                                   float* __restrict__ lse, float* __restrict__ each)
+                                                   float* __restrict__ lse, float* each, int reduction, int* ticket, float* __restrict__ loss,
+                                                   float* __restrict__ count)
 {
     __shared__ float2 part[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
@@ -43,75 +45,88 @@ __global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ pa
     }
     part[warp][lane] = make_float2(top, sum);
     __syncthreads();
-    if (warp || row >= rows) return;
-    top = -INFINITY, sum = 0.f;
+    if (warp == 0 && row < rows) {
+        top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) add(part[w][lane]);
-    const float l = logf(sum);
-    lse[row] = top + l;
-    const long long t = target[row];
-    if (!counted(t, ignore)) each[row] = 0.f;
-    else if (t < 0 || t >= vocabulary) each[row] = __int_as_float(0x7FC00000);   // no such target: not a number
-    else each[row] = l + (top - at_target[row]);
-}
-
-// Sum or mean of the rows' losses in double, in a fixed order, and the number of rows that count.
-__global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ each, const long long* __restrict__ target, long long ignore, int rows,
-                                                      int reduction, float* __restrict__ loss, float* __restrict__ count)
-{
-    __shared__ double sums[32];
-    __shared__ int counts[32];
+        for (int w = 0; w < 8; ++w) add(part[w][lane]);
+        const float l = logf(sum);
+        lse[row] = top + l;
+        const long long t = target[row];
+        if (!counted(t, ignore)) each[row] = 0.f;
+        else if (t < 0 || t >= vocabulary) each[row] = __int_as_float(0x7FC00000);   // no such target: not a number
+        else each[row] = l + (top - at_target[row]);
+    }
+    if (reduction == DS_LOSS_NONE) return;
+    __shared__ bool last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(ticket, 1) == int(gridDim.x) - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    __shared__ double sums[8];
+    __shared__ int counts[8];
     double s = 0.0;
     int n = 0;
-    for (int i = threadIdx.x; i < rows; i += 1024) {
+    for (int i = threadIdx.x; i < rows; i += 256) {
         const bool c = counted(target[i], ignore);
         n += c;
-        if (c) s += each[i];
+        if (c) s += __ldcg(each + i);
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
         s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
         n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
     }
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s, counts[threadIdx.x >> 5] = n;
+    if (lane == 0) sums[warp] = s, counts[warp] = n;
     __syncthreads();
     if (threadIdx.x) return;
     s = 0.0, n = 0;
-    for (int i = 0; i < 32; ++i) s += sums[i], n += counts[i];
+    for (int i = 0; i < 8; ++i) s += sums[i], n += counts[i];
     *count = float(n);
-    if (reduction == DS_LOSS_SUM) *loss = float(s);
-    if (reduction == DS_LOSS_MEAN) *loss = float(s / n);   // no row counts: 0 / 0
+    *loss = float(reduction == DS_LOSS_MEAN ? s / n : s);   // no row counts: 0 / 0
 }
 
-// Weight of each row in G, at most `top` in magnitude so that 16 bits hold it (2^15 for fp16, whose small numbers run out at
-// 2^-24: a probability of 10^-8 keeps eight digits' worth of bits), and the factor that takes it back.
+__global__ void no_rows_kernel(int reduction, float* loss, float* count)
+{
+    *count = 0.f;
+    *loss = reduction == DS_LOSS_MEAN ? __int_as_float(0x7FC00000) : 0.f;
+}
+
+// Losses of their own gradients: the weight of each row in G, at most `top` in magnitude, and the factor that takes it back.
 __global__ void __launch_bounds__(1024) weights_kernel(const float* __restrict__ grad, const long long* __restrict__ target, long long ignore, int rows,
-                                                       int vocabulary, int reduction, const float* __restrict__ count, float top,
-                                                       float* __restrict__ weight, float* __restrict__ scale)
+                                                       float top, float* __restrict__ weight, float* __restrict__ scale)
 {
     __shared__ float most[32];
     float m = 0.f;
-    if (reduction == DS_LOSS_NONE) {
-        for (int i = threadIdx.x; i < rows; i += 1024)
-            if (counted(target[i], ignore)) m = fmaxf(m, fabsf(grad[i]));
+    for (int i = threadIdx.x; i < rows; i += 1024)
+        if (counted(target[i], ignore)) m = fmaxf(m, fabsf(grad[i]));
 #pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-        if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = m;
-        __syncthreads();
-        m = 0.f;
-        for (int i = 0; i < 32; ++i) m = fmaxf(m, most[i]);
-        if (!(m > 0.f) || m > 3e38f) m = 1.f;
-    } else {
-        m = *grad;
-        if (reduction == DS_LOSS_MEAN) m = *count > 0.f ? m / *count : 0.f;
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = 0.f;
+    for (int i = 0; i < 32; ++i) m = fmaxf(m, most[i]);
+    if (!(m > 0.f) || m > 3e38f) m = 1.f;
+    for (int i = threadIdx.x; i < rows; i += 1024) weight[i] = counted(target[i], ignore) ? grad[i] / m * top : 0.f;
+    if (threadIdx.x == 0) *scale = m;
+}
+
+// Parts of a product's sums, added up in their order.
+__global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ acc, int parts, long long n, const __grid_constant__ Params p,
+                                                    unsigned short* __restrict__ out)
+{
+    const float scale = out_scale(p);
+    for (long long i = (blockIdx.x * 256ll + threadIdx.x) * 2; i < n; i += gridDim.x * 512ll) {
+        float a = 0.f, b = 0.f;
+        for (int q = 0; q < parts; ++q) {
+            a += acc[q * n + i];
+            if (i + 1 < n) b += acc[q * n + i + 1];
+        }
+        const unsigned w = pack2(a * scale, b * scale, p.is_bf16);
+        out[i] = (unsigned short)w;
+        if (i + 1 < n) out[i + 1] = (unsigned short)(w >> 16);
     }
-    for (int i = threadIdx.x; i < rows; i += 1024) {
-        const long long t = target[i];
-        if (!counted(t, ignore)) weight[i] = 0.f;
-        else if (t < 0 || t >= vocabulary) weight[i] = __int_as_float(0x7FC00000);   // as its loss
-        else weight[i] = reduction == DS_LOSS_NONE ? grad[i] / m * top : top;
-    }
-    if (threadIdx.x == 0) *scale = m / top;
 }
 
 // ---- launches ----
@@ -134,6 +149,11 @@ EncodeFn encode_fn()
 // A matrix [rows][width] of 16-bit values, rows `stride` elements apart, in boxes of 64 elements x box_rows.
 bool encode(CUtensorMap* map, const void* p, long long rows, int width, long long stride, int box_rows, bool is_bf16)
 {
+    // a thread that has made no call of the runtime yet (autograd's) has no context, and the driver's function wants one
+    static thread_local bool current = false;
+    int dev;
+    if (!current && (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)) return false;
+    current = true;
     const cuuint64_t dims[2] = {cuuint64_t(width), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride) * 2};
     const cuuint32_t box[2] = {64, cuuint32_t(box_rows)}, steps[2] = {1, 1};
     return encode_fn()(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p), dims, strides, box,
@@ -150,42 +170,86 @@ int multiprocessors()
     return known[dev];
 }
 
-template <int PAIR, int MODE>
-int launch(const CUtensorMap& a, const CUtensorMap& b, Params p, cudaStream_t st)
+// Shapes of a tile: two CTAs and 256 x 256, one and 128 x 256, one and 128 x 128.
+struct TileShape {
+    int pair, bn;
+};
+constexpr TileShape SHAPES[3] = {{2, 256}, {1, 256}, {1, 128}};
+
+int tiles_of(const TileShape& s, int m, int n) { return (m + 128 * s.pair - 1) / (128 * s.pair) * ((n + s.bn - 1) / s.bn); }
+
+// The shape that is done first: rounds of tiles over the SMs, each as long as its k steps take (512 cycles at the tensor core's pace; a single
+// CTA's tiles are held up by shared memory, which reads and fills one of both operands twice as often) and an epilogue that the last round
+// shows.  Measured on 2048 x 1024 -> 32000, cycles a step: 530, 570, 420.
+int tile_shape(const Product* q, int products, int sms)
+{
+    static const int step[3] = {530, 570, 420}, tail[3] = {4000, 4000, 2500};
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < 3; ++i) {
+        const int slots = sms / SHAPES[i].pair;
+        double work = 0;
+        long long tiles = 0, longest = 0;
+        for (int j = 0; j < products; ++j) {
+            const long long n = (long long)tiles_of(SHAPES[i], q[j].m_end, q[j].n_end) * q[j].splits, k = (q[j].k_steps + q[j].splits - 1) / q[j].splits;
+            tiles += n;
+            work += double(n) * k;
+            longest = k > longest ? k : longest;
+        }
+        const long long rounds = (tiles + slots - 1) / slots;
+        const double steps = products == 1 ? double(rounds) * q[0].k_steps / q[0].splits : work / slots + longest;
+        const double cost = steps * step[i] + tail[i];
+        if (i == 0 || cost < least) least = cost, best = i;
+    }
+    return best;
+}
+
+template <int PAIR, int BN, int MODE>
+int launch_shape(const Maps& maps, Params& p, int tiles, int sms, cudaStream_t st)
 {
     static bool done[kMaxDevices];
-    const int dev = device_slot(), sms = multiprocessors();
-    p.err_flag = kernel_error_flag();
-    if (dev < 0 || !sms || !p.err_flag) return DS_ERR_CUDA;
+    const int dev = device_slot();
+    if (dev < 0) return DS_ERR_CUDA;
+    constexpr int smem = Shape<PAIR, BN>::SMEM_BYTES;
     if (!done[dev]) {
-        if (cudaFuncSetAttribute(tile_kernel<PAIR, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return DS_ERR_CUDA;
+        if (cudaFuncSetAttribute(tile_kernel<PAIR, BN, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return DS_ERR_CUDA;
         done[dev] = true;
     }
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    if (tiles > INT_MAX) return DS_ERR_RANGE;
     const int most = sms / PAIR;
-    p.group = 8;
-    tile_kernel<PAIR, MODE><<<unsigned(tiles < most ? tiles : most) * PAIR, THREADS, SMEM_BYTES, st>>>(a, b, p);
+    tile_kernel<PAIR, BN, MODE><<<unsigned(tiles < most ? tiles : most) * PAIR, THREADS, smem, st>>>(maps, p);
     note_launch();
     return cudaGetLastError() == cudaSuccess ? DS_OK : DS_ERR_CUDA;
 }
 
+// Launches the first `products` of p in tiles of a shape (SHAPES).
 template <int MODE>
-int launch(int pair, const CUtensorMap& a, const CUtensorMap& b, Params p, cudaStream_t st)
+int launch(const Maps& maps, Params p, int products, int shape, cudaStream_t st)
 {
-    p.tiles_m = (p.m_end + 128 * pair - 1) / (128 * pair);
-    const int n = MODE == GRAD ? p.ldg : p.n_end;
-    p.tiles_n = (n + 128 * pair - 1) / (128 * pair);
-    return pair == 2 ? launch<2, MODE>(a, b, p, st) : launch<1, MODE>(a, b, p, st);
+    const int sms = multiprocessors();
+    p.err_flag = kernel_error_flag();
+    if (!sms || !p.err_flag) return DS_ERR_CUDA;
+    long long tiles = 0;
+    for (int i = 0; i < products; ++i) {
+        Product& q = p.product[i];
+        q.tiles_m = (q.m_end + 128 * SHAPES[shape].pair - 1) / (128 * SHAPES[shape].pair);
+        q.tiles_n = (q.n_end + SHAPES[shape].bn - 1) / SHAPES[shape].bn;
+        q.group = 8;
+        tiles += (long long)q.tiles_m * q.tiles_n * q.splits;
+    }
+    if (tiles > INT_MAX) return DS_ERR_RANGE;
+    if (shape == 0) return launch_shape<2, 256, MODE>(maps, p, int(tiles), sms, st);
+    if (shape == 1) return launch_shape<1, 256, MODE>(maps, p, int(tiles), sms, st);
+    return launch_shape<1, 128, MODE>(maps, p, int(tiles), sms, st);
 }
 
 // ---- layout of a call's scratch ----
 struct Layout {
     int dp;                 // width of a row of the operands that TMA reads
     long long h, w;         // copies of them, or -1
-    long long partial, at_target;   // forward
-    long long weight, scale, g, acc;  // backward
+    long long partial, at_target, ticket;   // forward
+    long long weight, scale, g, acc;        // backward
     int piece;              // columns of the vocabulary at a time
+    int parts;              // in which the sums of dH are formed
     long long bytes;
 };
 
@@ -201,7 +265,15 @@ int piece_of(long long rows, int v)
     return int(c < all ? c : all);
 }
 
-int pair_of(int rows) { return rows > 128 ? 2 : 1; }
+// Parts of the k steps of dH = G W: few tiles with a long sum each would run on long after those of dW.  As many as bring a part below what
+// the launch has for each SM; 8 at most.
+int parts_of(int rows, int d, int piece)
+{
+    const long long h = (long long)tiles_of(SHAPES[1], rows, d) * (piece / BK), w = (long long)tiles_of(SHAPES[1], piece, d) * ((rows + BK - 1) / BK);
+    int parts = 1;
+    while (parts < 8 && piece / BK / parts > (h + w) / 148 && piece / BK / parts >= 16) parts *= 2;
+    return parts;
+}
 
 Layout layout(int rows, int d, int v, bool backward, bool copies)
 {
@@ -219,12 +291,14 @@ Layout layout(int rows, int d, int v, bool backward, bool copies)
     if (!backward) {
         l.partial = take((v + 127ll) / 128 * rows * 8);
         l.at_target = take(rows * 4ll);
+        l.ticket = take(4);
     } else {
         l.piece = piece_of(rows, v);
         l.weight = take(rows * 4ll);
         l.scale = take(4);
         l.g = take((long long)rows * l.piece * 2);
-        l.acc = l.piece < v ? take((long long)rows * d * 4) : -1;
+        l.parts = l.piece < v ? 1 : parts_of(rows, d, l.piece);   // a last piece may have fewer steps than parts
+        l.acc = l.piece < v || l.parts > 1 ? take((long long)l.parts * rows * d * 4) : -1;
     }
     l.bytes = at;
     return l;
@@ -281,23 +355,25 @@ extern "C" int ds_loss_forward(const ds_loss_t* a, void* stream)
             if (const int e = pad(w, scratch + l.w, a->v, a->d, l.dp, st)) return e;
             h = scratch + l.h, w = scratch + l.w;
         }
-        CUtensorMap map_h, map_w;
+        Maps maps;
         const bool bf = a->type == DS_T_BF16;
-        if (!encode(&map_h, h, a->rows, l.dp, l.dp, CTA_ROWS, bf) || !encode(&map_w, w, a->v, l.dp, l.dp, CTA_ROWS, bf)) return DS_ERR_CUDA;
+        if (!encode(&maps.a[0], h, a->rows, l.dp, l.dp, CTA_ROWS, bf) || !encode(&maps.b[0], w, a->v, l.dp, l.dp, CTA_ROWS, bf)) return DS_ERR_CUDA;
         Params p = {};
-        p.k_steps = (l.dp + BK - 1) / BK, p.is_bf16 = bf;
-        p.m_end = a->rows, p.n_end = a->v;
+        Product& q = p.product[0];
+        q.splits = 1, q.k_steps = (l.dp + BK - 1) / BK;
+        q.m_end = a->rows, q.n_end = a->v;
+        p.is_bf16 = bf;
         p.target = reinterpret_cast<const long long*>(a->target);
         p.partial = reinterpret_cast<float2*>(scratch + l.partial);
         p.at_target = reinterpret_cast<float*>(scratch + l.at_target);
-        const int pair = pair_of(a->rows);
-        if (const int e = launch<STATS>(pair, map_h, map_w, p, st)) return e;
-        rows_kernel<<<(a->rows + 31) / 32, 256, 0, st>>>(p.partial, (a->v + 128 * pair - 1) / (128 * pair), p.at_target, p.target, a->ignore_index, a->rows,
-                                                         a->v, a->lse, a->each);
+        p.ticket = reinterpret_cast<int*>(scratch + l.ticket);
+        const int shape = tile_shape(&q, 1, multiprocessors());
+        if (const int e = launch<STATS>(maps, p, 1, shape, st)) return e;
+        rows_kernel<<<(a->rows + 31) / 32, 256, 0, st>>>(p.partial, (a->v + SHAPES[shape].bn - 1) / SHAPES[shape].bn, p.at_target, p.target, a->ignore_index,
+                                                         a->rows, a->v, a->lse, a->each, a->reduction, p.ticket, a->loss, a->count);
         ds::note_launch();
-    }
-    if (a->reduction != DS_LOSS_NONE) {
-        reduce_kernel<<<1, 1024, 0, st>>>(a->each, reinterpret_cast<const long long*>(a->target), a->ignore_index, a->rows, a->reduction, a->loss, a->count);
+    } else if (a->reduction != DS_LOSS_NONE) {
+        no_rows_kernel<<<1, 1, 0, st>>>(a->reduction, a->loss, a->count);
         ds::note_launch();
     }
     return cudaGetLastError() == cudaSuccess ? DS_OK : DS_ERR_CUDA;
@@ -325,50 +401,67 @@ extern "C" int ds_loss_backward(const ds_loss_t* a, void* stream)
         h = scratch + l.h, w = scratch + l.w;
     }
     const bool bf = a->type == DS_T_BF16;
-    float* weight = reinterpret_cast<float*>(scratch + l.weight);
-    float* scale = reinterpret_cast<float*>(scratch + l.scale);
-    weights_kernel<<<1, 1024, 0, st>>>(a->grad, reinterpret_cast<const long long*>(a->target), a->ignore_index, a->rows, a->v,
-                                       a->reduction, a->count, bf ? 1.f : 32768.f, weight, scale);
-    ds::note_launch();
-    const int pair = pair_of(a->rows);
-    CUtensorMap rows_h, cols_h;   // hidden with k along its rows, and with k across them
-    if (!encode(&rows_h, h, a->rows, l.dp, l.dp, CTA_ROWS, bf) || !encode(&cols_h, h, a->rows, l.dp, l.dp, BK, bf)) return DS_ERR_CUDA;
+    Params p = {};
+    p.is_bf16 = bf;
+    p.target = reinterpret_cast<const long long*>(a->target);
+    p.ignore = a->ignore_index;
+    p.lse = a->lse;
+    p.vocabulary = a->v;
+    // fp16's small numbers run out at 2^-24: G begins at 2^15, so that a probability of 10^-8 keeps eight bits
+    p.top = bf ? 1.f : 32768.f;
+    p.scale = a->grad;
+    if (a->reduction == DS_LOSS_MEAN) p.count = a->count;
+    if (a->reduction == DS_LOSS_NONE) {
+        float *weight = reinterpret_cast<float*>(scratch + l.weight), *scale = reinterpret_cast<float*>(scratch + l.scale);
+        weights_kernel<<<1, 1024, 0, st>>>(a->grad, p.target, a->ignore_index, a->rows, p.top, weight, scale);
+        ds::note_launch();
+        p.row_weight = weight, p.scale = scale;
+    }
+    const int sms = multiprocessors();
     const unsigned short* w16 = static_cast<const unsigned short*>(w);
+    unsigned short* g = reinterpret_cast<unsigned short*>(scratch + l.g);
+    float* acc = l.acc < 0 ? nullptr : reinterpret_cast<float*>(scratch + l.acc);
     for (int first = 0; first < a->v; first += l.piece) {
         const int cols = a->v - first < l.piece ? a->v - first : l.piece;
         const int ldg = (cols + 63) / 64 * 64;
-        unsigned short* g = reinterpret_cast<unsigned short*>(scratch + l.g);
-        CUtensorMap rows_w, cols_w, rows_g, cols_g;
         const void* wp = w16 + (long long)first * l.dp;
-        if (!encode(&rows_w, wp, cols, l.dp, l.dp, CTA_ROWS, bf) || !encode(&cols_w, wp, cols, l.dp, l.dp, BK, bf) ||
-            !encode(&rows_g, g, a->rows, ldg, ldg, CTA_ROWS, bf) || !encode(&cols_g, g, a->rows, ldg, ldg, BK, bf))
-            return DS_ERR_CUDA;
-        Params p = {};
-        p.is_bf16 = bf;
-        p.k_steps = (l.dp + BK - 1) / BK;
-        p.m_end = a->rows, p.n_end = cols;
-        p.target = reinterpret_cast<const long long*>(a->target);
-        p.lse = a->lse, p.row_weight = weight, p.n_first = first;
+        Maps maps;
+        if (!encode(&maps.a[0], h, a->rows, l.dp, l.dp, CTA_ROWS, bf) || !encode(&maps.b[0], wp, cols, l.dp, l.dp, CTA_ROWS, bf)) return DS_ERR_CUDA;
+        Product z = {};
+        z.splits = 1, z.k_steps = (l.dp + BK - 1) / BK;
+        z.m_end = a->rows, z.n_end = cols;
+        p.product[0] = z;
+        p.n_first = first;
         p.g = g, p.ldg = ldg;
-        if (const int e = launch<GRAD>(pair, rows_h, rows_w, p, st)) return e;
-        p.scale = scale;
+        if (const int e = launch<GRAD>(maps, p, 1, tile_shape(&z, 1, sms), st)) return e;
+        int n = 0;
         if (a->dhidden) {   // dH (+)= G W
-            Params q = p;
-            q.k_steps = ldg / BK, q.b_mn = 1;
-            q.n_end = a->d;
-            q.acc = l.acc < 0 ? nullptr : reinterpret_cast<float*>(scratch + l.acc);
-            q.first = first == 0, q.last = first + cols == a->v;
+            Product& q = p.product[n] = {};
+            q.splits = l.parts, q.k_steps = ldg / BK, q.b_mn = 1;
+            q.m_end = a->rows, q.n_end = a->d;
+            q.acc = acc;
+            q.first = first == 0, q.last = l.parts == 1 && first + cols == a->v;
             q.out = static_cast<unsigned short*>(a->dhidden);
-            if (const int e = launch<PRODUCT>(pair, rows_g, cols_w, q, st)) return e;
+            if (!encode(&maps.a[n], g, a->rows, ldg, ldg, CTA_ROWS, bf) || !encode(&maps.b[n], wp, cols, l.dp, l.dp, BK, bf)) return DS_ERR_CUDA;
+            ++n;
         }
         if (a->dweight) {   // dW of the piece = G^T H
-            Params q = p;
-            q.k_steps = (a->rows + BK - 1) / BK, q.a_mn = q.b_mn = 1;
+            Product& q = p.product[n] = {};
+            q.splits = 1, q.k_steps = (a->rows + BK - 1) / BK, q.a_mn = q.b_mn = 1;
             q.m_end = cols, q.n_end = a->d;
-            q.acc = nullptr, q.first = q.last = 1;
+            q.first = q.last = 1;
             q.out = static_cast<unsigned short*>(a->dweight) + (long long)first * a->d;
-            if (const int e = launch<PRODUCT>(pair, cols_g, cols_h, q, st)) return e;
+            if (!encode(&maps.a[n], g, a->rows, ldg, ldg, BK, bf) || !encode(&maps.b[n], h, a->rows, l.dp, l.dp, BK, bf)) return DS_ERR_CUDA;
+            ++n;
         }
+        if (n == 1) p.product[1] = {};
+        if (n)
+            if (const int e = launch<PRODUCT>(maps, p, n, tile_shape(p.product, n, sms), st)) return e;
     }
-    return DS_OK;
+    if (a->dhidden && l.parts > 1) {
+        const long long n = (long long)a->rows * a->d, blocks = (n + 511) / 512;
+        parts_kernel<<<unsigned(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(acc, l.parts, n, p, static_cast<unsigned short*>(a->dhidden));
+        ds::note_launch();
+    }
+    return cudaGetLastError() == cudaSuccess ? DS_OK : DS_ERR_CUDA;
 }

@@ -10,7 +10,8 @@
 //
 // Bound by the tensor cores: one kernel for the four products, persistent, a pair of CTAs (two SMs) on one tile of 256 x 256, each
 // with half of both operands in shared memory (TMA, 128-byte swizzle, six stages of 64 k) and 128 rows of fp32 sums in tensor memory,
-// twice, so that one tile's epilogue runs beside the next one's products.  Up to 128 rows single CTAs take tiles of 128 x 128.
+// twice, so that one tile's epilogue runs beside the next one's products.  Where such tiles fill the SMs badly, single CTAs take tiles of
+// 128 x 256 or 128 x 128 (tile_shape in ds_loss.cu).  Both products of the backward pass share a launch.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -21,50 +22,95 @@
 namespace ds {
 namespace loss {
 
-constexpr int STAGES = 6, BK = 64, CTA_ROWS = 128;
-constexpr int TILE_BYTES = CTA_ROWS * BK * 2, STAGE_BYTES = 2 * TILE_BYTES;
+constexpr int BK = 64, CTA_ROWS = 128, A_BYTES = CTA_ROWS * BK * 2;
 constexpr int THREADS = 256;   // warp 0 loads, warp 1 multiplies, warps 4-7 are the epilogue: a warp reads the tensor-memory lanes of its number mod 4
 constexpr unsigned WAIT_NS = 2000000000u;
 
+// A tile of 128 PAIR x BN by PAIR CTAs; each holds 128 rows of one operand and BN / PAIR of the other.
+template <int PAIR, int BN>
+struct Shape {
+    static constexpr int B_ROWS = BN / PAIR, B_BYTES = B_ROWS * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 196608 / STAGE_BYTES;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+};
+
 struct Shared {
-    unsigned long long full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], done;
+    unsigned long long full[6], empty[6], acc_full[2], acc_empty[2], done;
     unsigned tmem;
     int err;
 };
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + int(sizeof(Shared));
+static_assert(sizeof(Shared) <= 256, "room behind the tiles");
 
 enum Mode { STATS, GRAD, PRODUCT };
 
-struct Params {
-    int tiles_m, tiles_n, k_steps, group;   // group: row tiles that neighbouring tiles of the order share
+// One product [m_end][n_end] = A B^T over k_steps steps of 64, cut into tiles, and in `splits` parts of the steps.
+struct Product {
+    int tiles_m, tiles_n, splits, k_steps, group;   // group: row tiles that neighbouring tiles of the order share
     int a_mn, b_mn;                         // operand lies with its rows (not k) contiguous
-    int is_bf16;
     int m_end, n_end;                       // rows and columns of the result
-    // STATS
+    // PRODUCT
+    float* acc;                             // [splits][m_end][n_end] sums of parts, or of several pieces, or null
+    int first, last;                        // of the pieces that acc sums; with parts none is the last, they are summed behind
+    unsigned short* out;
+};
+
+struct Params {
+    Product product[2];                     // the second one in mode PRODUCT alone
+    int is_bf16;
     const long long* target;
+    long long ignore;
+    // STATS
     float2* partial;                        // [tiles_n][m_end]: maximum, sum of exponentials
     float* at_target;                       // logit of the target
+    int* ticket;                            // zeroed for rows_kernel
     // GRAD
     const float* lse;
-    const float* row_weight;
+    const float* row_weight;                // or null: `top` for each row that counts
+    float top;
     long long n_first;                      // vocabulary index of column 0
+    int vocabulary;
     unsigned short* g;                      // [m_end][ldg]
     int ldg;
     // PRODUCT
-    float* acc;                             // [m_end][n_end] sums of several pieces, or null
-    int first, last;                        // of the pieces that acc sums
-    unsigned short* out;
-    const float* scale;
+    const float* scale;                     // one value, and where it is the mean's gradient, `count` to divide it by
+    const float* count;
     int* err_flag;
 };
 
+// What the products of G have to be multiplied by.
+__device__ __forceinline__ float out_scale(const Params& p)
+{
+    float s = *p.scale;
+    if (p.count) s = *p.count > 0.f ? s / *p.count : 0.f;
+    return s / p.top;
+}
+
 // Order of tiles: down `group` row tiles, then to the next column, so that tiles in work at once share both operands in L2.
-__device__ __forceinline__ void tile_at(const Params& p, int t, int& m, int& n)
+__device__ __forceinline__ void tile_at(const Product& p, int t, int& m, int& n)
 {
     const int per = p.group * p.tiles_n, block = t / per, first = block * p.group;
     const int high = min(p.group, p.tiles_m - first), in = t - block * per;
     m = first + in % high;
     n = in / high;
+}
+
+// Tile number t of a launch: its product, row and column, and the part of the k steps.
+struct Tile {
+    int which, m, n, part, k, k_end;
+};
+__device__ __forceinline__ Tile tile_of(const Params& p, int t)
+{
+    Tile x;
+    const int ahead = p.product[0].tiles_m * p.product[0].tiles_n * p.product[0].splits;
+    x.which = t >= ahead;
+    const Product& q = p.product[x.which];
+    t -= x.which ? ahead : 0;
+    const int tiles = q.tiles_m * q.tiles_n;
+    x.part = t / tiles;
+    tile_at(q, t - x.part * tiles, x.m, x.n);
+    x.k = int((long long)q.k_steps * x.part / q.splits);
+    x.k_end = int((long long)q.k_steps * (x.part + 1) / q.splits);
+    return x;
 }
 
 __device__ __forceinline__ unsigned cluster_rank()
@@ -100,15 +146,17 @@ __device__ __forceinline__ void load_box(unsigned dst, const CUtensorMap* map, i
                      : "memory");
 }
 
-// 128 rows of an operand, 64 k, from row `row` and index `k`: [row][k] in one box of 64 k x 128 rows, or, where rows are
-// contiguous, [k][row] in two boxes of 64 rows x 64 k.
-template <int PAIR>
+// ROWS rows of an operand, 64 k, from row `row` and index `k`: [row][k] in boxes of 64 k x 128 rows, or, where rows are
+// contiguous, [k][row] in boxes of 64 rows x 64 k.
+template <int PAIR, int ROWS>
 __device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap* map, int mn, int row, int k, unsigned bar)
 {
-    if (!mn) load_box<PAIR>(dst, map, k, row, bar);
-    else {
-        load_box<PAIR>(dst, map, row, k, bar);
-        load_box<PAIR>(dst + TILE_BYTES / 2, map, row + 64, k, bar);
+    if (!mn) {
+#pragma unroll
+        for (int i = 0; i < ROWS; i += 128) load_box<PAIR>(dst + i * BK * 2, map, k, row + i, bar);
+    } else {
+#pragma unroll
+        for (int i = 0; i < ROWS; i += 64) load_box<PAIR>(dst + i * BK * 2, map, row + i, k, bar);
     }
 }
 
@@ -116,7 +164,7 @@ __device__ __forceinline__ void load_tile(unsigned dst, const CUtensorMap* map, 
 // contiguous, k by 8 every 1024 bytes and rows by 64 every 8192.
 __device__ __forceinline__ unsigned long long descriptor(unsigned addr, int mn)
 {
-    const unsigned long long lead = mn ? (TILE_BYTES / 2) >> 4 : 1, stride = 1024 >> 4;
+    const unsigned long long lead = mn ? (64 * BK * 2) >> 4 : 1, stride = 1024 >> 4;
     return (unsigned long long)((addr & 0x3FFFFu) >> 4) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
 
@@ -180,12 +228,12 @@ __device__ __forceinline__ unsigned pack2(float lo, float hi, int is_bf16)
 }
 
 // One warp's 32 rows of a finished tile; `row` is this lane's, `tmem` the address of the sums of its first column.
-template <int PAIR, int MODE>
-__device__ __forceinline__ void epilogue(const Params& p, unsigned tmem, int row, int tile_n)
+template <int BN, int MODE>
+__device__ __forceinline__ void epilogue(const Params& p, const Tile& tile, unsigned tmem, int row)
 {
-    constexpr int BN = 128 * PAIR;
-    const int n0 = tile_n * BN, cols = min(BN, p.n_end - n0);
-    const bool live = row < p.m_end;
+    const Product& q = p.product[MODE == PRODUCT ? tile.which : 0];
+    const int n0 = tile.n * BN, cols = min(BN, q.n_end - n0);
+    const bool live = row < q.m_end;
     if constexpr (MODE == STATS) {
         const long long t = live ? p.target[row] - n0 : -1;
         float top = -INFINITY, sum = 0.f;
@@ -214,12 +262,14 @@ __device__ __forceinline__ void epilogue(const Params& p, unsigned tmem, int row
             sum += (part[0] + part[1]) + (part[2] + part[3]);
             top = next;
         }
-        if (live) p.partial[(long long)tile_n * p.m_end + row] = make_float2(top, sum);
+        if (live) p.partial[(long long)tile.n * q.m_end + row] = make_float2(top, sum);
     } else if constexpr (MODE == GRAD) {
         // p = exp(z - lse); 1 comes off at the target before the rounding to 16 bits, which is one of half a unit in the last
         // place of each element.  A weight of 0 makes the row 0 whatever its logits are.
-        const long long t = live ? p.target[row] - p.n_first - n0 : -1;
-        const float lse = live ? p.lse[row] : 0.f, weight = live ? p.row_weight[row] : 0.f;
+        const long long at = live ? p.target[row] : p.ignore, t = at - p.n_first - n0;
+        const float lse = live ? p.lse[row] : 0.f;
+        float weight = at == p.ignore ? 0.f : p.row_weight ? p.row_weight[row] : p.top;
+        if (at != p.ignore && (at < 0 || at >= p.vocabulary)) weight = __int_as_float(0x7FC00000);   // no such target: not a number
         const int width = min(BN, p.ldg - n0);
         for (int c = 0; c < width; c += 32) {
             int v[32];
@@ -231,9 +281,9 @@ __device__ __forceinline__ void epilogue(const Params& p, unsigned tmem, int row
                 float e[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float q = exp2_fast((__int_as_float(v[i + j]) - lse) * LOG2E);
-                    if (t == c + i + j) q -= 1.f;
-                    e[j] = weight == 0.f || c + i + j >= cols ? 0.f : q * weight;
+                    float x = exp2_fast((__int_as_float(v[i + j]) - lse) * LOG2E);
+                    if (t == c + i + j) x -= 1.f;
+                    e[j] = weight == 0.f || c + i + j >= cols ? 0.f : x * weight;
                 }
                 w[i / 2] = pack2(e[0], e[1], p.is_bf16);
             }
@@ -244,7 +294,8 @@ __device__ __forceinline__ void epilogue(const Params& p, unsigned tmem, int row
             }
         }
     } else {
-        const float scale = p.last ? *p.scale : 0.f;
+        const float scale = q.last ? out_scale(p) : 0.f;
+        float* acc = q.acc + (long long)tile.part * q.m_end * q.n_end;
         for (int c = 0; c < cols; c += 32) {
             int v[32];
             __syncwarp();
@@ -253,29 +304,29 @@ __device__ __forceinline__ void epilogue(const Params& p, unsigned tmem, int row
             float f[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = __int_as_float(v[i]);
-            const long long at = (long long)row * p.n_end + n0 + c;
-            const bool whole = cols - c >= 32 && p.n_end % 8 == 0;   // 16-byte stores
-            if (p.acc && !p.first) {
+            const long long at = (long long)row * q.n_end + n0 + c;
+            const bool whole = cols - c >= 32 && q.n_end % 8 == 0;   // 16-byte stores
+            if (q.acc && !q.first) {
                 if (whole) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        const float4 a = *reinterpret_cast<const float4*>(p.acc + at + i);
+                        const float4 a = *reinterpret_cast<const float4*>(acc + at + i);
                         f[i] += a.x, f[i + 1] += a.y, f[i + 2] += a.z, f[i + 3] += a.w;
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (c + i < cols) f[i] += p.acc[at + i];
+                        if (c + i < cols) f[i] += acc[at + i];
                 }
             }
-            if (!p.last) {
+            if (!q.last) {
                 if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(p.acc + at + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(acc + at + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (c + i < cols) p.acc[at + i] = f[i];
+                        if (c + i < cols) acc[at + i] = f[i];
                 }
                 continue;
             }
@@ -285,24 +336,29 @@ __device__ __forceinline__ void epilogue(const Params& p, unsigned tmem, int row
             if (whole) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    reinterpret_cast<uint4*>(p.out + at)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    reinterpret_cast<uint4*>(q.out + at)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    if (c + i < cols) p.out[at + i] = (unsigned short)(w[i / 2] >> (16 * (i & 1)));
+                    if (c + i < cols) q.out[at + i] = (unsigned short)(w[i / 2] >> (16 * (i & 1)));
             }
         }
     }
 }
 
-template <int PAIR, int MODE>
+struct Maps {
+    CUtensorMap a[2], b[2];   // of both products
+};
+
+template <int PAIR, int BN, int MODE>
 __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(PAIR, 1, 1)
-    tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params p)
+    tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p)
 {
-    constexpr int BN = 128 * PAIR;
+    using S = Shape<PAIR, BN>;
+    constexpr int STAGES = S::STAGES;
     extern __shared__ unsigned char raw[];
     unsigned char* tiles = raw + (1024 - (s32(raw) & 1023)) % 1024;
-    Shared& s = *reinterpret_cast<Shared*>(tiles + STAGES * STAGE_BYTES);
+    Shared& s = *reinterpret_cast<Shared*>(tiles + STAGES * S::STAGE_BYTES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned rank = PAIR == 2 ? cluster_rank() : 0;
     volatile int* err = &s.err;
@@ -325,25 +381,29 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(PAIR, 1, 1)
     if (PAIR == 2) cluster_sync();
     tc_fence_after();
     const unsigned tmem = s.tmem;
-    const int total = p.tiles_m * p.tiles_n, mine = blockIdx.x / PAIR, step = gridDim.x / PAIR;
+    int total = p.product[0].tiles_m * p.product[0].tiles_n * p.product[0].splits;
+    if (MODE == PRODUCT) total += p.product[1].tiles_m * p.product[1].tiles_n * p.product[1].splits;
+    const int mine = blockIdx.x / PAIR, step = gridDim.x / PAIR;
+    if (MODE == STATS && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
 
     if (warp == 0) {
         if (elect_one()) {
             unsigned stage = 0, phase = 1;   // a fresh barrier is past the phase before its first
-            for (int t = mine; t < total && !*err; t += step) {
-                int m, n;
-                tile_at(p, t, m, n);
-                const int row_a = m * BN + int(rank) * CTA_ROWS, row_b = n * BN + int(rank) * CTA_ROWS;
-                for (int k = 0; k < p.k_steps; ++k) {
+            for (int i = mine; i < total && !*err; i += step) {
+                const Tile t = tile_of(p, i);
+                const Product& q = p.product[MODE == PRODUCT ? t.which : 0];
+                const CUtensorMap *map_a = &maps.a[MODE == PRODUCT ? t.which : 0], *map_b = &maps.b[MODE == PRODUCT ? t.which : 0];
+                const int row_a = t.m * CTA_ROWS * PAIR + int(rank) * CTA_ROWS, row_b = t.n * BN + int(rank) * S::B_ROWS;
+                for (int k = t.k; k < t.k_end; ++k) {
                     if (!bar_wait(&s.empty[stage], phase, err, WAIT_NS)) break;
                     const unsigned bar = PAIR == 2 ? in_leader(&s.full[stage]) : s32(&s.full[stage]);
                     if (rank == 0)
                         asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(s32(&s.full[stage])),
-                                     "n"(STAGE_BYTES * PAIR)
+                                     "n"(S::STAGE_BYTES * PAIR)
                                      : "memory");
-                    const unsigned at = s32(tiles) + stage * STAGE_BYTES;
-                    load_tile<PAIR>(at, &map_a, p.a_mn, row_a, k * BK, bar);
-                    load_tile<PAIR>(at + TILE_BYTES, &map_b, p.b_mn, row_b, k * BK, bar);
+                    const unsigned at = s32(tiles) + stage * S::STAGE_BYTES;
+                    load_tile<PAIR, CTA_ROWS>(at, map_a, q.a_mn, row_a, k * BK, bar);
+                    load_tile<PAIR, S::B_ROWS>(at + A_BYTES, map_b, q.b_mn, row_b, k * BK, bar);
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                 }
             }
@@ -354,22 +414,24 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(PAIR, 1, 1)
     } else if (warp == 1 && rank == 0) {
         if (elect_one()) {
             const unsigned type = p.is_bf16 ? 1 : 0;
-            const unsigned idesc = 1u << 4 | type << 7 | type << 10 | unsigned(p.a_mn) << 15 | unsigned(p.b_mn) << 16 | unsigned(BN / 8) << 17 |
-                                   unsigned(CTA_ROWS * PAIR / 16) << 24;
-            const unsigned step_a = p.a_mn ? 2048 >> 4 : 32 >> 4, step_b = p.b_mn ? 2048 >> 4 : 32 >> 4;   // 16 k further on
             unsigned stage = 0, phase = 0, buf = 0, buf_phase = 1;
-            for (int t = mine; t < total; t += step) {
+            for (int i = mine; i < total; i += step) {
+                const Tile t = tile_of(p, i);
+                const Product& q = p.product[MODE == PRODUCT ? t.which : 0];
+                const unsigned idesc = 1u << 4 | type << 7 | type << 10 | unsigned(q.a_mn) << 15 | unsigned(q.b_mn) << 16 | unsigned(BN / 8) << 17 |
+                                       unsigned(CTA_ROWS * PAIR / 16) << 24;
+                const unsigned step_a = q.a_mn ? 2048 >> 4 : 32 >> 4, step_b = q.b_mn ? 2048 >> 4 : 32 >> 4;   // 16 k further on
                 if (!bar_wait(&s.acc_empty[buf], buf_phase, err, WAIT_NS)) break;
                 tc_fence_after();
                 const unsigned d = tmem + buf * BN;
                 bool ok = true;
-                for (int k = 0; k < p.k_steps; ++k) {
+                for (int k = t.k; k < t.k_end; ++k) {
                     if (!(ok = bar_wait(&s.full[stage], phase, err, WAIT_NS))) break;
                     tc_fence_after();
-                    const unsigned at = s32(tiles) + stage * STAGE_BYTES;
-                    const unsigned long long a = descriptor(at, p.a_mn), b = descriptor(at + TILE_BYTES, p.b_mn);
+                    const unsigned at = s32(tiles) + stage * S::STAGE_BYTES;
+                    const unsigned long long a = descriptor(at, q.a_mn), b = descriptor(at + A_BYTES, q.b_mn);
 #pragma unroll
-                    for (int i = 0; i < BK / 16; ++i) mma<PAIR>(d, a + i * step_a, b + i * step_b, idesc, (k | i) != 0);
+                    for (int j = 0; j < BK / 16; ++j) mma<PAIR>(d, a + j * step_a, b + j * step_b, idesc, k > t.k || j);
                     commit<PAIR>(&s.empty[stage]);
                     if (++stage == STAGES) stage = 0, phase ^= 1;
                 }
@@ -382,12 +444,11 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(PAIR, 1, 1)
     } else if (warp >= 4) {
         unsigned buf = 0, buf_phase = 0;
         const int quarter = warp & 3;
-        for (int t = mine; t < total; t += step) {
-            int m, n;
-            tile_at(p, t, m, n);
+        for (int i = mine; i < total; i += step) {
+            const Tile t = tile_of(p, i);
             if (!__all_sync(0xFFFFFFFFu, bar_wait(&s.acc_full[buf], buf_phase, err, WAIT_NS))) break;
             tc_fence_after();
-            epilogue<PAIR, MODE>(p, tmem + buf * BN + (unsigned(quarter * 32) << 16), m * BN + int(rank) * CTA_ROWS + quarter * 32 + lane, n);
+            epilogue<BN, MODE>(p, t, tmem + buf * BN + (unsigned(quarter * 32) << 16), (t.m * PAIR + int(rank)) * CTA_ROWS + quarter * 32 + lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {

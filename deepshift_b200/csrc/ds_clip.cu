@@ -25,7 +25,7 @@ struct ClipTable {
     void* dst[CAP];
     long long n[CAP];
     int first[CAP + 1];      // first chunk of each tensor
-    unsigned char kind[CAP]; // type of src, type of dst << 2, src 16-byte aligned << 4, both << 5
+    unsigned char kind[CAP]; // type of src, type of dst << 2, both 16-byte aligned << 4
     int count;
     int steps;               // a chunk: this many steps of U pieces a thread
 };
@@ -39,34 +39,58 @@ __device__ __forceinline__ float2 unpack(unsigned v, int kind)
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-// The elements of a thread's piece: `per` consecutive ones from `at`, or, in tensors that are not 16-byte aligned, every CLIP_THREADS-th, so
-// that a warp's accesses lie side by side all the same (one by one and 16 bytes apart they took four times as long).
-__device__ __forceinline__ long long element(bool vec, long long at, int i) { return at + (vec ? i : i * CLIP_THREADS); }
-
-// Where a thread's piece u of a step that begins at element `start` begins.
-__device__ __forceinline__ long long piece_at(bool vec, long long start, int u, int per)
+// Elements before the first 16-byte boundary of a tensor.
+__device__ __forceinline__ int head_of(const void* p, int per)
 {
-    return start + (long long)u * CLIP_THREADS * per + (vec ? threadIdx.x * per : threadIdx.x);
+    return (int(16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (16 / per);
 }
 
-// The piece at element `at` of a tensor of n, zeros behind its end.
-__device__ __forceinline__ uint4 load_piece(const void* p, int kind, bool vec, long long at, long long n)
+__device__ __forceinline__ float element(const void* p, int kind, long long i)
+{
+    return kind == DS_T_F32 ? static_cast<const float*>(p)[i] : unpack(static_cast<const unsigned short*>(p)[i], kind).x;
+}
+
+// The piece at element `at`, a 16-byte boundary, of a tensor of n; zeros behind its end.
+__device__ __forceinline__ uint4 load_piece(const void* p, int kind, long long at, long long n)
 {
     const int per = per_piece(kind);
-    if (vec && at + per <= n) return *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at * (16 / per));
+    if (at + per <= n) return *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at * (16 / per));
     unsigned w[4] = {0, 0, 0, 0};
     if (at < n) {
         if (kind == DS_T_F32) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (element(vec, at, i) < n) w[i] = static_cast<const unsigned*>(p)[element(vec, at, i)];
+                if (at + i < n) w[i] = static_cast<const unsigned*>(p)[at + i];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (element(vec, at, i) < n) w[i >> 1] |= unsigned(static_cast<const unsigned short*>(p)[element(vec, at, i)]) << (16 * (i & 1));
+                if (at + i < n) w[i >> 1] |= unsigned(static_cast<const unsigned short*>(p)[at + i]) << (16 * (i & 1));
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The piece at any element: the bytes between two boundaries come from the two aligned pieces that hold them (the second of which
+// is the neighbour's first, and in L1).  Only for at + per <= n.
+__device__ __forceinline__ uint4 load_shifted(const void* p, int kind, long long at)
+{
+    const char* q = static_cast<const char*>(p) + at * (16 / per_piece(kind));
+    const unsigned off = unsigned(reinterpret_cast<uintptr_t>(q) & 15);
+    const uint4* from = reinterpret_cast<const uint4*>(q - off);
+    const uint4 a = from[0];
+    if (off == 0) return a;
+    const uint4 b = from[1];
+    const unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    unsigned v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // words off / 4 + i and the next, by selection: an index would put w into local memory
+        unsigned lo = w[i], hi = w[i + 1];
+#pragma unroll
+        for (int s = 1; s < 4; ++s)
+            if (off >> 2 == s) lo = w[i + s], hi = w[i + s + 1 < 8 ? i + s + 1 : 7];
+        v[i] = __funnelshift_r(lo, hi, (off & 3) * 8);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // Values of a piece; fp32 has four, and zeros.
@@ -90,29 +114,25 @@ __device__ __forceinline__ unsigned short narrow(float f, int kind)
 
 __device__ __forceinline__ unsigned narrow2(float a, float b, int kind) { return narrow(a, kind) | unsigned(narrow(b, kind)) << 16; }
 
-// The `per` (4 or 8) values of a piece to element `at`.  Nothing reads them soon: the stores give way to what the sums left in L2.
-__device__ __forceinline__ void store_piece(void* p, int kind, bool vec, long long at, long long n, int per, const float (&v)[8])
+__device__ __forceinline__ void store_element(void* p, int kind, long long i, float v)
 {
-    if (vec && at + per <= n) {
-        if (kind == DS_T_F32) {
-            float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-            __stcs(q, make_float4(v[0], v[1], v[2], v[3]));
-            if (per == 8) __stcs(q + 1, make_float4(v[4], v[5], v[6], v[7]));
-        } else {
-            char* q = static_cast<char*>(p) + at * 2;
-            const uint2 a = make_uint2(narrow2(v[0], v[1], kind), narrow2(v[2], v[3], kind));
-            if (per == 8) __stcs(reinterpret_cast<uint4*>(q), make_uint4(a.x, a.y, narrow2(v[4], v[5], kind), narrow2(v[6], v[7], kind)));
-            else __stcs(reinterpret_cast<uint2*>(q), a);
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long to = element(vec, at, i);
-        if (i < per && to < n) {
-            if (kind == DS_T_F32) static_cast<float*>(p)[to] = v[i];
-            else static_cast<unsigned short*>(p)[to] = narrow(v[i], kind);
-        }
+    if (kind == DS_T_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<unsigned short*>(p)[i] = narrow(v, kind);
+}
+
+// The `per` (4 or 8) values of a piece to element `at`, a 16-byte boundary.  Nothing reads them soon: the stores give way to what the sums
+// left in L2.
+__device__ __forceinline__ void store_piece(void* p, int kind, long long at, int per, const float (&v)[8])
+{
+    if (kind == DS_T_F32) {
+        float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+        __stcs(q, make_float4(v[0], v[1], v[2], v[3]));
+        if (per == 8) __stcs(q + 1, make_float4(v[4], v[5], v[6], v[7]));
+    } else {
+        char* q = static_cast<char*>(p) + at * 2;
+        const uint2 a = make_uint2(narrow2(v[0], v[1], kind), narrow2(v[2], v[3], kind));
+        if (per == 8) __stcs(reinterpret_cast<uint4*>(q), make_uint4(a.x, a.y, narrow2(v[4], v[5], kind), narrow2(v[6], v[7], kind)));
+        else __stcs(reinterpret_cast<uint2*>(q), a);
     }
 }
 
@@ -153,14 +173,18 @@ __global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constan
     for (int chunk = blockIdx.x; chunk < t.first[t.count]; chunk += gridDim.x) {
         const int i = tensor_of(t, chunk);
         const int kind = t.kind[i] & 3, per = per_piece(kind);
-        const bool vec = t.kind[i] & 16;
         const void* p = t.src[i];
         const long long n = t.n[i];
-        long long at = (long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS * per;
+        const int head = head_of(p, per);
+        if (chunk == t.first[i] && int(threadIdx.x) < head && threadIdx.x < n) {
+            const double v = element(p, kind, threadIdx.x);
+            acc += v * v;
+        }
+        long long at = head + ((long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS + threadIdx.x) * per;
         for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
             uint4 q[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = load_piece(p, kind, vec, piece_at(vec, at, u, per), n);
+            for (int u = 0; u < U; ++u) q[u] = load_piece(p, kind, at + u * CLIP_THREADS * per, n);
             float s[U / 2];
             bool fits = true;
 #pragma unroll
@@ -182,7 +206,7 @@ __global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constan
                 const unsigned size = kind == DS_T_F32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
 #pragma unroll 1
                 for (int u = 0; u < U; ++u) {
-                    const uint4 w = load_piece(p, kind, vec, piece_at(vec, at, u, per), n);
+                    const uint4 w = load_piece(p, kind, at + u * CLIP_THREADS * per, n);
                     if (((w.x | w.y | w.z | w.w) & size) == 0) continue;
                     float v[8];
                     widen(w, kind, v);
@@ -216,20 +240,36 @@ __global__ void __launch_bounds__(CLIP_THREADS) scale_kernel(const __grid_consta
         const int i = tensor_of(t, chunk);
         if (f == 1.f && t.src[i] == t.dst[i]) continue;
         const int kind = t.kind[i] & 3, per = per_piece(kind), to = t.kind[i] >> 2 & 3;
-        const bool vec = t.kind[i] & 32;
-        const long long n = t.n[i];
-        long long at = (long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS * per;
+        const void* src = t.src[i];
+        void* dst = t.dst[i];
+        const long long n = t.n[i], begin = (long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS * per;
+        if (kind != to && !(t.kind[i] & 16)) {   // another type, and no common alignment: one by one
+            const long long end = min(n, begin + (long long)t.steps * U * CLIP_THREADS * per);
+#pragma unroll 8
+            for (long long at = begin + threadIdx.x; at < end; at += CLIP_THREADS) store_element(dst, to, at, element(src, kind, at) * f);
+            continue;
+        }
+        // pieces between the boundaries of the place, the head before the first one by one
+        const int head = head_of(dst, per);
+        if (chunk == t.first[i] && int(threadIdx.x) < head && threadIdx.x < n) store_element(dst, to, threadIdx.x, element(src, kind, threadIdx.x) * f);
+        long long at = head + begin + threadIdx.x * per;
         for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
             uint4 q[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = load_piece(t.src[i], kind, vec, piece_at(vec, at, u, per), n);
+            for (int u = 0; u < U; ++u)
+                if (at + u * CLIP_THREADS * per + per <= n) q[u] = load_shifted(src, kind, at + u * CLIP_THREADS * per);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float v[8];
-                widen(q[u], kind, v);
+                const long long here = at + u * CLIP_THREADS * per;
+                if (here + per <= n) {
+                    float v[8];
+                    widen(q[u], kind, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] *= f;
-                store_piece(t.dst[i], to, vec, piece_at(vec, at, u, per), n, per, v);
+                    for (int e = 0; e < 8; ++e) v[e] *= f;
+                    store_piece(dst, to, here, per, v);
+                } else {
+                    for (long long e = here; e < n; ++e) store_element(dst, to, e, element(src, kind, e) * f);
+                }
             }
         }
     }
@@ -260,8 +300,8 @@ int fill(ClipTable<CAP>& t, const ds_tensor_t* tensors, int count, int steps, in
         t.src[k] = a.src;
         t.dst[k] = a.dst;
         t.n[k] = a.n;
-        const uintptr_t src = reinterpret_cast<uintptr_t>(a.src), dst = reinterpret_cast<uintptr_t>(a.dst);
-        t.kind[k] = (unsigned char)(a.src_type | a.dst_type << 2 | (src & 15 ? 0 : 16) | ((src | dst) & 15 ? 0 : 32));
+        const bool both = ((reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst)) & 15) == 0;
+        t.kind[k] = (unsigned char)(a.src_type | a.dst_type << 2 | (both ? 16 : 0));
         t.first[k + 1] = t.first[k] + int(chunks_of(a, bytes));
     }
     return t.first[t.count];
@@ -331,6 +371,7 @@ extern "C" int ds_clip_norm(const ds_tensor_t* tensors, int count, float max_nor
         if (a.src_type < 0 || a.src_type > DS_T_F16 || a.dst_type < 0 || a.dst_type > DS_T_F16) return DS_ERR_UNSUPPORTED;
         if (a.n > 1ll << 42) return DS_ERR_RANGE;
         if (a.n) ++(a.dst ? with : without);
+        if (reinterpret_cast<uintptr_t>(a.src) % ds::type_bytes(a.src_type) || reinterpret_cast<uintptr_t>(a.dst) % ds::type_bytes(a.dst_type)) return DS_ERR_ALIGN;
         bytes += a.n * ds::type_bytes(a.src_type);
         chunks += ds::chunks_of(a, 4 * ds::CLIP_STEP);
     }

@@ -47,33 +47,38 @@ def _call(name, hidden, weight, target, ignore_index, reduction, each=0, lse=0, 
 
 
 def _forward(hidden, weight, target, ignore_index, reduction):
-    """Losses and log-sum-exps of the rows [2, rows], and their sum or mean and the number that it is over."""
+    """The loss, or each row's, and what the backward pass needs: log-sum-exps of the rows, and behind them the number that the mean
+    is over."""
     rows = hidden.shape[0]
-    out = hidden.new_empty(2 * rows + 2, dtype=torch.float32)
-    at = out.data_ptr()
-    _call("ds_loss_forward", hidden, weight, target, ignore_index, reduction, at, at + 4 * rows, at + 8 * rows, at + 8 * rows + 4)
-    return out
+    kept = hidden.new_empty(rows + 1 if not reduction else 2 * rows + 1, dtype=torch.float32)
+    loss = hidden.new_empty(() if reduction else (rows,), dtype=torch.float32)
+    lse, to = kept.data_ptr(), loss.data_ptr()
+    if reduction:
+        _call("ds_loss_forward", hidden, weight, target, ignore_index, reduction, lse + 4 * (rows + 1), lse, to, lse + 4 * rows)
+    else:
+        _call("ds_loss_forward", hidden, weight, target, ignore_index, reduction, to, lse)
+    return loss, kept
 
 
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        out = _forward(hidden, weight, target, ignore_index, reduction)
-        rows = hidden.shape[0]
-        ctx.save_for_backward(hidden, weight, target, out)
+        loss, kept = _forward(hidden, weight, target, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, target, kept)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        return out[2 * rows].clone() if reduction else out[:rows].clone()
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, target, out = ctx.saved_tensors
+        hidden, weight, target, kept = ctx.saved_tensors
         grad = grad.contiguous()
-        rows, at = hidden.shape[0], out.data_ptr()
-        dhidden = torch.empty_like(hidden) if ctx.needs_input_grad[0] else None
-        dweight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        _call("ds_loss_backward", hidden, weight, target, ctx.ignore_index, ctx.reduction, lse=at + 4 * rows, count=at + 8 * rows + 4,
-              grad=grad.data_ptr(), dhidden=dhidden.data_ptr() if dhidden is not None else 0, dweight=dweight.data_ptr() if dweight is not None else 0)
+        need_h, need_w = ctx.needs_input_grad[:2]
+        dhidden = torch.empty_like(hidden) if need_h else None
+        dweight = torch.empty_like(weight) if need_w else None
+        lse = kept.data_ptr()
+        _call("ds_loss_backward", hidden, weight, target, ctx.ignore_index, ctx.reduction, lse=lse, count=lse + 4 * hidden.shape[0],
+              grad=grad.data_ptr(), dhidden=dhidden.data_ptr() if need_h else 0, dweight=dweight.data_ptr() if need_w else 0)
         return dhidden, dweight, None, None, None
 
 
@@ -94,6 +99,5 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         loss = _Loss.apply(rows, weight, flat, int(ignore_index), code)
     else:
-        out, n = _forward(rows, weight, flat, int(ignore_index), code), rows.shape[0]
-        loss = out[2 * n] if code else out[:n]
+        loss = _forward(rows, weight, flat, int(ignore_index), code)[0]
     return loss if code or shape == loss.shape else loss.view(shape)

@@ -50,47 +50,28 @@ __device__ __forceinline__ float element(const void* p, int kind, long long i)
     return kind == DS_T_F32 ? static_cast<const float*>(p)[i] : unpack(static_cast<const unsigned short*>(p)[i], kind).x;
 }
 
-// The piece at element `at`, a 16-byte boundary, of a tensor of n; zeros behind its end.
-__device__ __forceinline__ uint4 load_piece(const void* p, int kind, long long at, long long n)
+// A tensor's pieces lie between its 16-byte boundaries; what is before the first of them (`head` elements) and behind the last whole one
+// are single elements, which one chunk's first threads deal with.  Element of this thread among those, or -1.
+__device__ __forceinline__ long long odd_element(int head, int per, long long n)
 {
-    const int per = per_piece(kind);
-    if (at + per <= n) return *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at * (16 / per));
-    unsigned w[4] = {0, 0, 0, 0};
-    if (at < n) {
-        if (kind == DS_T_F32) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (at + i < n) w[i] = static_cast<const unsigned*>(p)[at + i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (at + i < n) w[i >> 1] |= unsigned(static_cast<const unsigned short*>(p)[at + i]) << (16 * (i & 1));
-        }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    const long long before = head < n ? head : n, behind = before + (n - before) / per * per;   // [0, before) and [behind, n)
+    const long long i = threadIdx.x < before ? threadIdx.x : behind + threadIdx.x - before;
+    return i < n ? i : -1;
 }
 
-// The piece at any element: the bytes between two boundaries come from the two aligned pieces that hold them (the second of which
-// is the neighbour's first, and in L1).  Only for at + per <= n.
-__device__ __forceinline__ uint4 load_shifted(const void* p, int kind, long long at)
+// Sixteen bytes from byte `off` of two neighbouring pieces.
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, unsigned off)
 {
-    const char* q = static_cast<const char*>(p) + at * (16 / per_piece(kind));
-    const unsigned off = unsigned(reinterpret_cast<uintptr_t>(q) & 15);
-    const uint4* from = reinterpret_cast<const uint4*>(q - off);
-    const uint4 a = from[0];
-    if (off == 0) return a;
-    const uint4 b = from[1];
     const unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    unsigned v[4];
+    unsigned x[6], v[5];
+    // by 8 bytes, 4 and what is left: an index would put w into local memory
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {   // words off / 4 + i and the next, by selection: an index would put w into local memory
-        unsigned lo = w[i], hi = w[i + 1];
+    for (int i = 0; i < 6; ++i) x[i] = off & 8 ? w[i + 2] : w[i];
 #pragma unroll
-        for (int s = 1; s < 4; ++s)
-            if (off >> 2 == s) lo = w[i + s], hi = w[i + s + 1 < 8 ? i + s + 1 : 7];
-        v[i] = __funnelshift_r(lo, hi, (off & 3) * 8);
-    }
-    return make_uint4(v[0], v[1], v[2], v[3]);
+    for (int i = 0; i < 5; ++i) v[i] = off & 4 ? x[i + 1] : x[i];
+    const unsigned bits = (off & 3) * 8;
+    return make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits), __funnelshift_r(v[2], v[3], bits),
+                      __funnelshift_r(v[3], v[4], bits));
 }
 
 // Values of a piece; fp32 has four, and zeros.
@@ -167,7 +148,7 @@ __device__ __forceinline__ double cta_sum(double v)
 // Where a sum leaves the range that fp32 can hold (values beyond 1e18, or all so small that their squares vanish) the warp squares in
 // double instead, save for pieces that are 0 altogether.
 template <int CAP, int U>
-__global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* __restrict__ partial)
+__global__ void __launch_bounds__(CLIP_THREADS, 4) norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* __restrict__ partial)
 {
     double acc = 0.0;
     for (int chunk = blockIdx.x; chunk < t.first[t.count]; chunk += gridDim.x) {
@@ -176,15 +157,19 @@ __global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constan
         const void* p = t.src[i];
         const long long n = t.n[i];
         const int head = head_of(p, per);
-        if (chunk == t.first[i] && int(threadIdx.x) < head && threadIdx.x < n) {
-            const double v = element(p, kind, threadIdx.x);
+        if (chunk == t.first[i]) {
+            const long long e = odd_element(head, per, n);
+            const double v = e < 0 ? 0.f : element(p, kind, e);
             acc += v * v;
         }
         long long at = head + ((long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS + threadIdx.x) * per;
         for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
             uint4 q[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = load_piece(p, kind, at + u * CLIP_THREADS * per, n);
+            for (int u = 0; u < U; ++u) {
+                const long long here = at + u * CLIP_THREADS * per;
+                q[u] = here + per <= n ? *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + here * (16 / per)) : make_uint4(0, 0, 0, 0);
+            }
             float s[U / 2];
             bool fits = true;
 #pragma unroll
@@ -206,11 +191,13 @@ __global__ void __launch_bounds__(CLIP_THREADS) norm_kernel(const __grid_constan
                 const unsigned size = kind == DS_T_F32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
 #pragma unroll 1
                 for (int u = 0; u < U; ++u) {
-                    const uint4 w = load_piece(p, kind, at + u * CLIP_THREADS * per, n);
+                    const long long here = at + u * CLIP_THREADS * per;
+                    if (here + per > n) break;
+                    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + here * (16 / per));
                     if (((w.x | w.y | w.z | w.w) & size) == 0) continue;
                     float v[8];
                     widen(w, kind, v);
-#pragma unroll 1
+#pragma unroll
                     for (int e = 0; e < 8; ++e) acc += double(v[e]) * v[e];
                 }
             }
@@ -227,10 +214,14 @@ __device__ __forceinline__ float total_norm(const double* __restrict__ partial, 
     return float(sqrt(cta_sum(s)));
 }
 
-template <int CAP, int U>
-__global__ void __launch_bounds__(CLIP_THREADS) scale_kernel(const __grid_constant__ ClipTable<CAP> t, const double* __restrict__ partial,
-                                                             int partials, float max_norm, float* __restrict__ norm)
+// A chunk is `steps` steps of U pieces a thread.  ALIGNED: every place and source is 16-byte aligned, and eight pieces are on their way; four elsewhere,
+// where each takes two loads and what puts them together (one kernel for both, with eight, spilled: 700 instead of 755 us for 1 G aligned
+// bf16 values, but 71 instead of 47 for 40 M of two types at any alignment).
+template <int CAP, bool ALIGNED>
+__global__ void __launch_bounds__(CLIP_THREADS, 3) scale_kernel(const __grid_constant__ ClipTable<CAP> t, int steps, const double* __restrict__ partial,
+                                                                int partials, float max_norm, float* __restrict__ norm)
 {
+    constexpr int U = ALIGNED ? 8 : 4;
     const float all = total_norm(partial, partials);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = all;
     float f = max_norm / (all + 1e-6f);
@@ -242,34 +233,48 @@ __global__ void __launch_bounds__(CLIP_THREADS) scale_kernel(const __grid_consta
         const int kind = t.kind[i] & 3, per = per_piece(kind), to = t.kind[i] >> 2 & 3;
         const void* src = t.src[i];
         void* dst = t.dst[i];
-        const long long n = t.n[i], begin = (long long)(chunk - t.first[i]) * t.steps * U * CLIP_THREADS * per;
-        if (kind != to && !(t.kind[i] & 16)) {   // another type, and no common alignment: one by one
-            const long long end = min(n, begin + (long long)t.steps * U * CLIP_THREADS * per);
+        const long long n = t.n[i], begin = (long long)(chunk - t.first[i]) * steps * U * CLIP_THREADS * per;
+        if (!ALIGNED && kind != to && !(t.kind[i] & 16)) {   // another type, and no common alignment: one by one
+            const long long end = min(n, begin + (long long)steps * U * CLIP_THREADS * per);
 #pragma unroll 8
             for (long long at = begin + threadIdx.x; at < end; at += CLIP_THREADS) store_element(dst, to, at, element(src, kind, at) * f);
             continue;
         }
-        // pieces between the boundaries of the place, the head before the first one by one
-        const int head = head_of(dst, per);
-        if (chunk == t.first[i] && int(threadIdx.x) < head && threadIdx.x < n) store_element(dst, to, threadIdx.x, element(src, kind, threadIdx.x) * f);
+        // pieces between the boundaries of the place
+        const int head = ALIGNED ? 0 : head_of(dst, per);
+        if (chunk == t.first[i]) {
+            const long long e = odd_element(head, per, n);
+            if (e >= 0) store_element(dst, to, e, element(src, kind, e) * f);
+        }
         long long at = head + begin + threadIdx.x * per;
-        for (int step = 0; step < t.steps; ++step, at += U * CLIP_THREADS * per) {
-            uint4 q[U];
+        // where the source's boundaries lie elsewhere, the bytes of a piece come from the two aligned pieces of the source that hold them, the
+        // second of which is the neighbour's first, and in L1
+        const int size = 16 / per;
+        const unsigned off = ALIGNED ? 0 : unsigned(reinterpret_cast<uintptr_t>(src) + head * size & 15);
+        auto finish = [&](const uint4& q, long long here) {
+            if (here + per > n) return;
+            float v[8];
+            widen(q, kind, v);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (at + u * CLIP_THREADS * per + per <= n) q[u] = load_shifted(src, kind, at + u * CLIP_THREADS * per);
+            for (int e = 0; e < 8; ++e) v[e] *= f;
+            store_piece(dst, to, here, per, v);
+        };
+        for (int step = 0; step < steps; ++step, at += U * CLIP_THREADS * per) {
+            const uint4* from = reinterpret_cast<const uint4*>(static_cast<const char*>(src) + at * size - off);
+            if (off == 0) {
+                uint4 q[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const long long here = at + u * CLIP_THREADS * per;
-                if (here + per <= n) {
-                    float v[8];
-                    widen(q[u], kind, v);
+                for (int u = 0; u < U; ++u)
+                    if (at + (u * CLIP_THREADS + 1) * per <= n) q[u] = from[u * CLIP_THREADS];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] *= f;
-                    store_piece(dst, to, here, per, v);
-                } else {
-                    for (long long e = here; e < n; ++e) store_element(dst, to, e, element(src, kind, e) * f);
-                }
+                for (int u = 0; u < U; ++u) finish(q[u], at + u * CLIP_THREADS * per);
+            } else if (!ALIGNED) {
+                uint4 a[U], b[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (at + (u * CLIP_THREADS + 1) * per <= n) a[u] = from[u * CLIP_THREADS], b[u] = from[u * CLIP_THREADS + 1];
+#pragma unroll
+                for (int u = 0; u < U; ++u) finish(shifted(a[u], b[u], off), at + u * CLIP_THREADS * per);
             }
         }
     }
@@ -310,7 +315,7 @@ int fill(ClipTable<CAP>& t, const ds_tensor_t* tensors, int count, int steps, in
 int ctas(int chunks) { return chunks < CLIP_CTAS ? chunks : CLIP_CTAS; }
 
 template <int CAP, int U>
-int run(const ds_tensor_t* tensors, int count, int steps, float max_norm, float* norm, double* partial, cudaStream_t st, bool scale)
+int run(const ds_tensor_t* tensors, int count, int steps, bool aligned, float max_norm, float* norm, double* partial, cudaStream_t st, bool scale)
 {
     ClipTable<CAP> t;
     int partials = 0, chunks = 0;
@@ -325,7 +330,7 @@ int run(const ds_tensor_t* tensors, int count, int steps, float max_norm, float*
     for (int at = 0; scale && at < count; at += CAP) {
         if (count > CAP) chunks = fill(t, tensors + at, count - at < CAP ? count - at : CAP, steps, steps * U * CLIP_STEP);
         if (!chunks) continue;
-        scale_kernel<CAP, U><<<ctas(chunks), CLIP_THREADS, 0, st>>>(t, partial, partials, max_norm, written ? nullptr : norm);
+        (aligned ? scale_kernel<CAP, true> : scale_kernel<CAP, false>)<<<ctas(chunks), CLIP_THREADS, 0, st>>>(t, steps * U / (aligned ? 8 : 4), partial, partials, max_norm, written ? nullptr : norm);
         note_launch();
         written = true;
     }
@@ -339,10 +344,10 @@ int run(const ds_tensor_t* tensors, int count, int steps, float max_norm, float*
 // Four pieces a thread and small chunks where all gradients together would not give every SM a few of the larger ones; then eight pieces, and
 // chunks of up to four such steps, so that finding a chunk's tensor (a search in the table) stays small.
 template <int CAP>
-int run(const ds_tensor_t* tensors, int count, long long bytes, float max_norm, float* norm, double* partial, cudaStream_t st, bool scale)
+int run(const ds_tensor_t* tensors, int count, long long bytes, bool aligned, float max_norm, float* norm, double* partial, cudaStream_t st, bool scale)
 {
-    if (bytes < 148ll * 4 * 8 * CLIP_STEP) return run<CAP, 4>(tensors, count, 1, max_norm, norm, partial, st, scale);
-    return run<CAP, 8>(tensors, count, bytes < 148ll * 64 * 8 * CLIP_STEP ? 1 : 4, max_norm, norm, partial, st, scale);
+    if (bytes < 148ll * 4 * 8 * CLIP_STEP) return run<CAP, 4>(tensors, count, 1, false, max_norm, norm, partial, st, scale);
+    return run<CAP, 8>(tensors, count, bytes < 148ll * 64 * 8 * CLIP_STEP ? 1 : 4, aligned, max_norm, norm, partial, st, scale);
 }
 
 constexpr int CAP_FEW = 32, CAP_MANY = 512;
@@ -364,6 +369,7 @@ extern "C" int ds_clip_norm(const ds_tensor_t* tensors, int count, float max_nor
     if (scratch_bytes < ds_clip_bytes(count)) return DS_ERR_SCRATCH;
     if (reinterpret_cast<uintptr_t>(scratch) & 7) return DS_ERR_ALIGN;
     int with = 0, without = 0;   // tensors that have somewhere to go, and that have not: all or none
+    bool aligned = true;
     long long bytes = 0, chunks = 0;
     for (int i = 0; i < count; ++i) {
         const ds_tensor_t& a = tensors[i];
@@ -372,6 +378,7 @@ extern "C" int ds_clip_norm(const ds_tensor_t* tensors, int count, float max_nor
         if (a.n > 1ll << 42) return DS_ERR_RANGE;
         if (a.n) ++(a.dst ? with : without);
         if (reinterpret_cast<uintptr_t>(a.src) % ds::type_bytes(a.src_type) || reinterpret_cast<uintptr_t>(a.dst) % ds::type_bytes(a.dst_type)) return DS_ERR_ALIGN;
+        aligned = aligned && ((reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst)) & 15) == 0;
         bytes += a.n * ds::type_bytes(a.src_type);
         chunks += ds::chunks_of(a, 4 * ds::CLIP_STEP);
     }
@@ -380,6 +387,6 @@ extern "C" int ds_clip_norm(const ds_tensor_t* tensors, int count, float max_nor
     const bool scale = with > 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     double* partial = static_cast<double*>(scratch);
-    return count <= ds::CAP_FEW ? ds::run<ds::CAP_FEW>(tensors, count, bytes, max_norm, norm, partial, st, scale)
-                                : ds::run<ds::CAP_MANY>(tensors, count, bytes, max_norm, norm, partial, st, scale);
+    return count <= ds::CAP_FEW ? ds::run<ds::CAP_FEW>(tensors, count, bytes, aligned, max_norm, norm, partial, st, scale)
+                                : ds::run<ds::CAP_MANY>(tensors, count, bytes, aligned, max_norm, norm, partial, st, scale);
 }

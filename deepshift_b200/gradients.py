@@ -15,7 +15,7 @@ from . import _ffi
 from .adapters import TYPES
 
 
-_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+_dtype = attrgetter("dtype")
 
 
 def _flat(t):
@@ -40,8 +40,8 @@ def _run(tensors, to, max_norm):
         raise RuntimeError("all gradients must be on one GPU")
     count = len(tensors)
     kinds = list(map(TYPES.get, map(_dtype, tensors)))
-    if None in kinds or any(map(attrgetter("is_sparse"), tensors)):
-        raise RuntimeError("gradients must be dense, float32, bfloat16 or float16")
+    if None in kinds:
+        raise RuntimeError("gradients must be float32, bfloat16 or float16")
     whole = all(map(torch.Tensor.is_contiguous, tensors))
     if not whole and not all(map(_flat, tensors)):
         raise RuntimeError("a gradient must fill its memory without gaps")
@@ -54,8 +54,8 @@ def _run(tensors, to, max_norm):
             places = list(map(TYPES.get, map(_dtype, to)))
             if set(map(torch.Tensor.get_device, to)) != {device} or None in places:
                 raise RuntimeError("out must be float32, bfloat16 or float16, on the gradients' device")
-            if list(map(_shape, to)) != list(map(_shape, tensors)) or not (
-                    whole and all(map(torch.Tensor.is_contiguous, to)) or [o.stride() for o in to] == [t.stride() for t in tensors]):
+            whole = whole and all(map(torch.Tensor.is_contiguous, to))
+            if list(map(torch.Tensor.numel, to)) != n or not whole and [(o.shape, o.stride()) for o in to] != [(t.shape, t.stride()) for t in tensors]:
                 raise RuntimeError("out must have the shapes and layouts of the gradients")
             at = list(map(torch.Tensor.data_ptr, to))
             kinds = [k | o << 32 for k, o in zip(kinds, places)]
@@ -79,8 +79,8 @@ def clip_norm(tensors, max_norm, out=None):
     """Scales ``tensors`` (float32, bfloat16, float16, mixed, of any shapes, on one GPU) so that their norm together is at most
     ``max_norm``; returns the norm before that as a float32 tensor on the GPU.
 
-    ``out``: where the scaled values go, one tensor for each of ``tensors``, of its shape and layout and of any of the three
-    types; None: in place.  ``max_norm = inf`` leaves the values as they are.  A norm that is NaN makes them NaN, an infinite
+    ``out``: where the scaled values go, one tensor for each of ``tensors``, of its shape and layout (contiguous ones: of its number of
+    elements) and of any of the three types; None: in place.  ``max_norm = inf`` leaves the values as they are.  A norm that is NaN makes them NaN, an infinite
     one 0 (and NaN where they are infinite).  Empty tensors count for nothing."""
     tensors = list(tensors)
     max_norm = float(max_norm)

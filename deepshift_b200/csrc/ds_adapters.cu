@@ -1,5 +1,5 @@
-// Low-rank adapters beside a shared projection: the plan of rows, and the entry points (kernels in ds_adapters.cuh).
-#include "ds_adapters.cuh"
+// Low-rank adapters beside a shared projection: the plan of rows, and the entry points (kernels in ds_adapters.cuh for few rows, ds_adapters_tc.cuh for many).
+#include "ds_adapters_tc.cuh"
 
 #include <type_traits>
 
@@ -164,11 +164,11 @@ bool allow_smem(int bytes)
 }
 
 template <auto KERNEL, class... A>
-int launch_cluster(dim3 grid, dim3 cluster, int smem, cudaStream_t st, const A&... a)
+int launch_cluster(dim3 grid, dim3 cluster, int threads, int smem, cudaStream_t st, const A&... a)
 {
     cudaLaunchConfig_t c = {};
     c.gridDim = grid;
-    c.blockDim = dim3(THREADS);
+    c.blockDim = dim3(threads);
     c.dynamicSmemBytes = smem;
     c.stream = st;
     cudaLaunchAttribute attribute;
@@ -187,62 +187,73 @@ int launch_down(const Args& a, cudaStream_t st)
     static_assert(smem <= 227 * 1024, "shared memory of an SM");
     if (!allow_smem<down_kernel<X, W, MT, NT, VEC>>(smem)) return DS_ERR_CUDA;
     const int blocks = (a.rank8 + 8 * NT - 1) / (8 * NT), chunk = 4 * Down<X, W, MT, NT, DOWN_BUDGET>::LK, shares = splits_of(a, blocks, (a.width + chunk - 1) / chunk);
-    return launch_cluster<down_kernel<X, W, MT, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), smem, st, a);
+    return launch_cluster<down_kernel<X, W, MT, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), THREADS, smem, st, a);
 }
 
-// Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere, where 64 would not fit the
-// registers and the rows are read again from L2 instead.
-template <class X, class W, int MT>
-int down_tile(const Args& a, bool vec, cudaStream_t st)
+// Few rows (tiles of 16).  Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere.
+template <class X, class W>
+int down_few(const Args& a, bool vec, cudaStream_t st)
 {
-    if (!vec) return a.rank8 <= 8 ? launch_down<X, W, MT, 1, false>(a, st) : launch_down<X, W, MT, 4, false>(a, st);
-    if (a.rank8 <= 8) return launch_down<X, W, MT, 1, true>(a, st);
-    if (a.rank8 <= 16) return launch_down<X, W, MT, 2, true>(a, st);
-    if constexpr (Down<X, W, MT, 8, DOWN_BUDGET>::SAME)
-        if (a.rank8 > 32) return launch_down<X, W, MT, 8, true>(a, st);
-    return launch_down<X, W, MT, 4, true>(a, st);
+    if (!vec) return a.rank8 <= 8 ? launch_down<X, W, 1, 1, false>(a, st) : launch_down<X, W, 1, 4, false>(a, st);
+    if (a.rank8 <= 8) return launch_down<X, W, 1, 1, true>(a, st);
+    if (a.rank8 <= 16) return launch_down<X, W, 1, 2, true>(a, st);
+    if constexpr (Down<X, W, 1, 8, DOWN_BUDGET>::SAME)
+        if (a.rank8 > 32) return launch_down<X, W, 1, 8, true>(a, st);
+    return launch_down<X, W, 1, 4, true>(a, st);
+}
+
+template <class X, class W, bool VEC>
+int launch_tc_down(const Args& a, cudaStream_t st)
+{
+    using S = TcDown<X, W>;
+    static_assert(S::STAGES >= 2 && TC_ROWS * S::RED * 4 <= S::STAGES * S::STAGE, "stages of a CTA");
+    if (!allow_smem<tc_down_kernel<X, W, VEC>>(S::SMEM)) return DS_ERR_CUDA;
+    const int blocks = (a.rank8 + TC_RANKS - 1) / TC_RANKS, chunks = (a.width + 63) / 64;
+    // CTAs a tile's sums are shared by: until each SM has one, as long as each has four steps
+    const long long tiles = plan_tiles(a.rows, a.count) * blocks;
+    int shares = 1;
+    while (shares < 8 && tiles * shares * 2 <= 148 && chunks >= 2 * shares * 4) shares *= 2;
+    return launch_cluster<tc_down_kernel<X, W, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), TC_THREADS, S::SMEM, st, a);
 }
 
 template <class X, class W>
 int down(const Args& a, bool vec, cudaStream_t st)
 {
-    return plan_tile_rows(a.rows) == 32 ? down_tile<X, W, 2>(a, vec, st) : down_tile<X, W, 1>(a, vec, st);
+    if (plan_tile_rows(a.rows) == 16) return down_few<X, W>(a, vec, st);
+    return vec ? launch_tc_down<X, W, true>(a, st) : launch_tc_down<X, W, false>(a, st);
 }
 
-template <class X, class W, int MT, bool VEC>
+template <class X, class W, bool VEC>
 int launch_up(const Args& a, cudaStream_t st)
 {
-    // h of the tile in two parts, and the base's columns
-    constexpr int rows = VEC ? MT * base_bytes<X> : WARPS * 16 * 65 * 4;
-    const int smem = a.rank8 * 16 * MT * 8 + rows;
-    if (!allow_smem<up_kernel<X, W, MT, VEC>>(MAX_RANK * 16 * MT * 8 + rows)) return DS_ERR_CUDA;
-    const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS), VEC ? 1 : MT);
-    up_kernel<X, W, MT, VEC><<<grid, THREADS, smem, st>>>(a);
+    // h of sixteen rows in two parts, and the base's columns
+    constexpr int rows = VEC ? base_bytes<X> : WARPS * 16 * 65 * 4;
+    const int smem = a.rank8 * 16 * 8 + rows;
+    if (!allow_smem<up_kernel<X, W, VEC>>(MAX_RANK * 16 * 8 + rows)) return DS_ERR_CUDA;
+    const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS), plan_tile_rows(a.rows) / 16);
+    up_kernel<X, W, VEC><<<grid, THREADS, smem, st>>>(a);
     return finish();
 }
 
-template <class X, class W>
-int launch_up_stream(const Args& a, cudaStream_t st)
+template <class X, class W, bool VEC>
+int launch_tc_up(const Args& a, cudaStream_t st)
 {
-    using S = Stream<X, W>;
-    static_assert(S::smem(S::MOST_RANK) <= 227 * 1024, "shared memory of an SM");
-    if (!allow_smem<up_stream_kernel<X, W>>(S::smem(S::MOST_RANK))) return DS_ERR_CUDA;
-    const int columns = (a.width + S::COLS - 1) / S::COLS, per_sm = S::smem(a.rank8) <= 113 * 1024 ? 2 : 1;
+    using S = TcUp<X, W>;
+    static_assert(S::smem(TC_RANKS) <= 227 * 1024, "shared memory of an SM");
+    if (!allow_smem<tc_up_kernel<X, W, VEC>>(S::smem(TC_RANKS))) return DS_ERR_CUDA;
+    const int columns = (a.width + S::COLS - 1) / S::COLS;
     const long long tiles = plan_tiles(a.rows, a.count);
-    long long runs = 148 * per_sm / columns;   // one wave
+    long long runs = 148 / columns;   // one round
     runs = runs < 1 ? 1 : runs > tiles ? tiles : runs;
-    up_stream_kernel<X, W><<<dim3(unsigned(runs), columns), THREADS, S::smem(a.rank8), st>>>(a);
+    tc_up_kernel<X, W, VEC><<<dim3(unsigned(runs), columns), TC_THREADS, S::smem((a.rank8 + 15) / 16 * 16), st>>>(a);
     return finish();
 }
 
 template <class X, class W>
 int up(const Args& a, bool vec, cudaStream_t st)
 {
-    const bool wide = plan_tile_rows(a.rows) == 32;
-    if (!vec) return wide ? launch_up<X, W, 2, false>(a, st) : launch_up<X, W, 1, false>(a, st);
-    if (!wide) return launch_up<X, W, 1, true>(a, st);
-    if (a.rank8 <= Stream<X, W>::MOST_RANK) return launch_up_stream<X, W>(a, st);
-    return launch_up<X, W, 2, true>(a, st);
+    if (plan_tile_rows(a.rows) == 16 || a.rank8 > TC_RANKS) return vec ? launch_up<X, W, true>(a, st) : launch_up<X, W, false>(a, st);
+    return vec ? launch_tc_up<X, W, true>(a, st) : launch_tc_up<X, W, false>(a, st);
 }
 
 template <class X, class W, int RT, int CW, bool VEC>
@@ -257,7 +268,7 @@ int launch_grad(const Args& a, cudaStream_t st)
     // rows spread evenly
     int shares = 1;
     while (shares < 8 && (long long)columns * a.count * blocks * shares < 296 && a.rows / a.count >= 2 * shares * 2 * block) shares *= 2;
-    return launch_cluster<grad_kernel<X, W, RT, CW, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), smem, st, a);
+    return launch_cluster<grad_kernel<X, W, RT, CW, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), THREADS, smem, st, a);
 }
 
 template <class X, class W, int RT, bool VEC>
@@ -268,9 +279,23 @@ int grad_columns(const Args& a, cudaStream_t st)
     return launch_grad<X, W, RT, 8, VEC>(a, st);
 }
 
+template <class X, class W, bool VEC>
+int launch_tc_grad(const Args& a, cudaStream_t st)
+{
+    using S = TcGrad<X>;
+    static_assert(S::STAGES >= 2 && TC_RANKS * S::RED * 4 <= S::STAGES * S::STAGE, "stages of a CTA");
+    if (!allow_smem<tc_grad_kernel<X, W, VEC>>(S::SMEM)) return DS_ERR_CUDA;
+    const int columns = (a.width + 127) / 128, blocks = (a.rank8 + TC_RANKS - 1) / TC_RANKS;
+    // CTAs that share an adapter's rows: until each SM has one, as long as each has four steps, were the rows spread evenly
+    int shares = 1;
+    while (shares < 8 && (long long)columns * a.count * blocks * shares * 2 <= 148 && a.rows / a.count >= 2 * shares * 4 * 64) shares *= 2;
+    return launch_cluster<tc_grad_kernel<X, W, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), TC_THREADS, S::SMEM, st, a);
+}
+
 template <class X, class W>
 int grad(const Args& a, bool vec, cudaStream_t st)
 {
+    if (plan_tile_rows(a.rows) != 16) return vec ? launch_tc_grad<X, W, true>(a, st) : launch_tc_grad<X, W, false>(a, st);
     if (!vec) return launch_grad<X, W, 2, 4, false>(a, st);
     return a.rank <= 16 ? grad_columns<X, W, 1, true>(a, st) : grad_columns<X, W, 2, true>(a, st);
 }
@@ -286,7 +311,7 @@ int launch_both(const Args& d, const Args& u, cudaStream_t st)
     const long long tiles = plan_tiles(d.rows, d.count);
     int shares = 1;
     while (shares < 8 && tiles * shares * 2 <= 296 && shares < (steps > columns ? steps : columns)) shares *= 2;
-    return launch_cluster<both_kernel<X, W, NT, VEC>>(dim3(unsigned(tiles), shares), dim3(1, shares, 1), smem, st, d, u);
+    return launch_cluster<both_kernel<X, W, NT, VEC>>(dim3(unsigned(tiles), shares), dim3(1, shares, 1), THREADS, smem, st, d, u);
 }
 
 // h = x down^T and out = base + s h up.  One launch for up to 512 rows, whose tiles are of 16 rows, and up to 64 ranks; two otherwise.
@@ -333,6 +358,7 @@ int check(const ds_adapters_t* a, bool backward)
     if (!a->plan || !a->down || !a->up) return DS_ERR_BAD_ARG;
     if (a->rows && (!a->x || !a->h)) return DS_ERR_BAD_ARG;
     if (backward ? (a->rows && (!a->grad || !a->dh)) : (a->rows && !a->out)) return DS_ERR_BAD_ARG;
+    if (!kernel_error_flag()) return DS_ERR_CUDA;
     if (reinterpret_cast<uintptr_t>(a->plan) & 15 || reinterpret_cast<uintptr_t>(a->h) & 15 || reinterpret_cast<uintptr_t>(a->dh) & 15)
         return DS_ERR_ALIGN;
     const long long need = ds_adapters_h_bytes(a->rows, a->rank);
@@ -343,6 +369,7 @@ int check(const ds_adapters_t* a, bool backward)
 Args common(const ds_adapters_t* a)
 {
     Args p = {};
+    p.err_flag = kernel_error_flag();
     p.plan = plan_view(a->plan, a->rows, a->count);
     p.scale = a->scale;
     p.rows = a->rows, p.rank = a->rank, p.rank8 = rank8(a->rank), p.count = a->count;

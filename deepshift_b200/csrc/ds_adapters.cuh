@@ -35,7 +35,7 @@ struct PlanView {
     const int* order;
 };
 constexpr int PLAN_HEAD = 4;
-__host__ __device__ inline int plan_tile_rows(int rows) { return rows <= 512 ? 16 : 32; }
+__host__ __device__ inline int plan_tile_rows(int rows) { return rows <= 512 ? 16 : 128; }
 __host__ __device__ inline long long plan_tiles(int rows, int count)
 {
     const long long groups = rows < count + 1 ? rows : count + 1;
@@ -60,6 +60,7 @@ struct Args {
     void* out;            // [rows][ldout], or a gradient [count][rank][width]
     long long ldout;
     int rows, width, rank, rank8, count;
+    int* err_flag;        // of the kernels whose waits have limits
 };
 
 using bf16 = __nv_bfloat16;
@@ -219,13 +220,6 @@ __device__ __forceinline__ uint4 slot(unsigned at)
 {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ uint2 slot8(unsigned at)
-{
-    uint2 v;
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
     return v;
 }
 
@@ -502,12 +496,12 @@ __device__ __forceinline__ void put_parts(unsigned* at, float v)
     at[128] = lo;
 }
 
-// Values r .. r + 3 (r a multiple of 4) of row `at` of a tile into the order in which the instruction reads its first operand [row][rank]:
-// blocks [rank / 8][halves of 16 rows][hi, lo][lane][4], the lane that holds row at % 8 and rank pair r % 8 / 2, its
+// Values r .. r + 3 (r a multiple of 4) of row `at` of sixteen into the order in which the instruction reads its first operand [row][rank]:
+// blocks [rank / 8][hi, lo][lane][4], the lane that holds row at % 8 and rank pair r % 8 / 2, its
 // elements by rows of 8 and then by the pair's second.
-__device__ __forceinline__ void put_h4(unsigned* h, int halves, int at, int r, const float4& v, float scale)
+__device__ __forceinline__ void put_h4(unsigned* h, int at, int r, const float4& v, float scale)
 {
-    unsigned* to = h + (r / 8 * halves + at / 16) * 256 + (at % 8 * 4 + r % 8 / 2) * 4 + (at / 8 & 1);
+    unsigned* to = h + r / 8 * 256 + (at % 8 * 4 + r % 8 / 2) * 4 + (at / 8 & 1);
     put_parts(to, v.x * scale);
     put_parts(to + 2, v.y * scale);
     put_parts(to + 4, v.z * scale);
@@ -699,10 +693,10 @@ __device__ __forceinline__ void flush(float (&total)[8][4], float (&acc)[8][4])
         for (int e = 0; e < 4; ++e) total[j][e] += acc[j][e], acc[j][e] = 0.f;
 }
 
-// All ranks of one warp's 64 columns; `h` = the tile's h in shared memory, `halves` of 16 rows in a block, this being number `half`.  The next
-// ranks' columns are on their way during the products of the present ones.
+// All ranks of one warp's 64 columns; `h` = the rows' h in shared memory.  The next ranks' columns are on their way during the products of
+// the present ones.
 template <class X, class W, bool VEC>
-__device__ __forceinline__ void up_products(const Args& p, int adapter, int n0, unsigned h, int halves, int half, float (&acc)[8][4])
+__device__ __forceinline__ void up_products(const Args& p, int adapter, int n0, unsigned h, float (&acc)[8][4])
 {
     const int lane = threadIdx.x & 31, t = lane & 3;
     const W* w = static_cast<const W*>(p.w) + (long long)adapter * p.rank * p.width + n0;
@@ -717,54 +711,44 @@ __device__ __forceinline__ void up_products(const Args& p, int adapter, int n0, 
             load_w<X, W, VEC>(p, w, r + 8 + 2 * t, n0, next[0]);
             load_w<X, W, VEC>(p, w, r + 9 + 2 * t, n0, next[1]);
         }
-        up_step<X, W>(part, h + (r / 8 * halves + half) * 1024 + lane * 16, b);
+        up_step<X, W>(part, h + r / 8 * 1024 + lane * 16, b);
         if (r % 32 == 24) flush(acc, part);
     }
     flush(acc, part);
 }
 
-// One tile of the plan (MT halves of 16 rows) and 512 columns a CTA.  The tile's h, scaled and split, lies in shared memory for all
+// Sixteen rows of a tile of the plan (blockIdx.z) and 512 columns a CTA.  The rows' h, scaled and split, lies in shared memory for all
 // warps in the order in which the instructions read it; base is on its way meanwhile.
-template <class X, class W, int MT, bool VEC>
+template <class X, class W, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 {
     extern __shared__ __align__(16) unsigned char smem[];
     if (int(blockIdx.x) >= p.plan.head[0]) return;
     const int4 tile = p.plan.tiles[blockIdx.x];
     const bool none = tile.x >= p.count;
-    if (none && p.base == p.out) return;   // in place: these rows are there already
+    const int first = 16 * blockIdx.z;
+    if (first >= tile.z || (none && p.base == p.out)) return;   // in place: rows without an adapter are there already
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
     const int n0 = (blockIdx.y * WARPS + warp) * 64;
-    int row[MT][2];
-    const unsigned h = shared_address(smem), slots = h + p.rank8 * 16 * MT * 8;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        row[i][0] = tile_row(p.plan, tile, 16 * i + g), row[i][1] = tile_row(p.plan, tile, 16 * i + 8 + g);
-        if (VEC && p.base) issue_base<X>(p, row[i], n0, slots + i * base_bytes<X>);
-    }
+    const int row[2] = {tile_row(p.plan, tile, first + g), tile_row(p.plan, tile, first + 8 + g)};
+    const unsigned h = shared_address(smem), slots = h + p.rank8 * 16 * 8;
+    if (VEC && p.base) issue_base<X>(p, row, n0, slots);
     if (VEC) copies_end();
     if (!none) {
         const float scale = p.scale ? p.scale[tile.x] : 1.f;
-        constexpr int PER = THREADS / (16 * MT);   // threads a row
-        const int at = threadIdx.x / PER, m = tile_row(p.plan, tile, at);
-        for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(reinterpret_cast<unsigned*>(smem), MT, at, r, load_h4(p, m, r), scale);
+        constexpr int PER = THREADS / 16;   // threads a row
+        const int at = threadIdx.x / PER, m = tile_row(p.plan, tile, first + at);
+        for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(reinterpret_cast<unsigned*>(smem), at, r, load_h4(p, m, r), scale);
     }
     __syncthreads();
     if (n0 >= p.width) return;
-    float* stage = reinterpret_cast<float*>(smem + p.rank8 * 16 * MT * 8) + warp * 16 * 65;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        if (gridDim.z > 1 && i != int(blockIdx.z)) continue;   // a CTA for each half: there are few tiles, and much to wait for
-        float acc[8][4] = {};
-        if (!none) up_products<X, W, VEC>(p, tile.x, n0, h, MT, i, acc);
-        if constexpr (VEC) {
-            if (i == 0) {
-                copies_wait<0>();
-                __syncwarp();
-            }
-            finish_rows<X>(p, row[i], n0, slots + i * base_bytes<X>, acc);
-        } else finish_unaligned<X>(p, tile, 16 * i, n0, stage, acc);
-    }
+    float acc[8][4] = {};
+    if (!none) up_products<X, W, VEC>(p, tile.x, n0, h, acc);
+    if constexpr (VEC) {
+        copies_wait<0>();
+        __syncwarp();
+        finish_rows<X>(p, row, n0, slots, acc);
+    } else finish_unaligned<X>(p, tile, first, n0, reinterpret_cast<float*>(smem + p.rank8 * 16 * 8) + warp * 16 * 65, acc);
 }
 
 // Few rows: both projections of a tile of 16 in one launch (`d`: the down projection's operands, `u`: the up projection's).  The CTAs of
@@ -815,7 +799,7 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
             for (int e = 0; e < 4; ++e)
                 if (r + e >= d.rank) s[e] = 0.f;
             const float4 v = make_float4(s[0], s[1], s[2], s[3]);
-            put_h4(parts_h, 1, at, r, v, scale);
+            put_h4(parts_h, at, r, v, scale);
             const int m = tile_row(d.plan, tile, at);
             if (d.h && share == 0 && m >= 0) *reinterpret_cast<float4*>(d.h + (long long)m * d.rank8 + r) = v;
         }
@@ -829,7 +813,7 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
         }
         if (VEC) copies_end();
         float acc[8][4] = {};
-        if (!none) up_products<X, W, VEC>(u, tile.x, n0, h, 1, 0, acc);
+        if (!none) up_products<X, W, VEC>(u, tile.x, n0, h, acc);
         if constexpr (VEC) {
             copies_wait<0>();
             __syncwarp();
@@ -839,139 +823,6 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
 }
 template <class X, class W, int NT>
 constexpr int both_smem(bool vec) { return Down<X, W, 1, NT, BOTH_BUDGET>::smem(vec) + 8 * NT * 16 * 8 + (vec ? base_bytes<X> : WARPS * 16 * 65 * 4); }
-
-// Many rows: up_kernel's product for 256 columns and a run of consecutive tiles of 32 rows.  The adapter's part of `w` stays in shared memory
-// until a tile of another adapter comes (up_kernel reads it from L2 for every tile, and waits for it), and the next tile's
-// base and h are on their way during a tile's products.  Four warps side by side, two above one another.
-template <class X, class W>
-struct Stream {
-    static constexpr int COLS = 256, ROWS = 32;
-    static constexpr int WROW = COLS * int(sizeof(W)) + 16;   // a row of w: rows 2t of the lanes t fall on different banks
-    static constexpr int MOST_RANK = 64;
-    __host__ __device__ static constexpr int h_bytes(int rank8) { return ROWS * rank8 * 8; }
-    static constexpr int smem(int rank8) { return 2 * base_bytes<X> + 2 * h_bytes(rank8) + rank8 * WROW; }
-};
-
-template <class X, class W>
-__global__ void __launch_bounds__(THREADS, 2) up_stream_kernel(const Args p)
-{
-    using S = Stream<X, W>;
-    using C = Columns<X>;
-    extern __shared__ __align__(16) unsigned char smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int total = p.plan.head[0], first = int((long long)total * blockIdx.x / gridDim.x), last = int((long long)total * (blockIdx.x + 1) / gridDim.x);
-    if (first == last) return;
-    const int c0 = blockIdx.y * S::COLS, in_block = (warp & 3) * 64, n0 = c0 + in_block, half = warp >> 2;
-    const unsigned base_at = shared_address(smem), h_at = base_at + 2 * base_bytes<X>, w_at = h_at + 2 * S::h_bytes(p.rank8);
-    constexpr int PER = THREADS / S::ROWS, HV = S::MOST_RANK / 4 / PER;   // threads a row, and fours of its h that each brings in
-    const int h_row = threadIdx.x / PER, h_rank = threadIdx.x % PER * 4;
-    float4 hv[HV];
-    // what is known of a tile ahead of time: its rows of this lane, the one whose h this thread brings in, and its scale
-    struct Ahead {
-        int4 tile;
-        int row[2], h_m;
-        float scale;
-    };
-    auto tile_of = [&](int i) { return i < last ? p.plan.tiles[i] : make_int4(p.count, 0, 0, 0); };
-    auto rows_of = [&](Ahead& n) {
-        n.row[0] = tile_row(p.plan, n.tile, 16 * half + g);
-        n.row[1] = tile_row(p.plan, n.tile, 16 * half + 8 + g);
-        const bool none = n.tile.x >= p.count;
-        n.h_m = none ? -1 : tile_row(p.plan, n.tile, h_row);
-        n.scale = p.scale && !none ? p.scale[n.tile.x] : 1.f;
-    };
-    auto fetch_h = [&](const Ahead& n) {
-#pragma unroll
-        for (int q = 0; q < HV; ++q)
-            if (h_rank + q * PER * 4 < p.rank8) hv[q] = load_h4(p, n.h_m, h_rank + q * PER * 4);   // used, and waited for, in put_h
-    };
-    auto put_h = [&](const Ahead& n, int buf) {
-        unsigned* h = reinterpret_cast<unsigned*>(smem + 2 * base_bytes<X> + buf * S::h_bytes(p.rank8));
-#pragma unroll
-        for (int q = 0; q < HV; ++q)
-            if (h_rank + q * PER * 4 < p.rank8) put_h4(h, 2, h_row, h_rank + q * PER * 4, hv[q], n.scale);
-    };
-    auto load_all = [&](int adapter) {
-        constexpr int EACH = 16 / sizeof(W), PIECES = S::COLS / EACH;
-        const W* w = static_cast<const W*>(p.w) + (long long)adapter * p.rank * p.width + c0;
-        for (int i = threadIdx.x; i < p.rank8 * PIECES; i += THREADS) {
-            const int r = i / PIECES, c = i % PIECES * EACH;
-            const bool live = r < p.rank && c0 + c < p.width;
-            copy16(w_at + r * S::WROW + c * int(sizeof(W)), live ? w + (long long)r * p.width + c : static_cast<const W*>(p.w), live);
-        }
-        copies_end();
-    };
-    auto issue = [&](const Ahead& n, int buf) {
-        if (p.base) issue_base<X>(p, n.row, n0, base_at + buf * base_bytes<X>);
-        copies_end();
-    };
-    Ahead now, next;
-    now.tile = tile_of(first);
-    next.tile = tile_of(first + 1);
-    rows_of(now);
-    rows_of(next);
-    issue(now, 0);
-    int held = -1;   // whose w is in shared memory
-    if (now.tile.x < p.count) load_all(held = now.tile.x);
-    fetch_h(now);
-    put_h(now, 0);
-    copies_wait<0>();
-    __syncthreads();
-    for (int at = first, buf = 0; at < last; ++at, buf ^= 1) {
-        issue(next, buf ^ 1);
-        fetch_h(next);
-        Ahead then;
-        then.tile = tile_of(at + 2);
-        float acc[8][4] = {};
-        if (now.tile.x < p.count) {
-            const unsigned h = h_at + buf * S::h_bytes(p.rank8) + half * 1024 + lane * 16;
-            const unsigned w = w_at + 2 * t * S::WROW + (in_block + C::RUN * g) * int(sizeof(W));
-            float part[8][4] = {};
-            for (int r = 0; r < p.rank8; r += 8) {
-                float b[2][8];
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int q = 0; q < C::RUNS; ++q) {
-                        const unsigned from = w + (r + e) * S::WROW + 32 * q * int(sizeof(W));
-                        constexpr int BYTES = C::RUN * sizeof(W);
-                        float v[C::RUN];
-                        if constexpr (BYTES == 8) {
-                            const uint2 x = slot8(from);
-                            v[0] = widen<W>((unsigned short)(x.x & 0xFFFFu)), v[1] = widen<W>((unsigned short)(x.x >> 16));
-                            v[2] = widen<W>((unsigned short)(x.y & 0xFFFFu)), v[3] = widen<W>((unsigned short)(x.y >> 16));
-                        } else {
-                            uint4 x[BYTES / 16];
-#pragma unroll
-                            for (int i = 0; i < BYTES / 16; ++i) x[i] = slot(from + 16 * i);
-                            widen_pieces<W>(x, v);
-                        }
-#pragma unroll
-                        for (int i = 0; i < C::RUN; ++i) b[e][q * C::RUN + i] = v[i];
-                    }
-                if constexpr (is_f32<X>) {
-                    up_step<X, W>(part, h + r / 8 * 2048, b);
-                    if (r % 32 == 24) flush(acc, part);
-                } else up_step<X, W>(acc, h + r / 8 * 2048, b);
-            }
-            if constexpr (is_f32<X>)
-                if (p.rank8 % 32) flush(acc, part);
-        }
-        copies_wait<1>();
-        __syncwarp();
-        if (!(now.tile.x >= p.count && p.base == p.out)) finish_rows<X>(p, now.row, n0, base_at + buf * base_bytes<X>, acc);
-        rows_of(then);
-        put_h(next, buf ^ 1);
-        if (next.tile.x < p.count && next.tile.x != held) {
-            __syncthreads();   // everybody is done with the held one
-            load_all(held = next.tile.x);
-            copies_wait<0>();
-        }
-        __syncthreads();
-        now = next, next = then;
-    }
-    copies_wait<0>();
-}
 
 constexpr int GRAD_STAGES = 4;
 template <class X>

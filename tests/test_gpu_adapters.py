@@ -189,7 +189,7 @@ def test_plan(cuda_device, rows, count):
         assert plan.invalid() == 0
     key = torch.where(ids < 0, count, ids)
     words = plan.data.cpu()
-    tile_rows = 16 if rows <= 512 else 32
+    tile_rows = 16 if rows <= 512 else 128
     offsets = words[4:4 + count + 2]
     assert torch.equal(offsets, torch.searchsorted(key.sort().values, torch.arange(count + 2, dtype=torch.int32)).int())
     at = (4 + count + 2 + 3) // 4 * 4

@@ -135,15 +135,6 @@ bool aligned(const void* p, long long stride, int type)
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * (type == DS_T_F32 ? 4 : 2) % 16 == 0;
 }
 
-// CTAs a tile's sums are shared by: until there are two for each SM, as long as every warp keeps a piece of its own.
-int splits_of(const Args& a, int rank_blocks, int pieces)
-{
-    const long long ctas = plan_tiles(a.rows, a.count) * rank_blocks;
-    int s = 1;
-    while (s < 8 && ctas * s * 2 <= 296 && pieces >= 2 * s * WARPS) s *= 2;
-    return s;
-}
-
 int finish()
 {
     note_launch();
@@ -180,47 +171,52 @@ int launch_cluster(dim3 grid, dim3 cluster, int threads, int smem, cudaStream_t 
     return finish();
 }
 
-template <class X, class W, int MT, int NT, bool VEC>
+// Calls whose rows are many and aligned go to the tensor cores' kernels in tiles of 128 (ds_adapters_tc.cuh); those of up to 512 rows, at odd widths or
+// addresses, and such as move less than `least` elements (their sixteen rows a CTA are done before a tile of 128 has its first sums), to mma.sync's.
+bool on_tc(const Args& a, bool vec, long long least) { return plan_tile_rows(a.rows) != 16 && vec && (long long)a.rows * a.width >= least; }
+
+constexpr long long TC_DOWN_LEAST = 1 << 20, TC_UP_LEAST = 1 << 20, TC_GRAD_LEAST = 1 << 20;
+
+template <class X, class W, int NT, bool VEC>
 int launch_down(const Args& a, cudaStream_t st)
 {
-    constexpr int smem = Down<X, W, MT, NT, DOWN_BUDGET>::smem(VEC);
+    constexpr int smem = Down<X, W, 1, NT, DOWN_BUDGET>::smem(VEC);
     static_assert(smem <= 227 * 1024, "shared memory of an SM");
-    if (!allow_smem<down_kernel<X, W, MT, NT, VEC>>(smem)) return DS_ERR_CUDA;
-    const int blocks = (a.rank8 + 8 * NT - 1) / (8 * NT), chunk = 4 * Down<X, W, MT, NT, DOWN_BUDGET>::LK, shares = splits_of(a, blocks, (a.width + chunk - 1) / chunk);
-    return launch_cluster<down_kernel<X, W, MT, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), THREADS, smem, st, a);
+    if (!allow_smem<down_kernel<X, W, NT, VEC>>(smem)) return DS_ERR_CUDA;
+    const int parts = plan_tile_rows(a.rows) / 16, blocks = (a.rank8 + 8 * NT - 1) / (8 * NT), chunk = 4 * Down<X, W, 1, NT, DOWN_BUDGET>::LK;
+    // CTAs that share the sums: until there are two for each SM, as long as every warp keeps a step of its own
+    const long long ctas = (a.rows / 16 + 1ll) * blocks, steps = (a.width + chunk - 1) / chunk;
+    int shares = 1;
+    while (shares < 8 && ctas * shares * 2 <= 296 && steps >= 2 * shares * WARPS) shares *= 2;
+    return launch_cluster<down_kernel<X, W, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks * parts), dim3(1, shares, 1), THREADS, smem, st, a,
+                                                      parts);
 }
 
-// Few rows (tiles of 16).  Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere.
 template <class X, class W>
-int down_few(const Args& a, bool vec, cudaStream_t st)
-{
-    if (!vec) return a.rank8 <= 8 ? launch_down<X, W, 1, 1, false>(a, st) : launch_down<X, W, 1, 4, false>(a, st);
-    if (a.rank8 <= 8) return launch_down<X, W, 1, 1, true>(a, st);
-    if (a.rank8 <= 16) return launch_down<X, W, 1, 2, true>(a, st);
-    if constexpr (Down<X, W, 1, 8, DOWN_BUDGET>::SAME)
-        if (a.rank8 > 32) return launch_down<X, W, 1, 8, true>(a, st);
-    return launch_down<X, W, 1, 4, true>(a, st);
-}
-
-template <class X, class W, bool VEC>
 int launch_tc_down(const Args& a, cudaStream_t st)
 {
     using S = TcDown<X, W>;
     static_assert(S::STAGES >= 2 && TC_ROWS * S::RED * 4 <= S::STAGES * S::STAGE, "stages of a CTA");
-    if (!allow_smem<tc_down_kernel<X, W, VEC>>(S::SMEM)) return DS_ERR_CUDA;
+    if (!allow_smem<tc_down_kernel<X, W>>(S::SMEM)) return DS_ERR_CUDA;
     const int blocks = (a.rank8 + TC_RANKS - 1) / TC_RANKS, chunks = (a.width + 63) / 64;
-    // CTAs a tile's sums are shared by: until each SM has one, as long as each has four steps
+    // CTAs a tile's sums are shared by: until each SM has all that it takes, as long as each has four steps
     const long long tiles = plan_tiles(a.rows, a.count) * blocks;
     int shares = 1;
-    while (shares < 8 && tiles * shares * 2 <= 148 && chunks >= 2 * shares * 4) shares *= 2;
-    return launch_cluster<tc_down_kernel<X, W, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), TC_THREADS, S::SMEM, st, a);
+    while (shares < 8 && tiles * shares * 2 <= 148 * S::CTAS && chunks >= 2 * shares * 4) shares *= 2;
+    return launch_cluster<tc_down_kernel<X, W>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), S::NT + 32, S::SMEM, st, a);
 }
 
+// Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere.
 template <class X, class W>
 int down(const Args& a, bool vec, cudaStream_t st)
 {
-    if (plan_tile_rows(a.rows) == 16) return down_few<X, W>(a, vec, st);
-    return vec ? launch_tc_down<X, W, true>(a, st) : launch_tc_down<X, W, false>(a, st);
+    if (on_tc(a, vec, TC_DOWN_LEAST)) return launch_tc_down<X, W>(a, st);
+    if (!vec) return a.rank8 <= 8 ? launch_down<X, W, 1, false>(a, st) : launch_down<X, W, 4, false>(a, st);
+    if (a.rank8 <= 8) return launch_down<X, W, 1, true>(a, st);
+    if (a.rank8 <= 16) return launch_down<X, W, 2, true>(a, st);
+    if constexpr (Down<X, W, 1, 8, DOWN_BUDGET>::SAME)
+        if (a.rank8 > 32) return launch_down<X, W, 8, true>(a, st);
+    return launch_down<X, W, 4, true>(a, st);
 }
 
 template <class X, class W, bool VEC>
@@ -235,25 +231,25 @@ int launch_up(const Args& a, cudaStream_t st)
     return finish();
 }
 
-template <class X, class W, bool VEC>
+template <class X, class W>
 int launch_tc_up(const Args& a, cudaStream_t st)
 {
     using S = TcUp<X, W>;
     static_assert(S::smem(TC_RANKS) <= 227 * 1024, "shared memory of an SM");
-    if (!allow_smem<tc_up_kernel<X, W, VEC>>(S::smem(TC_RANKS))) return DS_ERR_CUDA;
+    if (!allow_smem<tc_up_kernel<X, W>>(S::smem(TC_RANKS))) return DS_ERR_CUDA;
     const int columns = (a.width + S::COLS - 1) / S::COLS;
     const long long tiles = plan_tiles(a.rows, a.count);
     long long runs = 148 / columns;   // one round
     runs = runs < 1 ? 1 : runs > tiles ? tiles : runs;
-    tc_up_kernel<X, W, VEC><<<dim3(unsigned(runs), columns), TC_THREADS, S::smem((a.rank8 + 15) / 16 * 16), st>>>(a);
+    tc_up_kernel<X, W><<<dim3(unsigned(runs), columns), S::NT + 32, S::smem((a.rank8 + 15) / 16 * 16), st>>>(a);
     return finish();
 }
 
 template <class X, class W>
 int up(const Args& a, bool vec, cudaStream_t st)
 {
-    if (plan_tile_rows(a.rows) == 16 || a.rank8 > TC_RANKS) return vec ? launch_up<X, W, true>(a, st) : launch_up<X, W, false>(a, st);
-    return vec ? launch_tc_up<X, W, true>(a, st) : launch_tc_up<X, W, false>(a, st);
+    if (a.rank8 <= TC_RANKS && on_tc(a, vec, TC_UP_LEAST)) return launch_tc_up<X, W>(a, st);
+    return vec ? launch_up<X, W, true>(a, st) : launch_up<X, W, false>(a, st);
 }
 
 template <class X, class W, int RT, int CW, bool VEC>
@@ -279,23 +275,23 @@ int grad_columns(const Args& a, cudaStream_t st)
     return launch_grad<X, W, RT, 8, VEC>(a, st);
 }
 
-template <class X, class W, bool VEC>
+template <class X, class W>
 int launch_tc_grad(const Args& a, cudaStream_t st)
 {
     using S = TcGrad<X>;
     static_assert(S::STAGES >= 2 && TC_RANKS * S::RED * 4 <= S::STAGES * S::STAGE, "stages of a CTA");
-    if (!allow_smem<tc_grad_kernel<X, W, VEC>>(S::SMEM)) return DS_ERR_CUDA;
+    if (!allow_smem<tc_grad_kernel<X, W>>(S::SMEM)) return DS_ERR_CUDA;
     const int columns = (a.width + 127) / 128, blocks = (a.rank8 + TC_RANKS - 1) / TC_RANKS;
     // CTAs that share an adapter's rows: until each SM has one, as long as each has four steps, were the rows spread evenly
     int shares = 1;
     while (shares < 8 && (long long)columns * a.count * blocks * shares * 2 <= 148 && a.rows / a.count >= 2 * shares * 4 * 64) shares *= 2;
-    return launch_cluster<tc_grad_kernel<X, W, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), TC_THREADS, S::SMEM, st, a);
+    return launch_cluster<tc_grad_kernel<X, W>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), S::NT + 32, S::SMEM, st, a);
 }
 
 template <class X, class W>
 int grad(const Args& a, bool vec, cudaStream_t st)
 {
-    if (plan_tile_rows(a.rows) != 16) return vec ? launch_tc_grad<X, W, true>(a, st) : launch_tc_grad<X, W, false>(a, st);
+    if (on_tc(a, vec, TC_GRAD_LEAST)) return launch_tc_grad<X, W>(a, st);
     if (!vec) return launch_grad<X, W, 2, 4, false>(a, st);
     return a.rank <= 16 ? grad_columns<X, W, 1, true>(a, st) : grad_columns<X, W, 2, true>(a, st);
 }

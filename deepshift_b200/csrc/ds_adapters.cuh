@@ -197,6 +197,9 @@ __device__ __forceinline__ void mma_16bit(float (&d)[4], unsigned a0, unsigned a
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Rows 16 i .. of a tile as a tile of their own (of none, behind its end).
+__device__ __forceinline__ int4 sixteen(const int4& tile, int i) { return make_int4(tile.x, tile.y + 16 * i, min(16, tile.z - 16 * i), 0); }
+
 // Row of lane's fragment rows: position p of the tile, or -1 behind its end.
 __device__ __forceinline__ int tile_row(const PlanView& plan, const int4& tile, int p) { return p < tile.z ? plan.order[tile.y + p] : -1; }
 
@@ -449,28 +452,28 @@ __device__ __forceinline__ float* gather_sums(unsigned char* smem, const float (
     return red;
 }
 
-// h for one tile of 16 MT rows: a CTA's warps share the summed index out among them, and so do the `gridDim.y` CTAs of a cluster,
-// which add up their sums over distributed shared memory, in their order.  blockIdx.z: ranks by 8 NT.
-template <class X, class W, int MT, int NT, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p)
+// h for sixteen rows of a tile of the plan: a CTA's warps share the summed index out among them, and so do the `gridDim.y` CTAs of a cluster,
+// which add up their sums over distributed shared memory, in their order.  blockIdx.z: which sixteen rows, and ranks by 8 NT.
+template <class X, class W, int NT, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p, int parts)
 {
-    constexpr int ROWS = 16 * MT, COLS = 8 * NT;
+    constexpr int COLS = 8 * NT;
     extern __shared__ __align__(16) unsigned char smem[];
     if (int(blockIdx.x) >= p.plan.head[0]) return;
-    const int4 tile = p.plan.tiles[blockIdx.x];
-    if (tile.x >= p.count) return;   // rows without an adapter: nothing reads their h
-    const int r0 = blockIdx.z * COLS, shares = gridDim.y;
-    float acc[MT][NT][4] = {};
-    down_sums<X, W, MT, NT, DOWN_BUDGET, VEC>(p, tile, r0, smem, blockIdx.y * WARPS + (threadIdx.x >> 5), WARPS * shares, acc);
+    const int4 tile = sixteen(p.plan.tiles[blockIdx.x], blockIdx.z % parts);
+    if (tile.x >= p.count || tile.z <= 0) return;   // rows without an adapter: nothing reads their h
+    const int r0 = blockIdx.z / parts * COLS, shares = gridDim.y;
+    float acc[1][NT][4] = {};
+    down_sums<X, W, 1, NT, DOWN_BUDGET, VEC>(p, tile, r0, smem, blockIdx.y * WARPS + (threadIdx.x >> 5), WARPS * shares, acc);
     const float* red = gather_sums(smem, acc, shares > 1);
     if (shares > 1) cluster_sync();
-    for (int i = (blockIdx.y * THREADS + threadIdx.x) * 4; i < ROWS * COLS; i += shares * THREADS * 4) {
+    for (int i = (blockIdx.y * THREADS + threadIdx.x) * 4; i < 16 * COLS; i += shares * THREADS * 4) {
         const int row = i / COLS, r = r0 + i % COLS;
         const int m = tile_row(p.plan, tile, row);
         if (m < 0 || r >= p.rank8) continue;
         float s[4] = {};
         for (int q = 0; q < (shares > 1 ? shares : WARPS); ++q) {
-            const float4 v = shares > 1 ? sums_of(red + i, q) : *reinterpret_cast<const float4*>(red + q * ROWS * COLS + i);
+            const float4 v = shares > 1 ? sums_of(red + i, q) : *reinterpret_cast<const float4*>(red + q * 16 * COLS + i);
             s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
         }
 #pragma unroll
@@ -603,7 +606,7 @@ __device__ __forceinline__ void finish_rows(const Args& p, const int (&row)[2], 
 // The same where rows have no alignment: through shared memory (`stage`, 16 x 65 floats of the warp's own), so that lanes side by
 // side read and write elements side by side.
 template <class X>
-__device__ __forceinline__ void finish_unaligned(const Args& p, const int4& tile, int first, int n0, float* stage, const float (&acc)[8][4])
+__device__ __forceinline__ void finish_unaligned(const Args& p, const int4& tile, int n0, float* stage, const float (&acc)[8][4])
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     __syncwarp();
@@ -617,7 +620,7 @@ __device__ __forceinline__ void finish_unaligned(const Args& p, const int4& tile
             for (int e = 0; e < Columns<X>::UNIT; ++e) stage[(8 * i + g) * 65 + Columns<X>::unit(u, t) + e] = v[e];
         }
     __syncwarp();
-    const int rows = tile_row(p.plan, tile, first + (lane & 15));   // a lane's each
+    const int rows = tile_row(p.plan, tile, lane & 15);   // a lane's each
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += 8) {
         float v[8][2];
@@ -724,20 +727,19 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 {
     extern __shared__ __align__(16) unsigned char smem[];
     if (int(blockIdx.x) >= p.plan.head[0]) return;
-    const int4 tile = p.plan.tiles[blockIdx.x];
+    const int4 tile = sixteen(p.plan.tiles[blockIdx.x], blockIdx.z);
     const bool none = tile.x >= p.count;
-    const int first = 16 * blockIdx.z;
-    if (first >= tile.z || (none && p.base == p.out)) return;   // in place: rows without an adapter are there already
+    if (tile.z <= 0 || (none && p.base == p.out)) return;   // in place: rows without an adapter are there already
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
     const int n0 = (blockIdx.y * WARPS + warp) * 64;
-    const int row[2] = {tile_row(p.plan, tile, first + g), tile_row(p.plan, tile, first + 8 + g)};
+    const int row[2] = {tile_row(p.plan, tile, g), tile_row(p.plan, tile, 8 + g)};
     const unsigned h = shared_address(smem), slots = h + p.rank8 * 16 * 8;
     if (VEC && p.base) issue_base<X>(p, row, n0, slots);
     if (VEC) copies_end();
     if (!none) {
         const float scale = p.scale ? p.scale[tile.x] : 1.f;
         constexpr int PER = THREADS / 16;   // threads a row
-        const int at = threadIdx.x / PER, m = tile_row(p.plan, tile, first + at);
+        const int at = threadIdx.x / PER, m = tile_row(p.plan, tile, at);
         for (int r = threadIdx.x % PER * 4; r < p.rank8; r += PER * 4) put_h4(reinterpret_cast<unsigned*>(smem), at, r, load_h4(p, m, r), scale);
     }
     __syncthreads();
@@ -748,7 +750,7 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
         copies_wait<0>();
         __syncwarp();
         finish_rows<X>(p, row, n0, slots, acc);
-    } else finish_unaligned<X>(p, tile, first, n0, reinterpret_cast<float*>(smem + p.rank8 * 16 * 8) + warp * 16 * 65, acc);
+    } else finish_unaligned<X>(p, tile, n0, reinterpret_cast<float*>(smem + p.rank8 * 16 * 8) + warp * 16 * 65, acc);
 }
 
 // Few rows: both projections of a tile of 16 in one launch (`d`: the down projection's operands, `u`: the up projection's).  The CTAs of
@@ -818,7 +820,7 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
             copies_wait<0>();
             __syncwarp();
             finish_rows<X>(u, row, n0, slots, acc);
-        } else finish_unaligned<X>(u, tile, 0, n0, stage, acc);
+        } else finish_unaligned<X>(u, tile, n0, stage, acc);
     }
 }
 template <class X, class W, int NT>

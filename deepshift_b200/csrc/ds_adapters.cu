@@ -231,24 +231,29 @@ int launch_up(const Args& a, cudaStream_t st)
     return finish();
 }
 
-template <class X, class W>
+template <class X, class W, int NB>
 int launch_tc_up(const Args& a, cudaStream_t st)
 {
-    using S = TcUp<X, W>;
-    static_assert(S::smem(TC_RANKS) <= 227 * 1024, "shared memory of an SM");
-    if (!allow_smem<tc_up_kernel<X, W>>(S::smem(TC_RANKS))) return DS_ERR_CUDA;
+    using S = TcUp<X, W, NB>;
+    constexpr int ranks = is_f32<X> && NB == 3 ? TC_RANKS / 2 : TC_RANKS;
+    static_assert(S::smem(ranks) <= 227 * 1024, "shared memory of an SM");
+    if (!allow_smem<tc_up_kernel<X, W, NB>>(S::smem(ranks))) return DS_ERR_CUDA;
     const int columns = (a.width + S::COLS - 1) / S::COLS;
     const long long tiles = plan_tiles(a.rows, a.count);
     long long runs = 148 / columns;   // one round
     runs = runs < 1 ? 1 : runs > tiles ? tiles : runs;
-    tc_up_kernel<X, W><<<dim3(unsigned(runs), columns), S::NT + 32, S::smem((a.rank8 + 15) / 16 * 16), st>>>(a);
+    tc_up_kernel<X, W, NB><<<dim3(unsigned(runs), columns), S::ALL, S::smem((a.rank8 + 15) / 16 * 16), st>>>(a);
     return finish();
 }
 
 template <class X, class W>
 int up(const Args& a, bool vec, cudaStream_t st)
 {
-    if (a.rank8 <= TC_RANKS && on_tc(a, vec, TC_UP_LEAST)) return launch_tc_up<X, W>(a, st);
+    if (a.rank8 <= TC_RANKS && on_tc(a, vec, TC_UP_LEAST)) {
+        // buffers of base a warp: as many as shared memory holds beside the adapter's planes, which take twice as much for more than 32 ranks
+        if constexpr (is_f32<X>) return a.rank8 <= TC_RANKS / 2 ? launch_tc_up<X, W, 3>(a, st) : launch_tc_up<X, W, 2>(a, st);
+        else return launch_tc_up<X, W, is_f32<W> ? 3 : 5>(a, st);
+    }
     return vec ? launch_up<X, W, true>(a, st) : launch_up<X, W, false>(a, st);
 }
 

@@ -145,23 +145,24 @@ __device__ __forceinline__ void mma_wide(unsigned d, unsigned a, bool a_mn, unsi
 }
 
 // Start and end of a kernel of this kind: barriers and tensor memory, and their return.
+// full_warps hand operands over, acc_warps leave sums; the warp from thread `last` on holds the tensor memory.
 template <int COLUMNS>
-__device__ __forceinline__ void tc_begin(TcShared& s, int warps)
+__device__ __forceinline__ void tc_begin(TcShared& s, int full_warps, int acc_warps, int last)
 {
     if (threadIdx.x == 0) {
         s.err = 0;
         for (int i = 0; i < 4; ++i) {
-            bar_init(&s.full[i], warps);
+            bar_init(&s.full[i], full_warps);
             bar_init(&s.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(&s.acc_full[i], 1);
-            bar_init(&s.acc_empty[i], warps);
+            bar_init(&s.acc_empty[i], acc_warps);
         }
         bar_init(&s.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (int(threadIdx.x) >= 32 * warps) {   // the last warp
+    if (int(threadIdx.x) >= last) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&s.tmem)), "n"(COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -172,10 +173,10 @@ __device__ __forceinline__ void tc_begin(TcShared& s, int warps)
 
 // Behind the last use of tensor memory by any warp and a barrier.
 template <int COLUMNS>
-__device__ __forceinline__ void tc_end(TcShared& s, int warps, int* err_flag)
+__device__ __forceinline__ void tc_end(TcShared& s, int last, int* err_flag)
 {
     if (threadIdx.x == 0 && s.err) *err_flag = 1;
-    if (int(threadIdx.x) >= 32 * warps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "n"(COLUMNS));
+    if (int(threadIdx.x) >= last) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "n"(COLUMNS));
 }
 
 __device__ __forceinline__ TcShared& tc_shared(unsigned char* raw, unsigned& tiles)
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
     unsigned tiles;
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
-    tc_begin<256>(s, S::NW);
+    tc_begin<256>(s, S::NW, 1, S::NT);
     const int t = threadIdx.x, shares = gridDim.y, r0 = blockIdx.z * TC_RANKS;
     const int ranks = min(TC_RANKS, p.rank8 - r0), n = (ranks + 15) / 16 * 16;
     const int chunks = (p.width + 63) / 64, first = int((long long)chunks * blockIdx.y / shares), last = int((long long)chunks * (blockIdx.y + 1) / shares);
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
     }
     if (shares > 1) cluster_sync();   // nobody leaves while its sums are being read
     tc_fence_after();
-    tc_end<256>(s, S::NW, p.err_flag);
+    tc_end<256>(s, S::NT, p.err_flag);
 }
 
 // ---- dw[a] = sum over a's rows of s h^T x: 128 columns x up to 64 ranks, the rows shared out among a cluster's CTAs (blockIdx.z) ----
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
     unsigned tiles;
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
-    tc_begin<256>(s, S::NW);
+    tc_begin<256>(s, S::NW, 1, S::NT);
     const int t = threadIdx.x, shares = gridDim.z, share = blockIdx.z;
     const int blocks = (p.rank8 + TC_RANKS - 1) / TC_RANKS, a = blockIdx.x / blocks, r0 = blockIdx.x % blocks * TC_RANKS, n0 = blockIdx.y * 128;
     const int ranks = min(TC_RANKS, p.rank8 - r0), n = (ranks + 15) / 16 * 16;
@@ -441,69 +442,154 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
     }
     if (shares > 1) cluster_sync();
     tc_fence_after();
-    tc_end<256>(s, S::NW, p.err_flag);
+    tc_end<256>(s, S::NT, p.err_flag);
 }
 
 // ---- out = base + s h up: 128 rows x 256 columns a tile, up to 64 ranks; a CTA takes a run of consecutive tiles ----
-// The adapter's planes stay in shared memory until a tile of another one comes.  A tile's sums are in tensor memory, twice: while the warps add one
-// tile's to base, the next tile's products run.  Lanes read sums by rows and base and out by columns, so each warp turns 32 x 32 of them in
-// shared memory.
-template <class X, class W>
+// Four warps cut the tiles' h, and the adapter's part of w where a tile of another adapter comes; one multiplies; eight add the sums, which are in tensor
+// memory twice so that the next tile's products run meanwhile, to base.  Lanes read sums by rows, and base and out by columns: 32 x 32 of base
+// come to shared memory by columns, several ahead of their sums, which are added by rows, and leave by columns.  (In registers they would
+// take as many as spill, and a load that is spilled is waited for: 102 us instead of 51.)
+template <class X, class W, int NB>
 struct TcUp {
-    static constexpr int NW = 16, NT = 32 * NW, COLS = 256, H = 3 * A_PLANE, TURN = 32 * 36 * 4;
+    static constexpr int NW = 8, NT = 32 * NW, CUT = 4, ALL = NT + 32 * CUT + 32;   // warps that add, all their threads, warps that cut, all threads
+    static constexpr int COLS = 256, H = 3 * A_PLANE;
+    static constexpr int PITCH = 32 * sizeof(X) + 16, BUF = 32 * PITCH;             // a row of 32 elements, 32 rows; NB of them a warp
+    static constexpr int EACH = 16 / sizeof(X), LANES = 32 / EACH, AT_ONCE = 32 / LANES, TIMES = 32 / AT_ONCE;   // 16 bytes a lane, by columns
     __host__ __device__ static constexpr int plane(int n) { return 4 * n * 128; }   // of w: four blocks of 64 columns, n ranks
-    static constexpr int smem(int n) { return H + PLANES<W> * plane(n) + NW * TURN + TC_EXTRA; }
+    static constexpr int smem(int n) { return H + PLANES<W> * plane(n) + NW * NB * BUF + TC_EXTRA; }
 };
 
-// Elements of a row a lane deals with when 32 columns of 32 rows are read by columns, and the rows at a time.
-template <class X>
-struct Turn {
-    static constexpr int EACH = 16 / sizeof(X), LANES = 32 / EACH, AT_ONCE = 32 / LANES, TIMES = 32 / AT_ONCE;
-};
-
-template <class X, class W>
-__global__ void __launch_bounds__(TcUp<X, W>::NT + 32, 1) tc_up_kernel(const Args p)
+template <class X, class W, int NB>
+__global__ void __launch_bounds__(TcUp<X, W, NB>::ALL, 1) tc_up_kernel(const Args p)
 {
-    using S = TcUp<X, W>;
-    using T = Turn<X>;
+    using S = TcUp<X, W, NB>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int total = p.plan.head[0], first = int((long long)total * blockIdx.x / gridDim.x), last = int((long long)total * (blockIdx.x + 1) / gridDim.x);
     if (first == last) return;
     unsigned tiles;
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
-    tc_begin<512>(s, S::NW);
+    tc_begin<512>(s, S::CUT, S::NW, S::ALL - 32);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n0 = blockIdx.y * S::COLS;
     const int k16 = (p.rank8 + 15) / 16 * 16;
     const unsigned h_at = tiles, w_at = tiles + S::H;
+    auto tile_at = [&](int i) { return i < last ? p.plan.tiles[i] : make_int4(p.count, 0, 0, 0); };
     if (t < S::NT) {
-        const int piece = t & 7, quarter = warp & 3, c0 = n0 + (warp >> 2) * 64;   // a warp's 32 rows and 64 columns
-        // what is known of a tile ahead of time: the lane's row of the warp's 32, the rows whose h this thread brings in, the scale
-        struct Ahead {
-            int4 tile;
-            int row, m[2];
-            float scale;
-        } now, next;
-        auto look = [&](Ahead& q, int i) {
-            q.tile = i < last ? p.plan.tiles[i] : make_int4(p.count, 0, 0, 0);
-            q.row = tile_row(p.plan, q.tile, quarter * 32 + lane);
+        const int quarter = warp & 3, c0 = n0 + (warp >> 2) * 128;   // a warp's 32 rows and 128 columns
+        const unsigned bufs = tiles + S::H + PLANES<W> * S::plane(k16) + warp * NB * S::BUF, by_row = lane * S::PITCH,
+                       by_column = lane / S::LANES * S::PITCH + lane % S::LANES * 16;
+        const X* base = static_cast<const X*>(p.base);
+        X* out = static_cast<X*>(p.out);
+        // base of 32 columns from c of the warp's rows (each lane knows one) to a buffer
+        auto issue = [&](int rows, int c, int buf) {
+            if (base) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) q.m[e] = q.tile.x < p.count && piece * 8 < p.rank8 ? tile_row(p.plan, q.tile, (t >> 3) + 64 * e) : -1;
-            q.scale = p.scale && q.tile.x < p.count ? p.scale[q.tile.x] : 1.f;
+                for (int k = 0; k < S::TIMES; ++k) {
+                    const int m = __shfl_sync(0xFFFFFFFFu, rows, S::AT_ONCE * k + lane / S::LANES), n = c + lane % S::LANES * S::EACH;
+                    const bool live = m >= 0 && n < p.width;
+                    copy16(bufs + buf * S::BUF + by_column + S::AT_ONCE * k * S::PITCH, base + (live ? m * p.ldbase + n : 0), live);
+                }
+            }
+            copies_end();
         };
-        Raw<float> h[2];
-        auto fetch_h = [&](const Ahead& q) {
+        // the buffer's 32 columns from c, whose sums begin at column `from` of tensor memory
+        auto finish = [&](int rows, int c, int buf, int from, bool none) {
+            copies_wait<NB - 1>();
+            __syncwarp();
+            const unsigned at = bufs + buf * S::BUF;
+            if (!none || !base) {
+                int v[32];
+                if (!none) tmem_ld(s.tmem + (unsigned(quarter * 32) << 16) + from, v);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) load_raw<float>(p.h + (q.m[e] >= 0 ? (long long)q.m[e] * p.rank8 + piece * 8 : 0), q.m[e] >= 0, h[e]);
+                for (int e = 0; e < 32; e += S::EACH) {
+                    const unsigned here = at + by_row + e * int(sizeof(X));
+                    float b[S::EACH] = {};
+                    if (base) {
+                        const uint4 x[1] = {slot(here)};
+                        widen_pieces<X>(x, b);
+                    }
+                    unsigned w[4];
+#pragma unroll
+                    for (int i = 0; i < S::EACH; ++i) b[i] += none ? 0.f : __int_as_float(v[e + i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (is_f32<X>) w[i] = __float_as_uint(b[i]);
+                        else w[i] = narrow<X>(b[2 * i]) | unsigned(narrow<X>(b[2 * i + 1])) << 16;
+                    }
+                    store_piece(here, make_uint4(w[0], w[1], w[2], w[3]));
+                }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int k = 0; k < S::TIMES; ++k) {
+                const int m = __shfl_sync(0xFFFFFFFFu, rows, S::AT_ONCE * k + lane / S::LANES), n = c + lane % S::LANES * S::EACH;
+                const uint4 w = slot(at + by_column + S::AT_ONCE * k * S::PITCH);
+                if (m >= 0 && n < p.width) *reinterpret_cast<uint4*>(out + m * p.ldout + n) = w;
+            }
+            __syncwarp();
         };
-        int held = -1;
-        auto give = [&](const Ahead& q) {   // the tile's h, and its adapter's part of w if another's is there
-            if (q.tile.x != held) {
-                held = q.tile.x;
+        // groups of 32 columns, four a tile: NB - 1 are on their way ahead of the one that is being added
+        int4 tile = tile_at(first), next = tile_at(first + 1);
+        int rows = tile_row(p.plan, tile, quarter * 32 + lane), next_rows = tile_row(p.plan, next, quarter * 32 + lane);
+        int buf = 0;
+#pragma unroll
+        for (int g = 0; g < NB - 1; ++g) issue(g < 4 ? rows : next_rows, c0 + g % 4 * 32, g);
+        unsigned phase = 0;
+        for (int i = first, acc = 0; i < last; ++i) {
+            const bool none = tile.x >= p.count;
+            const int4 then = tile_at(i + 2);
+            if (!none) {
+                if (!__all_sync(0xFFFFFFFFu, bar_wait(&s.acc_full[acc], phase, err, TC_WAIT))) break;
+                tc_fence_after();
+            } else if (p.base == p.out) break;   // in place, and rows without an adapter come last: they are there already
+            int then_rows = -1;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                // the group NB - 1 further on goes to the buffer that the last one has left
+                static_assert(NB <= 5, "groups of this tile and the next");
+                issue(g + NB - 1 < 4 ? rows : next_rows, c0 + (g + NB - 1) % 4 * 32, buf == 0 ? NB - 1 : buf - 1);
+                finish(rows, c0 + g * 32, buf, acc * 256 + (warp >> 2) * 128 + g * 32, none);
+                buf = buf + 1 == NB ? 0 : buf + 1;
+                if (g == 2) then_rows = tile_row(p.plan, then, quarter * 32 + lane);
+            }
+            if (!none) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&s.acc_empty[acc]);
+                if (acc ^= 1; acc == 0) phase ^= 1;
+            }
+            tile = next, next = then, rows = next_rows, next_rows = then_rows;
+        }
+        copies_wait<0>();
+    } else if (t < S::NT + 32 * S::CUT) {
+        constexpr int CT = 32 * S::CUT, HI = 1024 / CT;   // pieces of eight of h a thread: its rows are CT / 8 apart
+        const int u = t - S::NT, piece = u & 7;
+        const bool there = piece * 8 < p.rank8;
+        int m[HI], held = -1;
+        float scale = 1.f;
+        auto look = [&](const int4& tile) {
+#pragma unroll
+            for (int e = 0; e < HI; ++e) m[e] = there && tile.x < p.count ? tile_row(p.plan, tile, (u >> 3) + CT / 8 * e) : -1;
+            scale = p.scale && tile.x < p.count ? p.scale[tile.x] : 1.f;
+        };
+        int4 tile = tile_at(first);
+        look(tile);
+        unsigned phase = 1;   // of the products that read the previous tile's h: none before the first
+        for (int i = first, buf = 1; i < last && tile.x < p.count; ++i) {
+            const int4 next = tile_at(i + 1);
+            Raw<float> h[HI];
+#pragma unroll
+            for (int e = 0; e < HI; ++e) load_raw<float>(p.h + (m[e] >= 0 ? (long long)m[e] * p.rank8 + piece * 8 : 0), m[e] >= 0, h[e]);
+            const float by = scale;
+            look(next);
+            if (!__all_sync(0xFFFFFFFFu, bar_wait(&s.acc_full[buf], phase, err, TC_WAIT))) break;
+            if (tile.x != held) {
+                held = tile.x;
                 const W* w = static_cast<const W*>(p.w) + (long long)held * p.rank * p.width + n0;
-#pragma unroll 2
-                for (int i = t; i < k16 * 32; i += S::NT) {
-                    const int r = i >> 5, c = i & 31;
+#pragma unroll 4
+                for (int j = u; j < k16 * 32; j += CT) {
+                    const int r = j >> 5, c = j & 31;
                     Raw<W> x;
                     load_raw<W>(w + (long long)r * p.width + c * 8, r < p.rank && n0 + c * 8 < p.width, x);
                     put_planes<W>(w_at + (c >> 3) * k16 * 128, S::plane(k16), r, c & 7, x);
@@ -511,88 +597,11 @@ __global__ void __launch_bounds__(TcUp<X, W>::NT + 32, 1) tc_up_kernel(const Arg
             }
             if (piece * 8 < k16) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) put_planes<float>(h_at, A_PLANE, (t >> 3) + 64 * e, piece, times(h[e], q.scale));
+                for (int e = 0; e < HI; ++e) put_planes<float>(h_at, A_PLANE, (u >> 3) + CT / 8 * e, piece, times(h[e], by));
             }
             hand_over(&s.full[0]);
-        };
-        float* turn = reinterpret_cast<float*>(smem + (tiles - shared_address(smem)) + S::H + PLANES<W> * S::plane(k16)) + warp * (S::TURN / 4);
-        const X* base = static_cast<const X*>(p.base);
-        X* out = static_cast<X*>(p.out);
-        // base of 32 columns from c: of row AT_ONCE k + lane / LANES, EACH elements
-        auto fetch_base = [&](const Ahead& a, int c, uint4 (&q)[T::TIMES]) {
-#pragma unroll
-            for (int k = 0; k < T::TIMES; ++k) {
-                const int m = __shfl_sync(0xFFFFFFFFu, a.row, T::AT_ONCE * k + lane / T::LANES), n = c + lane % T::LANES * T::EACH;
-                q[k] = base && m >= 0 && n < p.width ? *reinterpret_cast<const uint4*>(base + m * p.ldbase + n) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        // 32 columns from c, whose sums begin at column `from` of tensor memory (none: zeros)
-        auto finish = [&](const Ahead& a, int c, int from, bool none, const uint4 (&q)[T::TIMES]) {
-            __syncwarp();
-            if (!none) {
-                int v[32];
-                tmem_ld(s.tmem + (unsigned(quarter * 32) << 16) + from, v);
-#pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    *reinterpret_cast<float4*>(turn + lane * 36 + e) =
-                        make_float4(__int_as_float(v[e]), __int_as_float(v[e + 1]), __int_as_float(v[e + 2]), __int_as_float(v[e + 3]));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(turn + lane * 36 + e) = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < T::TIMES; ++k) {
-                const int row = T::AT_ONCE * k + lane / T::LANES, col = lane % T::LANES * T::EACH;
-                const int m = __shfl_sync(0xFFFFFFFFu, a.row, row);
-                const uint4 x[1] = {q[k]};
-                float b[T::EACH];
-                widen_pieces<X>(x, b);
-                unsigned w[4];
-#pragma unroll
-                for (int e = 0; e < T::EACH; e += 4) {
-                    const float4 d = *reinterpret_cast<const float4*>(turn + row * 36 + col + e);
-                    b[e] += d.x, b[e + 1] += d.y, b[e + 2] += d.z, b[e + 3] += d.w;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (is_f32<X>) w[e] = __float_as_uint(b[e]);
-                    else w[e] = narrow<X>(b[2 * e]) | unsigned(narrow<X>(b[2 * e + 1])) << 16;
-                }
-                if (m >= 0 && c + col < p.width) *reinterpret_cast<uint4*>(out + m * p.ldout + c + col) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        };
-        look(now, first);
-        if (now.tile.x < p.count) {
-            fetch_h(now);
-            give(now);
-        }
-        look(next, first + 1);
-        uint4 left[T::TIMES], right[T::TIMES];   // base of the warp's two halves of 32 columns
-        fetch_base(now, c0, left);
-        unsigned phase = 0;
-        for (int i = first, buf = 0; i < last; ++i) {
-            const bool none = now.tile.x >= p.count, skip = none && p.base == p.out;
-            fetch_base(now, c0 + 32, right);
-            if (next.tile.x < p.count) fetch_h(next);
-            Ahead then;
-            look(then, i + 2);
-            if (!none) {
-                if (!__all_sync(0xFFFFFFFFu, bar_wait(&s.acc_full[buf], phase, err, TC_WAIT))) break;
-                tc_fence_after();
-            }
-            if (next.tile.x < p.count) give(next);   // the products that read the previous tile's operands are done
-            const int from = buf * 256 + (warp >> 2) * 64;
-            if (!skip) finish(now, c0, from, none, left);
-            fetch_base(next, c0, left);
-            if (!skip) finish(now, c0 + 32, from + 32, none, right);
-            if (!none) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&s.acc_empty[buf]);
-                if (buf ^= 1; buf == 0) phase ^= 1;
-            }
-            now = next, next = then;
+            tile = next;
+            if (buf ^= 1; buf == 0) phase ^= 1;
         }
     } else if (elect_one()) {
         const unsigned idesc = tc_idesc(false, true, S::COLS);
@@ -623,7 +632,7 @@ __global__ void __launch_bounds__(TcUp<X, W>::NT + 32, 1) tc_up_kernel(const Arg
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    tc_end<512>(s, S::NW, p.err_flag);
+    tc_end<512>(s, S::ALL - 32, p.err_flag);
 }
 
 }  // namespace adapters

@@ -475,6 +475,29 @@ __global__ void __launch_bounds__(TcUp<X, W, NB>::ALL, 1) tc_up_kernel(const Arg
     const int k16 = (p.rank8 + 15) / 16 * 16;
     const unsigned h_at = tiles, w_at = tiles + S::H;
     auto tile_at = [&](int i) { return i < last ? p.plan.tiles[i] : make_int4(p.count, 0, 0, 0); };
+    // an adapter's part of w, cut, by threads u of `threads`; four loads of each at a time
+    auto stage_w = [&](int adapter, int u, int threads) {
+        const W* w = static_cast<const W*>(p.w) + (long long)adapter * p.rank * p.width + n0;
+        for (int j0 = u; j0 < k16 * 32; j0 += 4 * threads) {
+            Raw<W> x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = j0 + e * threads, r = j >> 5, c = j & 31;
+                load_raw<W>(w + (long long)r * p.width + c * 8, r < p.rank && n0 + c * 8 < p.width, x[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = j0 + e * threads, r = j >> 5, c = j & 31;
+                if (j < k16 * 32) put_planes<W>(w_at + (c >> 3) * k16 * 128, S::plane(k16), r, c & 7, x[e]);
+            }
+        }
+    };
+    const int first_adapter = tile_at(first).x;
+    if (first_adapter < p.count) {   // the first one's by all threads: nobody has anything else to do yet
+        stage_w(first_adapter, t, S::ALL);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
     if (t < S::NT) {
         const int quarter = warp & 3, c0 = n0 + (warp >> 2) * 128;   // a warp's 32 rows and 128 columns
         const unsigned bufs = tiles + S::H + PLANES<W> * S::plane(k16) + warp * NB * S::BUF, by_row = lane * S::PITCH,
@@ -566,7 +589,7 @@ __global__ void __launch_bounds__(TcUp<X, W, NB>::ALL, 1) tc_up_kernel(const Arg
         constexpr int CT = 32 * S::CUT, HI = 1024 / CT;   // pieces of eight of h a thread: its rows are CT / 8 apart
         const int u = t - S::NT, piece = u & 7;
         const bool there = piece * 8 < p.rank8;
-        int m[HI], held = -1;
+        int m[HI], held = first_adapter;
         float scale = 1.f;
         auto look = [&](const int4& tile) {
 #pragma unroll
@@ -586,14 +609,7 @@ __global__ void __launch_bounds__(TcUp<X, W, NB>::ALL, 1) tc_up_kernel(const Arg
             if (!__all_sync(0xFFFFFFFFu, bar_wait(&s.acc_full[buf], phase, err, TC_WAIT))) break;
             if (tile.x != held) {
                 held = tile.x;
-                const W* w = static_cast<const W*>(p.w) + (long long)held * p.rank * p.width + n0;
-#pragma unroll 4
-                for (int j = u; j < k16 * 32; j += CT) {
-                    const int r = j >> 5, c = j & 31;
-                    Raw<W> x;
-                    load_raw<W>(w + (long long)r * p.width + c * 8, r < p.rank && n0 + c * 8 < p.width, x);
-                    put_planes<W>(w_at + (c >> 3) * k16 * 128, S::plane(k16), r, c & 7, x);
-                }
+                stage_w(held, u, CT);
             }
             if (piece * 8 < k16) {
 #pragma unroll

@@ -171,11 +171,12 @@ int launch_cluster(dim3 grid, dim3 cluster, int threads, int smem, cudaStream_t 
     return finish();
 }
 
-// Calls whose rows are many and aligned go to the tensor cores' kernels in tiles of 128 (ds_adapters_tc.cuh); those of up to 512 rows, at odd widths or
-// addresses, and such as move less than `least` elements (their sixteen rows a CTA are done before a tile of 128 has its first sums), to mma.sync's.
-bool on_tc(const Args& a, bool vec, long long least) { return plan_tile_rows(a.rows) != 16 && vec && (long long)a.rows * a.width >= least; }
-
-constexpr long long TC_DOWN_LEAST = 1 << 20, TC_UP_LEAST = 1 << 20, TC_GRAD_LEAST = 1 << 20;
+// Projections of many aligned rows go to the tensor cores' kernels in tiles of 128 (ds_adapters_tc.cuh); those of up to 512 rows, at odd widths or
+// addresses, and small ones to mma.sync's, whose tiles of sixteen have their sums before one of 128 has its first (a tile, its rows'
+// indexes, their h, and planes cut from it, one after the other: 20 us for any call that small).  Both projections measured together at
+// 520 .. 4096 rows of 256 .. 4096 and ranks of 8, 16, 64 take as long either way where rows x width x rank is 1.3 to 2.7 10^8: 2048 x 1024 of rank 64 in
+// fp32 25.4 and 24.7 us, 4096 x 4096 of rank 16 66 and 72, in bf16 41 and 45; a quarter of that 24.7 and 18, four times that 72 and 142.
+bool on_tc(const Args& a, bool vec) { return plan_tile_rows(a.rows) != 16 && vec && double(a.rows) * a.width * a.rank8 >= 2e8; }
 
 template <class X, class W, int NT, bool VEC>
 int launch_down(const Args& a, cudaStream_t st)
@@ -210,7 +211,7 @@ int launch_tc_down(const Args& a, cudaStream_t st)
 template <class X, class W>
 int down(const Args& a, bool vec, cudaStream_t st)
 {
-    if (on_tc(a, vec, TC_DOWN_LEAST)) return launch_tc_down<X, W>(a, st);
+    if (on_tc(a, vec)) return launch_tc_down<X, W>(a, st);
     if (!vec) return a.rank8 <= 8 ? launch_down<X, W, 1, false>(a, st) : launch_down<X, W, 4, false>(a, st);
     if (a.rank8 <= 8) return launch_down<X, W, 1, true>(a, st);
     if (a.rank8 <= 16) return launch_down<X, W, 2, true>(a, st);
@@ -249,7 +250,7 @@ int launch_tc_up(const Args& a, cudaStream_t st)
 template <class X, class W>
 int up(const Args& a, bool vec, cudaStream_t st)
 {
-    if (a.rank8 <= TC_RANKS && on_tc(a, vec, TC_UP_LEAST)) {
+    if (a.rank8 <= TC_RANKS && on_tc(a, vec)) {
         // buffers of base a warp: as many as shared memory holds beside the adapter's planes, which take twice as much for more than 32 ranks
         if constexpr (is_f32<X>) return a.rank8 <= TC_RANKS / 2 ? launch_tc_up<X, W, 3>(a, st) : launch_tc_up<X, W, 2>(a, st);
         else return launch_tc_up<X, W, is_f32<W> ? 3 : 5>(a, st);
@@ -257,27 +258,17 @@ int up(const Args& a, bool vec, cudaStream_t st)
     return vec ? launch_up<X, W, true>(a, st) : launch_up<X, W, false>(a, st);
 }
 
-template <class X, class W, int RT, int CW, bool VEC>
+template <class X, class W>
 int launch_grad(const Args& a, cudaStream_t st)
 {
-    constexpr int RW = WARPS / CW, block = RW == 8 ? 64 : 32;
-    constexpr int sums = RW * 16 * RT * 64 * CW * 4, work = 2 * block * 16 * RT * 8 + (VEC ? GRAD_STAGES * THREADS * 16 * grad_pieces<X> : 0);
-    constexpr int smem = sums > work ? sums : work;
-    if (!allow_smem<grad_kernel<X, W, RT, CW, VEC>>(smem)) return DS_ERR_CUDA;
-    const int columns = (a.width + 64 * CW - 1) / (64 * CW), blocks = (a.rank + 16 * RT - 1) / (16 * RT);
+    using G = Grad;
+    if (!allow_smem<grad_kernel<X, W>>(G::SMEM)) return DS_ERR_CUDA;
+    const int columns = (a.width + G::COLS - 1) / G::COLS, blocks = (a.rank + G::RANKS - 1) / G::RANKS;
     // CTAs that share an adapter's rows: until two for each SM are at work, as long as each has two blocks of rows, were the
     // rows spread evenly
     int shares = 1;
-    while (shares < 8 && (long long)columns * a.count * blocks * shares < 296 && a.rows / a.count >= 2 * shares * 2 * block) shares *= 2;
-    return launch_cluster<grad_kernel<X, W, RT, CW, VEC>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), THREADS, smem, st, a);
-}
-
-template <class X, class W, int RT, bool VEC>
-int grad_columns(const Args& a, cudaStream_t st)
-{
-    if (a.width <= 64) return launch_grad<X, W, RT, 1, VEC>(a, st);
-    if (a.width <= 256) return launch_grad<X, W, RT, 4, VEC>(a, st);
-    return launch_grad<X, W, RT, 8, VEC>(a, st);
+    while (shares < 8 && (long long)columns * a.count * blocks * shares < 296 && a.rows / a.count >= 2 * shares * 2 * G::BLOCK) shares *= 2;
+    return launch_cluster<grad_kernel<X, W>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), THREADS, G::SMEM, st, a);
 }
 
 template <class X, class W>
@@ -293,12 +284,11 @@ int launch_tc_grad(const Args& a, cudaStream_t st)
     return launch_cluster<tc_grad_kernel<X, W>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), S::NT + 32, S::SMEM, st, a);
 }
 
+// Aligned ones on the tensor cores whatever their number of rows: 520 x 1024 of rank 16 in fp32 10.3 us against mma.sync's 17.5, 4096 x 4096 22 against 61.
 template <class X, class W>
 int grad(const Args& a, bool vec, cudaStream_t st)
 {
-    if (on_tc(a, vec, TC_GRAD_LEAST)) return launch_tc_grad<X, W>(a, st);
-    if (!vec) return launch_grad<X, W, 2, 4, false>(a, st);
-    return a.rank <= 16 ? grad_columns<X, W, 1, true>(a, st) : grad_columns<X, W, 2, true>(a, st);
+    return vec ? launch_tc_grad<X, W>(a, st) : launch_grad<X, W>(a, st);
 }
 
 template <class X, class W, int NT, bool VEC>

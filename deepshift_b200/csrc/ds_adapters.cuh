@@ -125,32 +125,15 @@ __device__ __forceinline__ void load(const T* p, int live, float (&v)[N])
     }
 }
 
-template <class T, int N, bool VEC>
+// The first `live` of N elements.
+template <class T, int N>
 __device__ __forceinline__ void store(T* p, int live, const float (&v)[N])
 {
-    if (VEC && live >= N) {
-        if constexpr (is_f32<T>) {
 #pragma unroll
-            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else {
-            static_assert(N % 8 == 0, "whole 16-byte stores");
-#pragma unroll
-            for (int i = 0; i < N; i += 8) {
-                unsigned w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = narrow<T>(v[i + 2 * e]) | unsigned(narrow<T>(v[i + 2 * e + 1])) << 16;
-                *reinterpret_cast<uint4*>(p + i) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-        return;
-    }
-    if constexpr (!VEC) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i < live) {
-                if constexpr (is_f32<T>) p[i] = v[i];
-                else reinterpret_cast<unsigned short*>(p)[i] = narrow<T>(v[i]);
-            }
+    for (int i = 0; i < N; ++i) {
+        if (i < live) {
+            if constexpr (is_f32<T>) p[i] = v[i];
+            else reinterpret_cast<unsigned short*>(p)[i] = narrow<T>(v[i]);
         }
     }
 }
@@ -826,22 +809,22 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
 template <class X, class W, int NT>
 constexpr int both_smem(bool vec) { return Down<X, W, 1, NT, BOTH_BUDGET>::smem(vec) + 8 * NT * 16 * 8 + (vec ? base_bytes<X> : WARPS * 16 * 65 * 4); }
 
-constexpr int GRAD_STAGES = 4;
-template <class X>
-constexpr int grad_pieces = 8 * sizeof(X) / 16 * 2;   // of a lane's eight columns of two rows
+// dw[a][r0 .. r0 + 32)[n0 .. n0 + 256) over all rows of adapter a, at odd widths or addresses (aligned ones go to tc_grad_kernel).  Four warps side
+// by side, two above one another, share a block of 32 rows whose h, scaled and split, lies in shared memory in the order in which the
+// instructions read it; the next block's is on its way meanwhile.  The `gridDim.z` CTAs of a cluster take one part of the rows each and
+// add up their sums over distributed shared memory, in their order.
+struct Grad {
+    static constexpr int RT = 2, RANKS = 16 * RT, CW = 4, COLS = 64 * CW, RW = WARPS / CW, BLOCK = 32, STEPS = BLOCK / 8 / RW;
+    static constexpr int H_BYTES = BLOCK * RANKS * 8, SUMS = RW * RANKS * COLS * 4, SMEM = SUMS > 2 * H_BYTES ? SUMS : 2 * H_BYTES;
+};
 
-// dw[a][r0 .. r0 + 16 RT)[n0 .. n0 + 64 CW) over all rows of adapter a.  CW warps side by side, 8 / CW above one another, share a block of rows
-// whose h, scaled and split, lies in shared memory in the order in which the instructions read it; the next block's is on its way meanwhile, and
-// each lane's rows are several steps ahead.  The `gridDim.z` CTAs of a cluster take one part of the rows each and add up their
-// sums over distributed shared memory, in their order.
-template <class X, class W, int RT, int CW, bool VEC>
+template <class X, class W>
 __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
 {
-    constexpr int NJ = 8, RANKS = 16 * RT, COLS = 8 * NJ * CW, XP = grad_pieces<X> / 2, STAGE = THREADS * 16 * grad_pieces<X>;
-    constexpr int RW = WARPS / CW, BLOCK = RW == 8 ? 64 : 32, STEPS = BLOCK / 8 / RW;   // rows of a block, steps of a warp in it
-    constexpr int HV = (BLOCK * RANKS / 4 + THREADS - 1) / THREADS, H_BYTES = BLOCK * RANKS * 8;
-    extern __shared__ __align__(16) unsigned char smem[];   // h of two blocks, then the queue
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, cw = warp % CW, rw = warp / CW;
+    using G = Grad;
+    constexpr int NJ = 8, RT = G::RT, RANKS = G::RANKS, COLS = G::COLS, BLOCK = G::BLOCK;
+    extern __shared__ __align__(16) unsigned char smem[];   // h of two blocks; at the end the sums
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, cw = warp % G::CW, rw = warp / G::CW;
     const int blocks = (p.rank + RANKS - 1) / RANKS;
     const int a = blockIdx.x / blocks, n0 = blockIdx.y * COLS + 64 * cw, r0 = blockIdx.x % blocks * RANKS;
     const int shares = gridDim.z, share = blockIdx.z;
@@ -851,128 +834,75 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
     const float scale = p.scale ? p.scale[a] : 1.f;
     const int count = (end - begin + BLOCK - 1) / BLOCK;
     float acc[RT][NJ][4] = {};
-    // step i of this warp: rows 8 (i % STEPS RW + rw) ... of block i / STEPS
-    auto row_at = [&](int i, int e) {
-        const int at = begin + i / STEPS * BLOCK + (i % STEPS * RW + rw) * 8 + 2 * t + e;
-        return at < end ? p.plan.order[at] : -1;
+    static_assert(BLOCK * RANKS / 4 == THREADS, "four values of h a thread");
+    const int h_rank = threadIdx.x % (RANKS / 4) * 4, h_row = threadIdx.x / (RANKS / 4);
+    float4 hv;
+    int h_m;   // row of the block whose h is brought in next, read a block before
+    auto fetch_row = [&](int block) {
+        const int at = begin + block * BLOCK + h_row;
+        h_m = at < end && r0 + h_rank < p.rank8 ? p.plan.order[at] : -1;
     };
-    float4 hv[HV];
-    int h_m[HV];   // rows of the block whose h is brought in next, read a block before
-    auto fetch_rows = [&](int block) {
-#pragma unroll
-        for (int q = 0; q < HV; ++q) {
-            const int i = threadIdx.x + q * THREADS, r = r0 + i % (RANKS / 4) * 4, at = begin + block * BLOCK + i / (RANKS / 4);
-            h_m[q] = i < BLOCK * RANKS / 4 && at < end && r < p.rank8 ? p.plan.order[at] : -1;
-        }
-    };
-    auto fetch_h = [&] {
-#pragma unroll
-        for (int q = 0; q < HV; ++q) hv[q] = load_h4(p, h_m[q], r0 + (threadIdx.x + q * THREADS) % (RANKS / 4) * 4);
-    };
+    auto fetch_h = [&] { hv = load_h4(p, h_m, r0 + h_rank); };
     auto put_h = [&](int buf) {   // as put_h4, but of an operand [rank][row]: blocks [row / 8][RT][hi, lo][lane][4]
-        unsigned* h = reinterpret_cast<unsigned*>(smem + buf * H_BYTES);
-#pragma unroll
-        for (int q = 0; q < HV; ++q) {
-            const int i = threadIdx.x + q * THREADS, r = i % (RANKS / 4) * 4, at = i / (RANKS / 4);
-            if (i >= BLOCK * RANKS / 4) continue;
-            unsigned* to = h + (at / 8 * RT + r / 16) * 256 + (r % 8 * 4 + at % 8 / 2) * 4 + (r / 8 & 1) + 2 * (at & 1);
-            put_parts(to, hv[q].x * scale);
-            put_parts(to + 16, hv[q].y * scale);
-            put_parts(to + 32, hv[q].z * scale);
-            put_parts(to + 48, hv[q].w * scale);
-        }
+        unsigned* to = reinterpret_cast<unsigned*>(smem + buf * G::H_BYTES) + (h_row / 8 * RT + h_rank / 16) * 256 + (h_rank % 8 * 4 + h_row % 8 / 2) * 4 +
+                       (h_rank / 8 & 1) + 2 * (h_row & 1);
+        put_parts(to, hv.x * scale);
+        put_parts(to + 16, hv.y * scale);
+        put_parts(to + 32, hv.z * scale);
+        put_parts(to + 48, hv.w * scale);
     };
-    auto products = [&](const float (&b)[2][NJ], unsigned h) {
-        unsigned ah[RT][4], al[RT][4];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const uint4 u = slot(h + i * 1024), v = slot(h + i * 1024 + 512);
-            ah[i][0] = u.x, ah[i][1] = u.y, ah[i][2] = u.z, ah[i][3] = u.w;
-            al[i][0] = v.x, al[i][1] = v.y, al[i][2] = v.z, al[i][3] = v.w;
-        }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            unsigned h0, h1, l0, l1;
-            parts<!is_f32<X>>(b[0][j], h0, l0);
-            parts<!is_f32<X>>(b[1][j], h1, l1);
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                float s[4] = {};   // as in down_step
-                float(&d)[4] = is_f32<W> ? s : acc[i][j];
-                mma_tf32(d, al[i], h0, h1);
-                if (is_f32<X>) mma_tf32(d, ah[i], l0, l1);
-                mma_tf32(d, ah[i], h0, h1);
-                if (is_f32<W>) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] += s[e];
-                }
-            }
-        }
-    };
-    const unsigned mine = shared_address(smem) + 2 * H_BYTES + threadIdx.x * 16;
-    auto issue = [&](const int (&m)[2], int stage) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int q = 0; q < XP; ++q) {
-                const int n = n0 + 32 * q + Columns<X>::RUN * g;
-                const bool in = m[e] >= 0 && n < p.width;
-                copy16(mine + stage * STAGE + (e * XP + q) * THREADS * 16, static_cast<const X*>(p.x) + (in ? m[e] * p.ldx + n : 0), in);
-            }
-        copies_end();
-    };
-    int rows[2], stage = 0, ahead = GRAD_STAGES - 1;   // the rows of the step whose copies begin next
-    if constexpr (VEC) {
-#pragma unroll
-        for (int i = 0; i < GRAD_STAGES - 1; ++i) {
-            const int m[2] = {row_at(i, 0), row_at(i, 1)};
-            issue(m, i);
-        }
-        rows[0] = row_at(GRAD_STAGES - 1, 0), rows[1] = row_at(GRAD_STAGES - 1, 1);
-    }
-    fetch_rows(0);
+    fetch_row(0);
     fetch_h();
-    fetch_rows(1);
+    fetch_row(1);
     put_h(0);
     __syncthreads();
     for (int block = 0; block < count; ++block) {
         fetch_h();
-        fetch_rows(block + 2);
+        fetch_row(block + 2);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const int i = block * STEPS + s;
-            const unsigned h = shared_address(smem) + (block & 1) * H_BYTES + (s * RW + rw) * RT * 1024 + lane * 16;
+        for (int s = 0; s < G::STEPS; ++s) {
+            // eight rows of the block, of which this lane loads columns of 2t and 2t + 1
+            const int row = (s * G::RW + rw) * 8, at = begin + block * BLOCK + row + 2 * t;
             float b[2][NJ];
-            if constexpr (VEC) {
-                copies_wait<GRAD_STAGES - 2>();
-                uint4 q[2][XP];
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+                const int m = at + e < end ? p.plan.order[at + e] : -1;
 #pragma unroll
-                    for (int c = 0; c < XP; ++c) q[e][c] = slot(mine + stage * STAGE + (e * XP + c) * THREADS * 16);
-                issue(rows, ahead);
-                rows[0] = row_at(i + GRAD_STAGES, 0), rows[1] = row_at(i + GRAD_STAGES, 1);
-                stage = stage + 1 == GRAD_STAGES ? 0 : stage + 1;
-                ahead = ahead + 1 == GRAD_STAGES ? 0 : ahead + 1;
-                widen_pieces<X>(q[0], b[0]);
-                widen_pieces<X>(q[1], b[1]);
-            } else {
+                for (int j = 0; j < NJ; ++j) {
+                    const int n = n0 + 32 * (j / Columns<X>::RUN) + Columns<X>::RUN * g + j % Columns<X>::RUN;
+                    b[e][j] = m >= 0 && n < p.width ? one(static_cast<const X*>(p.x) + m * p.ldx + n) : 0.f;
+                }
+            }
+            const unsigned h = shared_address(smem) + (block & 1) * G::H_BYTES + (s * G::RW + rw) * RT * 1024 + lane * 16;
+            unsigned ah[RT][4], al[RT][4];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int m = row_at(i, e);
+            for (int i = 0; i < RT; ++i) {
+                const uint4 u = slot(h + i * 1024), v = slot(h + i * 1024 + 512);
+                ah[i][0] = u.x, ah[i][1] = u.y, ah[i][2] = u.z, ah[i][3] = u.w;
+                al[i][0] = v.x, al[i][1] = v.y, al[i][2] = v.z, al[i][3] = v.w;
+            }
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        const int n = n0 + 32 * (j / Columns<X>::RUN) + Columns<X>::RUN * g + j % Columns<X>::RUN;
-                        b[e][j] = m >= 0 && n < p.width ? one(static_cast<const X*>(p.x) + m * p.ldx + n) : 0.f;
+            for (int j = 0; j < NJ; ++j) {
+                unsigned h0, h1, l0, l1;
+                parts<!is_f32<X>>(b[0][j], h0, l0);
+                parts<!is_f32<X>>(b[1][j], h1, l1);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    float s4[4] = {};   // as in down_step
+                    float(&d)[4] = is_f32<W> ? s4 : acc[i][j];
+                    mma_tf32(d, al[i], h0, h1);
+                    if (is_f32<X>) mma_tf32(d, ah[i], l0, l1);
+                    mma_tf32(d, ah[i], h0, h1);
+                    if (is_f32<W>) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] += s4[e];
                     }
                 }
             }
-            products(b, h);
         }
         put_h(block + 1 & 1);
         __syncthreads();
     }
-    if (VEC) copies_wait<0>();
     float* red = reinterpret_cast<float*>(smem);   // [RW][RANKS][COLS]; the CTA's sums end up in the first
     __syncthreads();
 #pragma unroll
@@ -981,35 +911,22 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                red[(rw * RANKS + 16 * i + g + (e & 2) * 4) * COLS + 64 * cw + 32 * (j / Columns<X>::RUN) + Columns<X>::RUN * (2 * t + (e & 1)) + j % Columns<X>::RUN] = acc[i][j][e];
+                red[(rw * RANKS + 16 * i + g + (e & 2) * 4) * COLS + 64 * cw + 32 * (j / Columns<X>::RUN) + Columns<X>::RUN * (2 * t + (e & 1)) + j % Columns<X>::RUN] =
+                    acc[i][j][e];
     __syncthreads();
-    if (shares > 1) {
-        if (RW > 1)
-            for (int i = threadIdx.x; i < RANKS * COLS; i += THREADS) {
-                float s = 0.f;
-#pragma unroll
-                for (int q = 0; q < RW; ++q) s += red[q * RANKS * COLS + i];
-                red[i] = s;   // this thread alone reads and writes element i of each
-            }
-        cluster_sync();
-    }
-    for (int i = (share * THREADS + threadIdx.x) * 8; i < RANKS * COLS; i += shares * THREADS * 8) {
+    for (int i = threadIdx.x; i < RANKS * COLS; i += THREADS) red[i] += red[RANKS * COLS + i];   // this thread alone reads and writes element i of each
+    static_assert(G::RW == 2, "two sums");
+    __syncthreads();
+    if (shares > 1) cluster_sync();
+    for (int i = (share * THREADS + threadIdx.x) * 4; i < RANKS * COLS; i += shares * THREADS * 4) {
         const int r = r0 + i / COLS, at = blockIdx.y * COLS + i % COLS;
         if (r >= p.rank || at >= p.width) continue;
-        float s[8] = {};
-        if (shares == 1) {
-#pragma unroll
-            for (int q = 0; q < RW; ++q)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] += red[q * RANKS * COLS + i + e];
-        } else {
-            for (int q = 0; q < shares; ++q) {
-                const float4 u = sums_of(red + i, q), v = sums_of(red + i + 4, q);
-                s[0] += u.x, s[1] += u.y, s[2] += u.z, s[3] += u.w;
-                s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
-            }
+        float s[4] = {};
+        for (int q = 0; q < shares; ++q) {
+            const float4 u = shares > 1 ? sums_of(red + i, q) : *reinterpret_cast<const float4*>(red + i);
+            s[0] += u.x, s[1] += u.y, s[2] += u.z, s[3] += u.w;
         }
-        store<W, 8, VEC>(static_cast<W*>(p.out) + ((long long)a * p.rank + r) * p.width + at, p.width - at, s);
+        store<W, 4>(static_cast<W*>(p.out) + ((long long)a * p.rank + r) * p.width + at, p.width - at, s);
     }
     // nobody leaves while its sums are being read
     if (shares > 1) cluster_sync();

@@ -126,21 +126,29 @@ __host__ __device__ constexpr unsigned tc_idesc(bool a_mn, bool b_mn, int n)
     return 1u << 4 | 1u << 7 | 1u << 10 | unsigned(a_mn) << 15 | unsigned(b_mn) << 16 | unsigned(n / 8) << 17 | (128u / 16) << 24;
 }
 
-// One step of 64 of the summed index, A's rows (or, mn, columns) by the PB planes of B side by side, n columns each, whose sums stay apart (columns
-// j n .. of tensor memory): so that a plane of A is read from shared memory once for all planes of B that it meets.
+// One step of 64 of the summed index, A's rows (or, mn, columns) by the PB planes of B side by side: so that a plane of A is read from shared memory once
+// for all planes of B that it meets.  The product of planes i and j goes to columns (i + j) n .. of tensor memory, SUMS of them: products of
+// one size share a sum, and the large ones' is a short chain of additions.
+template <int PA, int PB> constexpr int SUMS = PA + PB - 1 < 3 ? PA + PB - 1 : 3;
 template <int PA, int PB>
 __device__ __forceinline__ void mma_wide(unsigned d, unsigned a, bool a_mn, unsigned b, bool b_mn, int n, bool add)
 {
     const unsigned step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
     const unsigned long long db = tile_descriptor(b, b_mn, B_PLANE);
 #pragma unroll
-    for (int i = 0; i < PA; ++i) {   // the first takes all columns, and clears them
+    for (int i = 0; i < PA; ++i) {
         constexpr int ALL = PB;
         const int with = 3 - i < ALL ? 3 - i : ALL;
         const unsigned idesc = tc_idesc(a_mn, b_mn, n * with);
         const unsigned long long da = tile_descriptor(a + i * A_PLANE, a_mn, B_PLANE);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_bf16(d, da + k * step_a, db + k * step_b, idesc, add || i || k);
+        for (int k = 0; k < 4; ++k) {
+            if (k || add || i == 0 || i + PB > 3) mma_bf16(d + i * n, da + k * step_a, db + k * step_b, idesc, add || i || k);
+            else {   // the last plane's product is the first in its columns (B's rows run along the summed index)
+                if (PB > 1) mma_bf16(d + i * n, da, db, tc_idesc(a_mn, b_mn, n * (PB - 1)), true);
+                mma_bf16(d + (i + PB - 1) * n, da, db + (PB - 1) * n * (128 >> 4), tc_idesc(a_mn, b_mn, n), false);
+            }
+        }
     }
 }
 
@@ -189,11 +197,57 @@ constexpr int TC_EXTRA = 2048;   // of shared memory: the barriers, and up to th
 // Stages of `bytes` each that fit an SM, or half of one: four at most.
 __host__ __device__ constexpr int tc_stages(int bytes, int ctas) { return (225 * 1024 / ctas - TC_EXTRA) / bytes < 4 ? (225 * 1024 / ctas - TC_EXTRA) / bytes : 4; }
 
+// The tensor core cuts off what it adds: by 2^-24 of the running sum on the average, always towards zero, so that a chain of 192 additions
+// was 7 10^-6 off (4096 rows x 4096, rank 32).  Where operands are fp32, EVERY steps of 64 end a chain (two: at most 24 additions); the next goes to the other of two
+// places in tensor memory, and the NW loading warps add the finished one up, rounded: lanes are rows, and each group of four warps has
+// its share of the n columns of each of the COUNT sums.
+constexpr int TC_ONE_CHAIN = 1 << 30;
+template <int COUNT, int EVERY, int NW>
+struct Sums {
+    static constexpr int GROUPS = NW / 4, SIZE = TC_RANKS / GROUPS;
+    float f[SIZE] = {};
+    int period = 0;   // the one that is added next
+    __device__ __forceinline__ void add(TcShared& s, int n, volatile int* err)
+    {
+        const int warp = threadIdx.x >> 5, at = period & 1;
+        if (!__all_sync(0xFFFFFFFFu, bar_wait(&s.acc_full[at], period >> 1 & 1, err, TC_WAIT))) return;
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < SIZE; i += 16)
+#pragma unroll
+            for (int j = COUNT - 1; j >= 0; --j) {   // small terms first; columns from n / GROUPS on are another group's
+                int v[16];
+                __syncwarp();
+                tmem_ld(s.tmem + (unsigned(warp & 3) << 21) + at * 256 + j * n + (warp >> 2) * (n / GROUPS) + i, v);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) f[i + k] += __int_as_float(v[k]);
+            }
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) bar_arrive(&s.acc_empty[at]);
+        ++period;
+    }
+    // behind step number `step`: the chain that ended two steps ago, if one did
+    __device__ __forceinline__ void after(TcShared& s, int step, int n, volatile int* err)
+    {
+        if constexpr (EVERY < TC_ONE_CHAIN)
+            if (step % EVERY == 1 && period < step / EVERY) add(s, n, err);
+    }
+    // behind the last of `count` steps: all that are left
+    __device__ __forceinline__ void rest(TcShared& s, int count, int n, volatile int* err)
+    {
+        if constexpr (EVERY < TC_ONE_CHAIN)
+            while (period < (count + EVERY - 1) / EVERY && !*err) add(s, n, err);
+        else if (count) add(s, n, err);
+    }
+};
+
 // ---- h = x down^T: 128 rows x up to 64 ranks, the summed index shared out among a cluster's CTAs (blockIdx.y) ----
 template <class X, class W>
 struct TcDown {
     static constexpr bool PLAIN = PLANES<X> + PLANES<W> == 2;                        // nothing is cut: half the warps, and two CTAs an SM
     static constexpr int NW = PLAIN ? 8 : 16, CTAS = PLAIN ? 2 : 1, NT = 32 * NW;    // warps that load
+    static constexpr int EVERY = is_f32<X> || is_f32<W> ? 4 : TC_ONE_CHAIN, COLUMNS = EVERY < TC_ONE_CHAIN ? 512 : 256;
     static constexpr int STAGE = PLANES<X> * A_PLANE + PLANES<W> * B_PLANE, STAGES = tc_stages(STAGE, CTAS);
     static constexpr int RED = 68;   // floats a row of the sums
     static constexpr int SMEM = STAGES * STAGE + TC_EXTRA;
@@ -211,10 +265,11 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
     unsigned tiles;
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
-    tc_begin<256>(s, S::NW, 1, S::NT);
+    tc_begin<S::COLUMNS>(s, S::NW, S::NW, S::NT);
     const int t = threadIdx.x, shares = gridDim.y, r0 = blockIdx.z * TC_RANKS;
     const int ranks = min(TC_RANKS, p.rank8 - r0), n = (ranks + 15) / 16 * 16;
     const int chunks = (p.width + 63) / 64, first = int((long long)chunks * blockIdx.y / shares), last = int((long long)chunks * (blockIdx.y + 1) / shares);
+    Sums<SUMS<PLANES<X>, PLANES<W>>, S::EVERY, S::NW> sums;
     if (t < S::NT) {
         const int piece = t & 7, at = piece * 8;
         constexpr int ROWS = S::NT / 8;   // a thread's pieces are this many rows apart
@@ -253,6 +308,7 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
                 if ((t >> 3) + ROWS * i < n) put_planes<W>(b, n * 128, (t >> 3) + ROWS * i, piece, q.b[i]);
             hand_over(&s.full[stage]);
             fetch(q, c + 2);
+            sums.after(s, c - first, n, err);
             if (++stage == S::STAGES) stage = 0, phase ^= 1;
             return true;
         };
@@ -262,15 +318,19 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
             if (!step(one, c)) break;
             if (c + 1 < last && !step(two, c + 1)) break;
         }
+        sums.rest(s, last - first, n, err);
     } else if (elect_one()) {
         int stage = 0;
         unsigned phase = 0;
         for (int c = first; c < last; ++c) {
+            const int i = c - first, period = i / S::EVERY, place = period & 1;
+            if (i % S::EVERY == 0 && !bar_wait(&s.acc_empty[place], (period >> 1 & 1) ^ 1, err, TC_WAIT)) break;
             if (!bar_wait(&s.full[stage], phase, err, TC_WAIT)) break;
             tc_fence_after();
             const unsigned a = tiles + stage * S::STAGE;
-            mma_wide<PLANES<X>, PLANES<W>>(s.tmem, a, false, a + PLANES<X> * A_PLANE, false, n, c > first);
+            mma_wide<PLANES<X>, PLANES<W>>(s.tmem + place * 256, a, false, a + PLANES<X> * A_PLANE, false, n, i % S::EVERY != 0);
             tc_commit(&s.empty[stage]);
+            if ((i + 1) % S::EVERY == 0 || c + 1 == last) tc_commit(&s.acc_full[place]);
             if (++stage == S::STAGES) stage = 0, phase ^= 1;
         }
         tc_commit(&s.done);
@@ -279,21 +339,11 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
     __syncthreads();
     tc_fence_after();
     float* red = reinterpret_cast<float*>(smem + (tiles - shared_address(smem)));   // [128][RED]
-    if (t < 128) {
-        for (int c = 0; c < n; c += 16) {
-            float f[16] = {};
+    if (t < S::NT) {
+        const int row = (t >> 5 & 3) * 32 + (t & 31), mine = n / sums.GROUPS, at = (t >> 7) * mine;
 #pragma unroll
-            for (int j = PLANES<W> - 1; j >= 0; --j) {   // small terms first
-                int v[16];
-                __syncwarp();
-                tmem_ld(s.tmem + (unsigned(t & 96) << 16) + j * n + c, v);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) f[i] += __int_as_float(v[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<float4*>(red + t * S::RED + c + i) = first < last ? make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        for (int i = 0; i < sums.SIZE; i += 4)
+            if (i < mine) *reinterpret_cast<float4*>(red + row * S::RED + at + i) = make_float4(sums.f[i], sums.f[i + 1], sums.f[i + 2], sums.f[i + 3]);
     }
     tc_fence_before();
     __syncthreads();
@@ -315,7 +365,7 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
     }
     if (shares > 1) cluster_sync();   // nobody leaves while its sums are being read
     tc_fence_after();
-    tc_end<256>(s, S::NT, p.err_flag);
+    tc_end<S::COLUMNS>(s, S::NT, p.err_flag);
 }
 
 // ---- dw[a] = sum over a's rows of s h^T x: 128 columns x up to 64 ranks, the rows shared out among a cluster's CTAs (blockIdx.z) ----
@@ -335,13 +385,15 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
     unsigned tiles;
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
-    tc_begin<256>(s, S::NW, 1, S::NT);
+    tc_begin<512>(s, S::NW, S::NW, S::NT);
     const int t = threadIdx.x, shares = gridDim.z, share = blockIdx.z;
     const int blocks = (p.rank8 + TC_RANKS - 1) / TC_RANKS, a = blockIdx.x / blocks, r0 = blockIdx.x % blocks * TC_RANKS, n0 = blockIdx.y * 128;
     const int ranks = min(TC_RANKS, p.rank8 - r0), n = (ranks + 15) / 16 * 16;
     // whole steps of 64 rows for each CTA
     const int from = p.plan.offsets[a], all = p.plan.offsets[a + 1] - from, part = ((all + shares - 1) / shares + 63) / 64 * 64;
     const int begin = from + min(all, share * part), end = from + min(all, (share + 1) * part), count = (end - begin + 63) / 64;
+    constexpr int EVERY = is_f32<W> ? 4 : TC_ONE_CHAIN;
+    Sums<SUMS<PLANES<X>, 3>, EVERY, S::NW> sums;
     if (t < S::NT) {
         const float scale = p.scale ? p.scale[a] : 1.f;
         const int piece = t & 15, col = n0 + piece * 8, group = t & 7;
@@ -381,6 +433,7 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
             hand_over(&s.full[stage]);
             fetch(q);
             rows(c + 3);
+            sums.after(s, c, n, err);
             if (++stage == S::STAGES) stage = 0, phase ^= 1;
             return true;
         };
@@ -393,15 +446,19 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
             if (!step(one, c)) break;
             if (c + 1 < count && !step(two, c + 1)) break;
         }
+        sums.rest(s, count, n, err);
     } else if (elect_one()) {
         int stage = 0;
         unsigned phase = 0;
         for (int c = 0; c < count; ++c) {
+            const int period = c / EVERY, place = period & 1;
+            if (c % EVERY == 0 && !bar_wait(&s.acc_empty[place], (period >> 1 & 1) ^ 1, err, TC_WAIT)) break;
             if (!bar_wait(&s.full[stage], phase, err, TC_WAIT)) break;
             tc_fence_after();
             const unsigned x = tiles + stage * S::STAGE;
-            mma_wide<PLANES<X>, 3>(s.tmem, x, true, x + PLANES<X> * A_PLANE, true, n, c > 0);
+            mma_wide<PLANES<X>, 3>(s.tmem + place * 256, x, true, x + PLANES<X> * A_PLANE, true, n, c % EVERY != 0);
             tc_commit(&s.empty[stage]);
+            if ((c + 1) % EVERY == 0 || c + 1 == count) tc_commit(&s.acc_full[place]);
             if (++stage == S::STAGES) stage = 0, phase ^= 1;
         }
         tc_commit(&s.done);
@@ -410,20 +467,11 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
     __syncthreads();
     tc_fence_after();
     float* red = reinterpret_cast<float*>(smem + (tiles - shared_address(smem)));   // [ranks][RED]
-    if (t < 128) {
-        for (int c = 0; c < n; c += 16) {
-            float f[16] = {};
+    if (t < S::NT) {
+        const int col = (t >> 5 & 3) * 32 + (t & 31), mine = n / sums.GROUPS, at = (t >> 7) * mine;
 #pragma unroll
-            for (int j = 2; j >= 0; --j) {
-                int v[16];
-                __syncwarp();
-                tmem_ld(s.tmem + (unsigned(t & 96) << 16) + j * n + c, v);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) f[i] += __int_as_float(v[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) red[(c + i) * S::RED + t] = count > 0 ? f[i] : 0.f;
-        }
+        for (int i = 0; i < sums.SIZE; ++i)
+            if (i < mine) red[(at + i) * S::RED + col] = sums.f[i];
     }
     tc_fence_before();
     __syncthreads();
@@ -442,7 +490,7 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
     }
     if (shares > 1) cluster_sync();
     tc_fence_after();
-    tc_end<256>(s, S::NT, p.err_flag);
+    tc_end<512>(s, S::NT, p.err_flag);
 }
 
 // ---- out = base + s h up: 128 rows x 256 columns a tile, up to 64 ranks; a CTA takes a run of consecutive tiles ----

@@ -2,6 +2,7 @@
 // tensor-core kernel is in ds_loss.cuh).
 #include "ds_loss.cuh"
 
+#include <algorithm>
 #include <climits>
 
 namespace ds {
@@ -23,32 +24,46 @@ __global__ void __launch_bounds__(256) pad_kernel(const unsigned short* __restri
 
 __device__ __forceinline__ bool counted(long long t, long long ignore) { return t != ignore; }
 
-// loss and log-sum-exp of 32 rows (a lane's each); the warps share the tiles out.  The loss is log(sum) + (max - logit), so that a
-// row that is sure of its target keeps the digits that lse - logit would lose.  The CTA that is done last sums all rows up, in double and
+// loss and log-sum-exp of 32 rows (a lane's each); the warps share the parts of the vocabulary out.  The loss is log(sum) + (max - logit), so
+// that a row that is sure of its target keeps the digits that lse - logit would lose.  The CTA that is done last sums all rows up, in double and
 // in a fixed order, whichever it is.
-__global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ partial, int tiles, const float* __restrict__ at_target,
-                                                   const long long* __restrict__ target, long long ignore, int rows, int vocabulary,
-                                                   float* __restrict__ lse, float* each, int reduction, int* ticket, float* __restrict__ loss,
-                                                   float* __restrict__ count)
+constexpr int ROW_WARPS = 32;
+__global__ void __launch_bounds__(32 * ROW_WARPS) rows_kernel(const float2* __restrict__ partial, int parts, const float* __restrict__ at_target,
+                                                              const long long* __restrict__ target, long long ignore, int rows, int vocabulary,
+                                                              float* __restrict__ lse, float* each, int reduction, int* ticket, float* __restrict__ loss,
+                                                              float* __restrict__ count)
 {
-    __shared__ float2 part[8][32];
+    __shared__ float2 part[ROW_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
     float top = -INFINITY, sum = 0.f;
-    auto add = [&](float2 v) {
-        const float next = fmaxf(top, v.x), from = next == -INFINITY ? 0.f : next;
-        sum = sum * exp2_fast((top - from) * LOG2E) + v.y * exp2_fast((v.x - from) * LOG2E);
+    auto add = [&](const auto& v, int n) {   // the largest first, so that the exponentials do not wait for one another
+        float next = top;
+#pragma unroll
+        for (int i = 0; i < n; ++i) next = fmaxf(next, v[i].x);
+        const float from = next == -INFINITY ? 0.f : next;
+        sum *= exp2_fast((top - from) * LOG2E);
+#pragma unroll
+        for (int i = 0; i < n; ++i) sum += v[i].y * exp2_fast((v[i].x - from) * LOG2E);
         top = next;
     };
     if (row < rows) {
-#pragma unroll 4
-        for (int t = warp; t < tiles; t += 8) add(partial[(long long)t * rows + row]);
+        for (int t = warp; t < parts; t += 4 * ROW_WARPS) {
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = t + i * ROW_WARPS < parts ? partial[(long long)(t + i * ROW_WARPS) * rows + row] : make_float2(-INFINITY, 0.f);
+            add(v, 4);
+        }
     }
     part[warp][lane] = make_float2(top, sum);
     __syncthreads();
     if (warp == 0 && row < rows) {
         top = -INFINITY, sum = 0.f;
+        for (int w = 0; w < ROW_WARPS; w += 8) {
+            float2 v[8];
 #pragma unroll
-        for (int w = 0; w < 8; ++w) add(part[w][lane]);
+            for (int i = 0; i < 8; ++i) v[i] = part[w + i][lane];
+            add(v, 8);
+        }
         const float l = logf(sum);
         lse[row] = top + l;
         const long long t = target[row];
@@ -64,11 +79,11 @@ __global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ pa
     __syncthreads();
     if (!last) return;
     __threadfence();
-    __shared__ double sums[8];
-    __shared__ int counts[8];
+    __shared__ double sums[ROW_WARPS];
+    __shared__ int counts[ROW_WARPS];
     double s = 0.0;
     int n = 0;
-    for (int i = threadIdx.x; i < rows; i += 256) {
+    for (int i = threadIdx.x; i < rows; i += 32 * ROW_WARPS) {
         const bool c = counted(target[i], ignore);
         n += c;
         if (c) s += __ldcg(each + i);
@@ -82,7 +97,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ pa
     __syncthreads();
     if (threadIdx.x) return;
     s = 0.0, n = 0;
-    for (int i = 0; i < 8; ++i) s += sums[i], n += counts[i];
+    for (int i = 0; i < ROW_WARPS; ++i) s += sums[i], n += counts[i];
     *count = float(n);
     *loss = float(reduction == DS_LOSS_MEAN ? s / n : s);   // no row counts: 0 / 0
 }
@@ -178,12 +193,15 @@ constexpr TileShape SHAPES[3] = {{2, 256}, {1, 256}, {1, 128}};
 
 int tiles_of(const TileShape& s, int m, int n) { return (m + 128 * s.pair - 1) / (128 * s.pair) * ((n + s.bn - 1) / s.bn); }
 
-// The shape that is done first: rounds of tiles over the SMs, each as long as its k steps take (512 cycles at the tensor core's pace; a single
-// CTA's tiles are held up by shared memory, which reads and fills one of both operands twice as often) and an epilogue that the last round
-// shows.  Measured on 2048 x 1024 -> 32000, cycles a step: 530, 570, 420.
+// The shape that is done first: rounds of tiles over the SMs, each as long as its k steps take or, with few of them, its epilogue; and one more epilogue
+// that the last round shows.  A single CTA's tiles are held up by shared memory, which reads and fills one of both operands twice as often.
+// In nanoseconds, one product (z) and both of the backward pass.  Measured for z: 2048 x 1024 and x 4096 -> 32000 took 357 to 370, 406 to 423 and 249 to
+// 261 a step, 2048 x 64 and x 256 3000, 2400 and 1600 a tile; for both products, whose tiles differ in length, those that chose best.  All three shapes
+// timed at sixteen sizes from 16 x 512 -> 1000 to 2048 x 4096 -> 32000: the one chosen took at most 4% (z) and 8% longer than the best.
 int tile_shape(const Product* q, int products, int sms)
 {
-    static const int step[3] = {530, 570, 420}, tail[3] = {4000, 4000, 2500};
+    static const int steps[2][3] = {{360, 410, 255}, {360, 388, 285}}, ends[2][3] = {{3000, 2400, 1600}, {2700, 2700, 1700}};
+    const int *step = steps[products - 1], *end = ends[products - 1];
     int best = 0;
     double least = 0;
     for (int i = 0; i < 3; ++i) {
@@ -197,8 +215,7 @@ int tile_shape(const Product* q, int products, int sms)
             longest = k > longest ? k : longest;
         }
         const long long rounds = (tiles + slots - 1) / slots;
-        const double steps = products == 1 ? double(rounds) * q[0].k_steps / q[0].splits : work / slots + longest;
-        const double cost = steps * step[i] + tail[i];
+        const double cost = products == 1 ? double(rounds) * std::max<long long>(longest * step[i], end[i]) + end[i] : (work / slots + longest) * step[i] + end[i];
         if (i == 0 || cost < least) least = cost, best = i;
     }
     return best;
@@ -289,7 +306,7 @@ Layout layout(int rows, int d, int v, bool backward, bool copies)
     l.h = copy ? take((long long)rows * l.dp * 2) : -1;
     l.w = copy ? take((long long)v * l.dp * 2) : -1;
     if (!backward) {
-        l.partial = take((v + 127ll) / 128 * rows * 8);
+        l.partial = take((v + 127ll) / 128 * 2 * rows * 8);   // of the narrowest tiles
         l.at_target = take(rows * 4ll);
         l.ticket = take(4);
     } else {
@@ -369,7 +386,7 @@ extern "C" int ds_loss_forward(const ds_loss_t* a, void* stream)
         p.ticket = reinterpret_cast<int*>(scratch + l.ticket);
         const int shape = tile_shape(&q, 1, multiprocessors());
         if (const int e = launch<STATS>(maps, p, 1, shape, st)) return e;
-        rows_kernel<<<(a->rows + 31) / 32, 256, 0, st>>>(p.partial, (a->v + SHAPES[shape].bn - 1) / SHAPES[shape].bn, p.at_target, p.target, a->ignore_index,
+        rows_kernel<<<(a->rows + 31) / 32, 32 * ROW_WARPS, 0, st>>>(p.partial, (a->v + SHAPES[shape].bn - 1) / SHAPES[shape].bn * 2, p.at_target, p.target, a->ignore_index,
                                                          a->rows, a->v, a->lse, a->each, a->reduction, p.ticket, a->loss, a->count);
         ds::note_launch();
     } else if (a->reduction != DS_LOSS_NONE) {

@@ -11,7 +11,10 @@
 // Bound by the tensor cores: one kernel for the four products, persistent, a pair of CTAs (two SMs) on one tile of 256 x 256, each
 // with half of both operands in shared memory (TMA, 128-byte swizzle, six stages of 64 k) and 128 rows of fp32 sums in tensor memory,
 // twice, so that one tile's epilogue runs beside the next one's products.  Where such tiles fill the SMs badly, single CTAs take tiles of
-// 128 x 256 or 128 x 128 (tile_shape in ds_loss.cu).  Both products of the backward pass share a launch.
+// 128 x 256 or 128 x 128 (tile_shape in ds_loss.cu).  Both products of the backward pass share a launch.  Measured, bf16: 2048 x 1024 -> 32000 forward
+// 88 us, 1.53 PFLOP/s; 8192 x 4096 -> 131072 forward and backward 24.8 to 27.7 ms, 1.27 to 1.42 PFLOP/s of its 8 N V D, where a loop of plain bf16 products
+// settles at 1.41 under the power limit.  Below some 700 k the epilogue bounds a tile: 2 to 3 us, mostly latency, of which the two warps
+// that each quarter of the rows has hide half (four warps instead of eight: 2048 x 256 -> 32000 67 us instead of 55).
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -23,7 +26,9 @@ namespace ds {
 namespace loss {
 
 constexpr int BK = 64, CTA_ROWS = 128, A_BYTES = CTA_ROWS * BK * 2;
-constexpr int THREADS = 256;   // warp 0 loads, warp 1 multiplies, warps 4-7 are the epilogue: a warp reads the tensor-memory lanes of its number mod 4
+// Warp 0 loads, warp 1 multiplies, warps 4-11 are the epilogue: a warp reads the tensor-memory lanes of its number mod 4, and of its tile's columns the first
+// or the second half.
+constexpr int THREADS = 384;
 constexpr unsigned WAIT_NS = 2000000000u;
 
 // A tile of 128 PAIR x BN by PAIR CTAs; each holds 128 rows of one operand and BN / PAIR of the other.
@@ -60,7 +65,7 @@ struct Params {
     const long long* target;
     long long ignore;
     // STATS
-    float2* partial;                        // [tiles_n][m_end]: maximum, sum of exponentials
+    float2* partial;                        // [2 tiles_n][m_end]: maximum, sum of exponentials of half a tile's columns
     float* at_target;                       // logit of the target
     int* ticket;                            // zeroed for rows_kernel
     // GRAD
@@ -227,17 +232,17 @@ __device__ __forceinline__ unsigned pack2(float lo, float hi, int is_bf16)
     return *reinterpret_cast<const unsigned*>(&v);
 }
 
-// One warp's 32 rows of a finished tile; `row` is this lane's, `tmem` the address of the sums of its first column.
+// One warp's 32 rows of half the columns of a finished tile; `row` is this lane's, `tmem` the address of the sums of the tile's first column.
 template <int BN, int MODE>
-__device__ __forceinline__ void epilogue(const Params& p, const Tile& tile, unsigned tmem, int row)
+__device__ __forceinline__ void epilogue(const Params& p, const Tile& tile, int half, unsigned tmem, int row)
 {
     const Product& q = p.product[MODE == PRODUCT ? tile.which : 0];
-    const int n0 = tile.n * BN, cols = min(BN, q.n_end - n0);
+    const int n0 = tile.n * BN, cols = min(BN, q.n_end - n0), begin = half * (BN / 2), end = min(begin + BN / 2, cols);
     const bool live = row < q.m_end;
     if constexpr (MODE == STATS) {
         const long long t = live ? p.target[row] - n0 : -1;
         float top = -INFINITY, sum = 0.f;
-        for (int c = 0; c < cols; c += 32) {
+        for (int c = begin; c < end; c += 32) {
             int v[32];
             __syncwarp();
             tmem_ld(tmem + c, v);
@@ -262,7 +267,7 @@ __device__ __forceinline__ void epilogue(const Params& p, const Tile& tile, unsi
             sum += (part[0] + part[1]) + (part[2] + part[3]);
             top = next;
         }
-        if (live) p.partial[(long long)tile.n * q.m_end + row] = make_float2(top, sum);
+        if (live) p.partial[(2ll * tile.n + half) * q.m_end + row] = make_float2(top, sum);
     } else if constexpr (MODE == GRAD) {
         // p = exp(z - lse); 1 comes off at the target before the rounding to 16 bits, which is one of half a unit in the last
         // place of each element.  A weight of 0 makes the row 0 whatever its logits are.
@@ -270,8 +275,8 @@ __device__ __forceinline__ void epilogue(const Params& p, const Tile& tile, unsi
         const float lse = live ? p.lse[row] : 0.f;
         float weight = at == p.ignore ? 0.f : p.row_weight ? p.row_weight[row] : p.top;
         if (at != p.ignore && (at < 0 || at >= p.vocabulary)) weight = __int_as_float(0x7FC00000);   // no such target: not a number
-        const int width = min(BN, p.ldg - n0);
-        for (int c = 0; c < width; c += 32) {
+        const int width = min(begin + BN / 2, p.ldg - n0);
+        for (int c = begin; c < width; c += 32) {
             int v[32];
             __syncwarp();
             tmem_ld(tmem + c, v);
@@ -296,7 +301,7 @@ __device__ __forceinline__ void epilogue(const Params& p, const Tile& tile, unsi
     } else {
         const float scale = q.last ? out_scale(p) : 0.f;
         float* acc = q.acc + (long long)tile.part * q.m_end * q.n_end;
-        for (int c = 0; c < cols; c += 32) {
+        for (int c = begin; c < end; c += 32) {
             int v[32];
             __syncwarp();
             tmem_ld(tmem + c, v);
@@ -370,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(PAIR, 1, 1)
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(&s.acc_full[i], 1);
-            bar_init(&s.acc_empty[i], 4 * PAIR);
+            bar_init(&s.acc_empty[i], 8 * PAIR);
         }
         bar_init(&s.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -448,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(PAIR, 1, 1)
             const Tile t = tile_of(p, i);
             if (!__all_sync(0xFFFFFFFFu, bar_wait(&s.acc_full[buf], buf_phase, err, WAIT_NS))) break;
             tc_fence_after();
-            epilogue<BN, MODE>(p, t, tmem + buf * BN + (unsigned(quarter * 32) << 16), (t.m * PAIR + int(rank)) * CTA_ROWS + quarter * 32 + lane);
+            epilogue<BN, MODE>(p, t, (warp >> 2) - 1, tmem + buf * BN + (unsigned(quarter * 32) << 16), (t.m * PAIR + int(rank)) * CTA_ROWS + quarter * 32 + lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {

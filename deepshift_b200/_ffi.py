@@ -184,7 +184,7 @@ def run(name, device, *args):
     fn = _functions.get(name)
     if fn is None:
         fn = _functions[name] = getattr(lib(), name)
-    if torch.cuda.current_device() == device:
+    if torch._C._cuda_getDevice() == device:   # the call's tensors have initialised CUDA
         status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):

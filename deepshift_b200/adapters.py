@@ -107,7 +107,8 @@ def _check(x, down, up, scale, plan):
     return count, rank, k, n, act, weight, device
 
 
-def _forward(x, down, up, scale, plan, base, out):
+def _forward(x, down, up, scale, plan, base, out, keep):
+    """The result, and h where the backward pass wants it (``keep``) or the library needs the place."""
     count, rank, k, n, act, weight, device = _check(x, down, up, scale, plan)
     rows = _rows(x, "x", k, x.dtype, device)
     m = plan.rows
@@ -130,18 +131,21 @@ def _forward(x, down, up, scale, plan, base, out):
         base_at, base_stride = add.data_ptr(), add.stride(0)
         if base_at == to.data_ptr() and base_stride != to_stride:
             raise RuntimeError("base and out overlap")
-    nbytes = 4 * m * ((rank + 7) // 8 * 8)   # ds_adapters_h_bytes
-    h = x.new_empty(nbytes // 4, dtype=torch.float32)
+    h, h_at, nbytes = None, 0, 0
+    if keep or m > 512 or rank > 64:
+        nbytes = 4 * m * ((rank + 7) // 8 * 8)   # ds_adapters_h_bytes
+        h = x.new_empty(nbytes // 4, dtype=torch.float32)
+        h_at = h.data_ptr()
     _ffi.run("ds_adapters_apply", device, _ffi.pack_adapters(
         m, k, n, rank, count, act, weight, plan.data.data_ptr(), down.data_ptr(), up.data_ptr(), scale.data_ptr() if scale is not None else 0,
-        rows.data_ptr(), rows.stride(0), base_at, base_stride, to.data_ptr(), to_stride, h.data_ptr(), nbytes, 0, 0, 0, 0, 0, 0, 0, 0))
+        rows.data_ptr(), rows.stride(0), base_at, base_stride, to.data_ptr(), to_stride, h_at, nbytes, 0, 0, 0, 0, 0, 0, 0, 0))
     return out, h
 
 
 class _Apply(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, down, up, scale, plan, base):
-        out, h = _forward(x, down, up, scale, plan, base, None)
+        out, h = _forward(x, down, up, scale, plan, base, None, True)
         ctx.save_for_backward(x, down, up, scale, h)
         ctx.plan = plan
         return out
@@ -184,7 +188,7 @@ def apply(x, down, up, scale, plan, base=None, out=None):
         if out is not None:
             raise RuntimeError("out= cannot be differentiated")
         return _Apply.apply(x, down, up, scale, plan, base)
-    return _forward(x, down, up, scale, plan, base, out)[0]
+    return _forward(x, down, up, scale, plan, base, out, False)[0]
 
 
 class AdaptedLinear(nn.Module):

@@ -305,11 +305,14 @@ int launch_both(const Args& d, const Args& u, cudaStream_t st)
     return launch_cluster<both_kernel<X, W, NT, VEC>>(dim3(unsigned(tiles), shares), dim3(1, shares, 1), THREADS, smem, st, d, u);
 }
 
-// h = x down^T and out = base + s h up.  One launch for up to 512 rows, whose tiles are of 16 rows, and up to 64 ranks; two otherwise.
+// One launch does both projections of up to 512 rows, whose tiles are of 16 rows, and up to 64 ranks.
+bool one_launch(int rows, int rank) { return plan_tile_rows(rows) == 16 && rank <= 64; }
+
+// h = x down^T and out = base + s h up.
 template <class X, class W>
 int both(const Args& d, bool vec_d, const Args& u, bool vec_u, cudaStream_t st)
 {
-    if (plan_tile_rows(d.rows) == 16 && d.rank8 <= 64) {
+    if (one_launch(d.rows, d.rank)) {
         const bool vec = vec_d && vec_u;
         if (!vec) return d.rank8 <= 8 ? launch_both<X, W, 1, false>(d, u, st) : launch_both<X, W, 8, false>(d, u, st);
         if (d.rank8 <= 8) return launch_both<X, W, 1, true>(d, u, st);
@@ -347,13 +350,14 @@ int check(const ds_adapters_t* a, bool backward)
     if (a->rank > MAX_RANK || a->count > 65535) return DS_ERR_UNSUPPORTED;
     if (a->rows > 1 << 24 || a->k > 1 << 20 || a->n > 1 << 20) return DS_ERR_RANGE;
     if (!a->plan || !a->down || !a->up) return DS_ERR_BAD_ARG;
-    if (a->rows && (!a->x || !a->h)) return DS_ERR_BAD_ARG;
+    const bool without = !backward && !a->h && one_launch(a->rows, a->rank);   // h stays on the chip
+    if (a->rows && (!a->x || (!a->h && !without))) return DS_ERR_BAD_ARG;
     if (backward ? (a->rows && (!a->grad || !a->dh)) : (a->rows && !a->out)) return DS_ERR_BAD_ARG;
     if (!kernel_error_flag()) return DS_ERR_CUDA;
     if (reinterpret_cast<uintptr_t>(a->plan) & 15 || reinterpret_cast<uintptr_t>(a->h) & 15 || reinterpret_cast<uintptr_t>(a->dh) & 15)
         return DS_ERR_ALIGN;
     const long long need = ds_adapters_h_bytes(a->rows, a->rank);
-    if (a->h_bytes < need || (backward && a->dh_bytes < need)) return DS_ERR_SCRATCH;
+    if ((a->h_bytes < need && !without) || (backward && a->dh_bytes < need)) return DS_ERR_SCRATCH;
     return DS_OK;
 }
 

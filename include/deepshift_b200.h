@@ -460,7 +460,8 @@ typedef struct {
     long long base_stride;
     void *out;                         /* [rows][n]                                                        */
     long long out_stride;
-    float *h;                          /* ds_adapters_h_bytes: written by _apply, read by _backward */
+    float *h;                          /* ds_adapters_h_bytes: written by _apply, read by _backward; NULL for
+                                        * _apply alone on up to 512 rows with a rank of up to 64           */
     long long h_bytes;
     const void *grad;                  /* _backward only: gradient of out [rows][n]                        */
     long long grad_stride;

@@ -53,7 +53,7 @@ def test_entry_points_check_their_arguments_first():
     fields = [f for f, _ in _ffi.Adapters._fields_]
     good = dict.fromkeys(fields, 0)
     good.update(rows=4, k=8, n=8, rank=4, count=2, plan=16, down=16, up=16, x=16, x_stride=8, out=16, out_stride=8, h=16, h_bytes=4 * 8 * 4)
-    for bad in (dict(rows=-1), dict(k=0), dict(n=0), dict(rank=0), dict(count=0), dict(plan=0), dict(down=0), dict(up=0), dict(x=0), dict(h=0), dict(out=0),
+    for bad in (dict(rows=-1), dict(k=0), dict(n=0), dict(rank=0), dict(count=0), dict(plan=0), dict(down=0), dict(up=0), dict(x=0), dict(h=0, rank=65, h_bytes=1 << 20), dict(out=0),
                 dict(rank=257), dict(count=65536), dict(rows=(1 << 24) + 1), dict(k=(1 << 20) + 1), dict(n=(1 << 20) + 1)):
         assert lib.ds_adapters_apply(_ffi.pack_adapters(*{**good, **bad}.values()), None) != 0, bad
         assert lib.ds_adapters_backward(_ffi.pack_adapters(*{**good, **bad}.values()), None) != 0, bad

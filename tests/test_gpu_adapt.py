@@ -44,3 +44,27 @@ def test_rows_answer_alone_as_in_a_batch(cuda_device):
     alone = torch.cat([adapt.serve(model, tokens[i:i + 1], ids[i:i + 1], 3) for i in range(40)])
     # hidden states are rounded to bfloat16 (2^-9) before the head: a logit of a few units may move by some 2^-9 of itself
     assert torch.allclose(together, alone, rtol=0.05, atol=0)
+
+
+@pytest.mark.parametrize("rows, rank", [(1, 1), (17, 8), (512, 64)])
+def test_products_without_keeping_the_inner_ones(cuda_device, rows, rank):
+    """Up to 512 rows and a rank of 64 need no place for h; the result is the one with it, bit for bit."""
+    import torch
+    from deepshift_b200 import _ffi, adapters
+    torch.manual_seed(rows)
+    x, down, up, base = (torch.randn(s, device="cuda") for s in ((rows, 100), (3, rank, 100), (3, rank, 72), (rows, 72)))
+    plan = adapters.plan_rows(torch.arange(rows) % 4 - 1, 3)
+    with torch.no_grad():
+        without = adapters.apply(x, down, up, None, plan, base=base)
+    kept = adapters.apply(x, down.requires_grad_(True), up, None, plan, base=base)
+    assert kept.requires_grad and torch.equal(without, kept)
+    # more of either have to bring it
+    for m, r in ((513, 8), (16, 65)):
+        more = (torch.randn(s, device="cuda") for s in ((m, 100), (3, r, 100), (3, r, 72)))
+        x, down, up = more
+        plan = adapters.plan_rows(torch.arange(m) % 4 - 1, 3)
+        out = torch.empty(m, 72, device="cuda")
+        with pytest.raises(RuntimeError, match="bad argument"):
+            _ffi.run("ds_adapters_apply", x.get_device(), _ffi.pack_adapters(
+                m, 100, 72, r, 3, 0, 0, plan.data.data_ptr(), down.data_ptr(), up.data_ptr(), 0, x.data_ptr(), 100, 0, 0, out.data_ptr(), 72,
+                0, 0, 0, 0, 0, 0, 0, 0, 0, 0))

@@ -738,7 +738,8 @@ __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 
 // Few rows: both projections of a tile of 16 in one launch (`d`: the down projection's operands, `u`: the up projection's).  The CTAs of
 // a cluster share the summed index out, each adds all their sums up over distributed shared memory, and takes every
-// gridDim.y-th 64 columns of the result, whose part of w and base are fetched while the sums are being formed.
+// gridDim.y-th 64 columns of the result, whose part of w and base are fetched while the sums are being formed.  Bound by that chain of dependent
+// loads, not by bytes: 1 x 512 -> 512 of rank 8 takes 6.2 us, 64 x 4096 -> 4096 of rank 16, 64 adapters, 14.4 (20 MB).
 template <class X, class W, int NT, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Args u)
 {
@@ -812,7 +813,7 @@ constexpr int both_smem(bool vec) { return Down<X, W, 1, NT, BOTH_BUDGET>::smem(
 // dw[a][r0 .. r0 + 32)[n0 .. n0 + 256) over all rows of adapter a, at odd widths or addresses (aligned ones go to tc_grad_kernel).  Four warps side
 // by side, two above one another, share a block of 32 rows whose h, scaled and split, lies in shared memory in the order in which the
 // instructions read it; the next block's is on its way meanwhile.  The `gridDim.z` CTAs of a cluster take one part of the rows each and
-// add up their sums over distributed shared memory, in their order.
+// add up their sums over distributed shared memory, in their order.  Bound by instructions: unaligned elements come one by one.
 struct Grad {
     static constexpr int RT = 2, RANKS = 16 * RT, CW = 4, COLS = 64 * CW, RW = WARPS / CW, BLOCK = 32, STEPS = BLOCK / 8 / RW;
     static constexpr int H_BYTES = BLOCK * RANKS * 8, SUMS = RW * RANKS * COLS * 4, SMEM = SUMS > 2 * H_BYTES ? SUMS : 2 * H_BYTES;

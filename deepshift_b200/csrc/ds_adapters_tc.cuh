@@ -7,8 +7,9 @@
 // what is left), fp16 two, bf16 one; a product is the sum over pairs of planes whose numbers add up to at most two, which leaves out
 // 2^-24 of it.  Which of an operand's dimensions lies along the rows is a matter of its descriptor alone.
 //
-// Bound by memory: activations pass once, the adapters' matrices come from L2.  With mma.sync, whose fp32 takes three TF32 products
-// at an eighth of this rate, the three kernels took 36, 57 and 55 us where these take 19, 31 and 26 (4096 x 4096 -> 4096 in fp32, rank 32).
+// Activations pass once, the adapters' matrices come from L2.  Measured from a cold L2 (each kernel alone): fp32, 4096 x 4096, rank 32, four adapters: down 32 us,
+// up 36 (44 with base), gradient 33, 2 to 3 TB/s; bf16, 8192 x 2048, rank 64, twelve adapters: down 23, up with base 31.5.  What bounds them is what a
+// CTA has on its way: two steps of 64 in registers (a third spilled), and in fp32 the cutting.
 #pragma once
 #include "ds_adapters.cuh"
 #include "ds_tc_ptx.cuh"

@@ -146,7 +146,7 @@ __device__ __forceinline__ double cta_sum(double v)
 // Squares are added up in fp32 by eights (two pieces of fp32, one of 16 bits), which rounds each sum by some 1e-7 of itself at
 // random, and the sums in double: one conversion for eight values, where one for each took twice as long as the reading.
 // Where a sum leaves the range that fp32 can hold (values beyond 1e18, or all so small that their squares vanish) the warp squares in
-// double instead, save for pieces that are 0 altogether.
+// double instead, save for pieces that are 0 altogether.  1 G of bf16 in 306 us: 7.0 TB/s.
 template <int CAP, int U>
 __global__ void __launch_bounds__(CLIP_THREADS, 4) norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* __restrict__ partial)
 {
@@ -216,7 +216,7 @@ __device__ __forceinline__ float total_norm(const double* __restrict__ partial, 
 
 // A chunk is `steps` steps of U pieces a thread.  ALIGNED: every place and source is 16-byte aligned, and eight pieces are on their way; four elsewhere,
 // where each takes two loads and what puts them together (one kernel for both, with eight, spilled: 700 instead of 755 us for 1 G aligned
-// bf16 values, but 71 instead of 47 for 40 M of two types at any alignment).
+// bf16 values, but 71 instead of 47 for 40 M of two types at any alignment).  700 us are 6.1 TB/s, read and written.
 template <int CAP, bool ALIGNED>
 __global__ void __launch_bounds__(CLIP_THREADS, 3) scale_kernel(const __grid_constant__ ClipTable<CAP> t, int steps, const double* __restrict__ partial,
                                                                 int partials, float max_norm, float* __restrict__ norm)

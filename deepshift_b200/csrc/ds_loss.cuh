@@ -12,7 +12,7 @@
 // with half of both operands in shared memory (TMA, 128-byte swizzle, six stages of 64 k) and 128 rows of fp32 sums in tensor memory,
 // twice, so that one tile's epilogue runs beside the next one's products.  Where such tiles fill the SMs badly, single CTAs take tiles of
 // 128 x 256 or 128 x 128 (tile_shape in ds_loss.cu).  Both products of the backward pass share a launch.  Measured, bf16: 2048 x 1024 -> 32000 forward
-// 88 us, 1.53 PFLOP/s; 8192 x 4096 -> 131072 forward and backward 24.8 to 27.7 ms, 1.27 to 1.42 PFLOP/s of its 8 N V D, where a loop of plain bf16 products
+// 88 us, 1.53 PFLOP/s; 8192 x 4096 -> 131072 forward and backward 24.8 to 29.6 ms, 1.19 to 1.42 PFLOP/s of its 8 N V D, where a loop of plain bf16 products
 // settles at 1.41 under the power limit.  Below some 700 k the epilogue bounds a tile: 2 to 3 us, mostly latency, of which the two warps
 // that each quarter of the rows has hide half (four warps instead of eight: 2048 x 256 -> 32000 67 us instead of 55).
 #pragma once

@@ -155,21 +155,11 @@ bool allow_smem(int bytes)
     return true;
 }
 
+// Both kinds of launches; a call's first waits for all earlier work, the others follow.
 template <auto KERNEL, class... A>
-int launch_cluster(dim3 grid, dim3 cluster, int threads, int smem, cudaStream_t st, const A&... a)
+int launch_kernel(dim3 grid, dim3 cluster, int threads, int smem, cudaStream_t st, bool follows, const A&... a)
 {
-    cudaLaunchConfig_t c = {};
-    c.gridDim = grid;
-    c.blockDim = dim3(threads);
-    c.dynamicSmemBytes = smem;
-    c.stream = st;
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim = {cluster.x, cluster.y, cluster.z};
-    c.attrs = &attribute;
-    c.numAttrs = 1;
-    if (cudaLaunchKernelEx(&c, KERNEL, a...) != cudaSuccess) return DS_ERR_CUDA;
-    return finish();
+    return ds::launch(KERNEL, grid, cluster, unsigned(threads), smem, st, follows, a...) ? finish() : DS_ERR_CUDA;
 }
 
 // Projections of many aligned rows go to the tensor cores' kernels in tiles of 128 (ds_adapters_tc.cuh); those of up to 512 rows, at odd widths or
@@ -190,7 +180,7 @@ int launch_down(const Args& a, cudaStream_t st)
     const long long ctas = (a.rows / 16 + 1ll) * blocks, steps = (a.width + chunk - 1) / chunk;
     int shares = 1;
     while (shares < 8 && ctas * shares * 2 <= 296 && steps >= 2 * shares * WARPS) shares *= 2;
-    return launch_cluster<down_kernel<X, W, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks * parts), dim3(1, shares, 1), THREADS, smem, st, a,
+    return launch_kernel<down_kernel<X, W, NT, VEC>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks * parts), dim3(1, shares, 1), THREADS, smem, st, false, a,
                                                       parts);
 }
 
@@ -205,7 +195,7 @@ int launch_tc_down(const Args& a, cudaStream_t st)
     const long long tiles = plan_tiles(a.rows, a.count) * blocks;
     int shares = 1;
     while (shares < 8 && tiles * shares * 2 <= 148 * S::CTAS && chunks >= 2 * shares * 4) shares *= 2;
-    return launch_cluster<tc_down_kernel<X, W>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), S::NT + 32, S::SMEM, st, a);
+    return launch_kernel<tc_down_kernel<X, W>>(dim3(unsigned(plan_tiles(a.rows, a.count)), shares, blocks), dim3(1, shares, 1), S::NT + 32, S::SMEM, st, false, a);
 }
 
 // Ranks by 64 where both operands are of one 16-bit type and go to the tensor core as they are; by 32 elsewhere.
@@ -229,8 +219,7 @@ int launch_up(const Args& a, cudaStream_t st)
     const int smem = a.rank8 * 16 * 8 + rows;
     if (!allow_smem<up_kernel<X, W, VEC>>(MAX_RANK * 16 * 8 + rows)) return DS_ERR_CUDA;
     const dim3 grid(unsigned(plan_tiles(a.rows, a.count)), (a.width + 64 * WARPS - 1) / (64 * WARPS), plan_tile_rows(a.rows) / 16);
-    up_kernel<X, W, VEC><<<grid, THREADS, smem, st>>>(a);
-    return finish();
+    return launch_kernel<up_kernel<X, W, VEC>>(grid, dim3(0), THREADS, smem, st, true, a);
 }
 
 template <class X, class W, int NB>
@@ -244,8 +233,7 @@ int launch_tc_up(const Args& a, cudaStream_t st)
     const long long tiles = plan_tiles(a.rows, a.count);
     long long runs = 148 / columns;   // one round
     runs = runs < 1 ? 1 : runs > tiles ? tiles : runs;
-    tc_up_kernel<X, W, NB><<<dim3(unsigned(runs), columns), S::ALL, S::smem((a.rank8 + 15) / 16 * 16), st>>>(a);
-    return finish();
+    return launch_kernel<tc_up_kernel<X, W, NB>>(dim3(unsigned(runs), columns), dim3(0), S::ALL, S::smem((a.rank8 + 15) / 16 * 16), st, true, a);
 }
 
 template <class X, class W>
@@ -260,7 +248,7 @@ int up(const Args& a, bool vec, cudaStream_t st)
 }
 
 template <class X, class W>
-int launch_grad(const Args& a, cudaStream_t st)
+int launch_grad(const Args& a, bool follows, cudaStream_t st)
 {
     using G = Grad;
     if (!allow_smem<grad_kernel<X, W>>(G::SMEM)) return DS_ERR_CUDA;
@@ -269,11 +257,11 @@ int launch_grad(const Args& a, cudaStream_t st)
     // rows spread evenly
     int shares = 1;
     while (shares < 8 && (long long)columns * a.count * blocks * shares < 296 && a.rows / a.count >= 2 * shares * 2 * G::BLOCK) shares *= 2;
-    return launch_cluster<grad_kernel<X, W>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), THREADS, G::SMEM, st, a);
+    return launch_kernel<grad_kernel<X, W>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), THREADS, G::SMEM, st, follows, a);
 }
 
 template <class X, class W>
-int launch_tc_grad(const Args& a, cudaStream_t st)
+int launch_tc_grad(const Args& a, bool follows, cudaStream_t st)
 {
     using S = TcGrad<X>;
     static_assert(S::STAGES >= 2 && TC_RANKS * S::RED * 4 <= S::STAGES * S::STAGE, "stages of a CTA");
@@ -282,14 +270,14 @@ int launch_tc_grad(const Args& a, cudaStream_t st)
     // CTAs that share an adapter's rows: until each SM has one, as long as each has four steps, were the rows spread evenly
     int shares = 1;
     while (shares < 8 && (long long)columns * a.count * blocks * shares * 2 <= 148 && a.rows / a.count >= 2 * shares * 4 * 64) shares *= 2;
-    return launch_cluster<tc_grad_kernel<X, W>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), S::NT + 32, S::SMEM, st, a);
+    return launch_kernel<tc_grad_kernel<X, W>>(dim3(a.count * blocks, columns, shares), dim3(1, 1, shares), S::NT + 32, S::SMEM, st, follows, a);
 }
 
 // Aligned ones on the tensor cores whatever their number of rows: 520 x 1024 of rank 16 in fp32 10.3 us against mma.sync's 17.5, 4096 x 4096 22 against 61.
 template <class X, class W>
-int grad(const Args& a, bool vec, cudaStream_t st)
+int grad(const Args& a, bool vec, bool follows, cudaStream_t st)
 {
-    return vec ? launch_tc_grad<X, W>(a, st) : launch_grad<X, W>(a, st);
+    return vec ? launch_tc_grad<X, W>(a, follows, st) : launch_grad<X, W>(a, follows, st);
 }
 
 template <class X, class W, int NT, bool VEC>
@@ -303,7 +291,7 @@ int launch_both(const Args& d, const Args& u, cudaStream_t st)
     const long long tiles = plan_tiles(d.rows, d.count);
     int shares = 1;
     while (shares < 8 && tiles * shares * 2 <= 296 && shares < (steps > columns ? steps : columns)) shares *= 2;
-    return launch_cluster<both_kernel<X, W, NT, VEC>>(dim3(unsigned(tiles), shares), dim3(1, shares, 1), THREADS, smem, st, d, u);
+    return launch_kernel<both_kernel<X, W, NT, VEC>>(dim3(unsigned(tiles), shares), dim3(1, shares, 1), THREADS, smem, st, false, d, u);
 }
 
 // One launch does both projections of up to 512 rows, whose tiles are of 16 rows, and up to 64 ranks.
@@ -449,12 +437,12 @@ extern "C" int ds_adapters_backward(const ds_adapters_t* a, void* stream)
         if (a->ddown) {
             Args p = dh;
             p.x = a->x, p.ldx = a->x_stride, p.width = a->k, p.out = a->ddown;
-            if (const int e = grad<X, W>(p, vec_k && aligned(a->ddown, a->k, a->weight_type), st)) return e;
+            if (const int e = grad<X, W>(p, vec_k && aligned(a->ddown, a->k, a->weight_type), a->rows > 0, st)) return e;
         }
         if (a->dup) {
             Args p = down_args(a, a->grad, a->grad_stride, nullptr, a->n, a->h);   // the forward's h
             p.out = a->dup;
-            if (const int e = grad<X, W>(p, vec_n && aligned(a->dup, a->n, a->weight_type), st)) return e;
+            if (const int e = grad<X, W>(p, vec_n && aligned(a->dup, a->n, a->weight_type), a->dx || a->ddown, st)) return e;
         }
         return int(DS_OK);
     });

@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include "ds_common.cuh"
+#include "ds_follow.cuh"
 
 namespace ds {
 namespace adapters {
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(THREADS, 2) down_kernel(const Args p, int part
 {
     constexpr int COLS = 8 * NT;
     extern __shared__ __align__(16) unsigned char smem[];
+    let_follow();
     if (int(blockIdx.x) >= p.plan.head[0]) return;
     const int4 tile = sixteen(p.plan.tiles[blockIdx.x], blockIdx.z % parts);
     if (tile.x >= p.count || tile.z <= 0) return;   // rows without an adapter: nothing reads their h
@@ -709,6 +711,8 @@ template <class X, class W, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) up_kernel(const Args p)
 {
     extern __shared__ __align__(16) unsigned char smem[];
+    let_follow();
+    wait_before();
     if (int(blockIdx.x) >= p.plan.head[0]) return;
     const int4 tile = sixteen(p.plan.tiles[blockIdx.x], blockIdx.z);
     const bool none = tile.x >= p.count;
@@ -745,6 +749,7 @@ __global__ void __launch_bounds__(THREADS, 2) both_kernel(const Args d, const Ar
 {
     constexpr int COLS = 8 * NT, SUMS = Down<X, W, 1, NT, BOTH_BUDGET>::smem(VEC);
     extern __shared__ __align__(16) unsigned char smem[];   // queue and sums, h, base or stage
+    let_follow();
     if (int(blockIdx.x) >= d.plan.head[0]) return;
     const int4 tile = d.plan.tiles[blockIdx.x];
     const bool none = tile.x >= d.count;
@@ -825,6 +830,8 @@ __global__ void __launch_bounds__(THREADS, 2) grad_kernel(const Args p)
     using G = Grad;
     constexpr int NJ = 8, RT = G::RT, RANKS = G::RANKS, COLS = G::COLS, BLOCK = G::BLOCK;
     extern __shared__ __align__(16) unsigned char smem[];   // h of two blocks; at the end the sums
+    let_follow();
+    wait_before();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, cw = warp % G::CW, rw = warp / G::CW;
     const int blocks = (p.rank + RANKS - 1) / RANKS;
     const int a = blockIdx.x / blocks, n0 = blockIdx.y * COLS + 64 * cw, r0 = blockIdx.x % blocks * RANKS;

@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(TcDown<X, W>::NT + 32, TcDown<X, W>::CTAS) tc_
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
     tc_begin<S::COLUMNS>(s, S::NW, S::NW, S::NT);
+    let_follow();
     const int t = threadIdx.x, shares = gridDim.y, r0 = blockIdx.z * TC_RANKS;
     const int ranks = min(TC_RANKS, p.rank8 - r0), n = (ranks + 15) / 16 * 16;
     const int chunks = (p.width + 63) / 64, first = int((long long)chunks * blockIdx.y / shares), last = int((long long)chunks * (blockIdx.y + 1) / shares);
@@ -387,6 +388,8 @@ __global__ void __launch_bounds__(TcGrad<X>::NT + 32, 1) tc_grad_kernel(const Ar
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
     tc_begin<512>(s, S::NW, S::NW, S::NT);
+    let_follow();
+    wait_before();
     const int t = threadIdx.x, shares = gridDim.z, share = blockIdx.z;
     const int blocks = (p.rank8 + TC_RANKS - 1) / TC_RANKS, a = blockIdx.x / blocks, r0 = blockIdx.x % blocks * TC_RANKS, n0 = blockIdx.y * 128;
     const int ranks = min(TC_RANKS, p.rank8 - r0), n = (ranks + 15) / 16 * 16;
@@ -515,11 +518,15 @@ __global__ void __launch_bounds__(TcUp<X, W, NB>::ALL, 1) tc_up_kernel(const Arg
     using S = TcUp<X, W, NB>;
     extern __shared__ __align__(16) unsigned char smem[];
     const int total = p.plan.head[0], first = int((long long)total * blockIdx.x / gridDim.x), last = int((long long)total * (blockIdx.x + 1) / gridDim.x);
-    if (first == last) return;
+    if (first == last) {   // what follows this kernel takes it to have waited
+        wait_before();
+        return;
+    }
     unsigned tiles;
     TcShared& s = tc_shared(smem, tiles);
     volatile int* err = &s.err;
     tc_begin<512>(s, S::CUT, S::NW, S::ALL - 32);
+    let_follow();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n0 = blockIdx.y * S::COLS;
     const int k16 = (p.rank8 + 15) / 16 * 16;
     const unsigned h_at = tiles, w_at = tiles + S::H;
@@ -546,6 +553,7 @@ __global__ void __launch_bounds__(TcUp<X, W, NB>::ALL, 1) tc_up_kernel(const Arg
         stage_w(first_adapter, t, S::ALL);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    wait_before();   // for h; w was there before the call
     __syncthreads();
     if (t < S::NT) {
         const int quarter = warp & 3, c0 = n0 + (warp >> 2) * 128;   // a warp's 32 rows and 128 columns

@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include "ds_common.cuh"
+#include "ds_follow.cuh"
 
 namespace ds {
 namespace {
@@ -150,6 +151,7 @@ __device__ __forceinline__ double cta_sum(double v)
 template <int CAP, int U>
 __global__ void __launch_bounds__(CLIP_THREADS, 4) norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* __restrict__ partial)
 {
+    let_follow();
     double acc = 0.0;
     for (int chunk = blockIdx.x; chunk < t.first[t.count]; chunk += gridDim.x) {
         const int i = tensor_of(t, chunk);
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(CLIP_THREADS, 4) norm_kernel(const __grid_cons
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
-__device__ __forceinline__ float total_norm(const double* __restrict__ partial, int partials)
+__device__ __forceinline__ float total_norm(const double* partial, int partials)
 {
     double s = 0.0;
     for (int i = threadIdx.x; i < partials; i += CLIP_THREADS) s += partial[i];
@@ -218,10 +220,12 @@ __device__ __forceinline__ float total_norm(const double* __restrict__ partial, 
 // where each takes two loads and what puts them together (one kernel for both, with eight, spilled: 700 instead of 755 us for 1 G aligned
 // bf16 values, but 71 instead of 47 for 40 M of two types at any alignment).  700 us are 6.1 TB/s, read and written.
 template <int CAP, bool ALIGNED>
-__global__ void __launch_bounds__(CLIP_THREADS, 3) scale_kernel(const __grid_constant__ ClipTable<CAP> t, int steps, const double* __restrict__ partial,
+__global__ void __launch_bounds__(CLIP_THREADS, 3) scale_kernel(const __grid_constant__ ClipTable<CAP> t, int steps, const double* partial,
                                                                 int partials, float max_norm, float* __restrict__ norm)
 {
     constexpr int U = ALIGNED ? 8 : 4;
+    let_follow();
+    wait_before();
     const float all = total_norm(partial, partials);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = all;
     float f = max_norm / (all + 1e-6f);
@@ -280,7 +284,7 @@ __global__ void __launch_bounds__(CLIP_THREADS, 3) scale_kernel(const __grid_con
     }
 }
 
-__global__ void __launch_bounds__(CLIP_THREADS) norm_only_kernel(const double* __restrict__ partial, int partials, float* __restrict__ norm)
+__global__ void __launch_bounds__(CLIP_THREADS) norm_only_kernel(const double* partial, int partials, float* __restrict__ norm)
 {
     const float all = total_norm(partial, partials);
     if (threadIdx.x == 0) *norm = all;
@@ -330,7 +334,9 @@ int run(const ds_tensor_t* tensors, int count, int steps, bool aligned, float ma
     for (int at = 0; scale && at < count; at += CAP) {
         if (count > CAP) chunks = fill(t, tensors + at, count - at < CAP ? count - at : CAP, steps, steps * U * CLIP_STEP);
         if (!chunks) continue;
-        (aligned ? scale_kernel<CAP, true> : scale_kernel<CAP, false>)<<<ctas(chunks), CLIP_THREADS, 0, st>>>(t, steps * U / (aligned ? 8 : 4), partial, partials, max_norm, written ? nullptr : norm);
+        if (!launch(aligned ? scale_kernel<CAP, true> : scale_kernel<CAP, false>, dim3(ctas(chunks)), dim3(0), CLIP_THREADS, 0, st, true, t, steps * U / (aligned ? 8 : 4),
+                    partial, partials, max_norm, written ? nullptr : norm))
+            return DS_ERR_CUDA;
         note_launch();
         written = true;
     }

@@ -1,0 +1,34 @@
+// Launches of one call that follow one another closely: a kernel that is launched as a follower may start while the one before it still runs, as soon
+// as each of that one's CTAs has called let_follow or ended, and itself calls wait_before, in every thread that goes on and in every CTA, before
+// it touches memory that a kernel writes or that it writes itself.  Only kernels of the same call follow one another this way: the first waits for
+// all earlier work as usual, so what was there before the call (operands, plans) may be read ahead of wait_before.
+// A kernel that takes tensor memory calls let_follow behind its allocation: a follower that held it could otherwise keep it waiting.
+// Worth 2 to 4 us a launch: what it takes to start a grid once the last one has drained.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace ds {
+
+__device__ __forceinline__ void let_follow() { cudaTriggerProgrammaticLaunchCompletion(); }
+__device__ __forceinline__ void wait_before() { cudaGridDependencySynchronize(); }
+
+// Launches `kernel`, in clusters of `cluster` CTAs where that has a size.  False: refused.
+template <class... P, class... A>
+bool launch(void (*kernel)(P...), dim3 grid, dim3 cluster, unsigned threads, size_t smem, cudaStream_t st, bool follows, const A&... a)
+{
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = st;
+    cudaLaunchAttribute attribute[2];
+    c.attrs = attribute;
+    if (cluster.x * cluster.y * cluster.z > 0) {
+        attribute[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attribute[c.numAttrs++].val.clusterDim = {cluster.x, cluster.y, cluster.z};
+    }
+    if (follows) {
+        attribute[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute[c.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    return cudaLaunchKernelEx(&c, kernel, P(a)...) == cudaSuccess;
+}
+
+}  // namespace ds

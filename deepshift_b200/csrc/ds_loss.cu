@@ -28,13 +28,14 @@ __device__ __forceinline__ bool counted(long long t, long long ignore) { return 
 // that a row that is sure of its target keeps the digits that lse - logit would lose.  The CTA that is done last sums all rows up, in double and
 // in a fixed order, whichever it is.
 constexpr int ROW_WARPS = 32;
-__global__ void __launch_bounds__(32 * ROW_WARPS) rows_kernel(const float2* __restrict__ partial, int parts, const float* __restrict__ at_target,
+__global__ void __launch_bounds__(32 * ROW_WARPS) rows_kernel(const float2* partial, int parts, const float* at_target,
                                                               const long long* __restrict__ target, long long ignore, int rows, int vocabulary,
                                                               float* __restrict__ lse, float* each, int reduction, int* ticket, float* __restrict__ loss,
                                                               float* __restrict__ count)
 {
     __shared__ float2 part[ROW_WARPS][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+    wait_before();
     float top = -INFINITY, sum = 0.f;
     auto add = [&](const auto& v, int n) {   // the largest first, so that the exponentials do not wait for one another
         float next = top;
@@ -222,7 +223,7 @@ int tile_shape(const Product* q, int products, int sms)
 }
 
 template <int PAIR, int BN, int MODE>
-int launch_shape(const Maps& maps, Params& p, int tiles, int sms, cudaStream_t st)
+int launch_shape(const Maps& maps, Params& p, int tiles, int sms, bool follows, cudaStream_t st)
 {
     static bool done[kMaxDevices];
     const int dev = device_slot();
@@ -233,14 +234,14 @@ int launch_shape(const Maps& maps, Params& p, int tiles, int sms, cudaStream_t s
         done[dev] = true;
     }
     const int most = sms / PAIR;
-    tile_kernel<PAIR, BN, MODE><<<unsigned(tiles < most ? tiles : most) * PAIR, THREADS, smem, st>>>(maps, p);
+    if (!ds::launch(tile_kernel<PAIR, BN, MODE>, dim3(unsigned(tiles < most ? tiles : most) * PAIR), dim3(0), THREADS, smem, st, follows, maps, p)) return DS_ERR_CUDA;
     note_launch();
-    return cudaGetLastError() == cudaSuccess ? DS_OK : DS_ERR_CUDA;
+    return DS_OK;
 }
 
 // Launches the first `products` of p in tiles of a shape (SHAPES).
 template <int MODE>
-int launch(const Maps& maps, Params p, int products, int shape, cudaStream_t st)
+int launch_tiles(const Maps& maps, Params p, int products, int shape, bool follows, cudaStream_t st)
 {
     const int sms = multiprocessors();
     p.err_flag = kernel_error_flag();
@@ -254,9 +255,9 @@ int launch(const Maps& maps, Params p, int products, int shape, cudaStream_t st)
         tiles += (long long)q.tiles_m * q.tiles_n * q.splits;
     }
     if (tiles > INT_MAX) return DS_ERR_RANGE;
-    if (shape == 0) return launch_shape<2, 256, MODE>(maps, p, int(tiles), sms, st);
-    if (shape == 1) return launch_shape<1, 256, MODE>(maps, p, int(tiles), sms, st);
-    return launch_shape<1, 128, MODE>(maps, p, int(tiles), sms, st);
+    if (shape == 0) return launch_shape<2, 256, MODE>(maps, p, int(tiles), sms, follows, st);
+    if (shape == 1) return launch_shape<1, 256, MODE>(maps, p, int(tiles), sms, follows, st);
+    return launch_shape<1, 128, MODE>(maps, p, int(tiles), sms, follows, st);
 }
 
 // ---- layout of a call's scratch ----
@@ -385,9 +386,10 @@ extern "C" int ds_loss_forward(const ds_loss_t* a, void* stream)
         p.at_target = reinterpret_cast<float*>(scratch + l.at_target);
         p.ticket = reinterpret_cast<int*>(scratch + l.ticket);
         const int shape = tile_shape(&q, 1, multiprocessors());
-        if (const int e = launch<STATS>(maps, p, 1, shape, st)) return e;
-        rows_kernel<<<(a->rows + 31) / 32, 32 * ROW_WARPS, 0, st>>>(p.partial, (a->v + SHAPES[shape].bn - 1) / SHAPES[shape].bn * 2, p.at_target, p.target, a->ignore_index,
-                                                         a->rows, a->v, a->lse, a->each, a->reduction, p.ticket, a->loss, a->count);
+        if (const int e = launch_tiles<STATS>(maps, p, 1, shape, false, st)) return e;
+        if (!ds::launch(rows_kernel, dim3((a->rows + 31) / 32), dim3(0), 32 * ROW_WARPS, 0, st, true, p.partial, (a->v + SHAPES[shape].bn - 1) / SHAPES[shape].bn * 2,
+                        p.at_target, p.target, a->ignore_index, a->rows, a->v, a->lse, a->each, a->reduction, p.ticket, a->loss, a->count))
+            return DS_ERR_CUDA;
         ds::note_launch();
     } else if (a->reduction != DS_LOSS_NONE) {
         no_rows_kernel<<<1, 1, 0, st>>>(a->reduction, a->loss, a->count);
@@ -450,7 +452,7 @@ extern "C" int ds_loss_backward(const ds_loss_t* a, void* stream)
         p.product[0] = z;
         p.n_first = first;
         p.g = g, p.ldg = ldg;
-        if (const int e = launch<GRAD>(maps, p, 1, tile_shape(&z, 1, sms), st)) return e;
+        if (const int e = launch_tiles<GRAD>(maps, p, 1, tile_shape(&z, 1, sms), first > 0, st)) return e;
         int n = 0;
         if (a->dhidden) {   // dH (+)= G W
             Product& q = p.product[n] = {};
@@ -473,7 +475,7 @@ extern "C" int ds_loss_backward(const ds_loss_t* a, void* stream)
         }
         if (n == 1) p.product[1] = {};
         if (n)
-            if (const int e = launch<PRODUCT>(maps, p, n, tile_shape(p.product, n, sms), st)) return e;
+            if (const int e = launch_tiles<PRODUCT>(maps, p, n, tile_shape(p.product, n, sms), true, st)) return e;
     }
     if (a->dhidden && l.parts > 1) {
         const long long n = (long long)a->rows * a->d, blocks = (n + 511) / 512;

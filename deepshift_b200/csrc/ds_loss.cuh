@@ -20,6 +20,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "ds_follow.cuh"
 #include "ds_tc_ptx.cuh"
 
 namespace ds {
@@ -386,6 +387,8 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(PAIR, 1, 1)
     if (PAIR == 2) cluster_sync();
     tc_fence_after();
     const unsigned tmem = s.tmem;
+    let_follow();
+    wait_before();
     int total = p.product[0].tiles_m * p.product[0].tiles_n * p.product[0].splits;
     if (MODE == PRODUCT) total += p.product[1].tiles_m * p.product[1].tiles_n * p.product[1].splits;
     const int mine = blockIdx.x / PAIR, step = gridDim.x / PAIR;

@@ -3,7 +3,8 @@
 // it touches memory that a kernel writes or that it writes itself.  Only kernels of the same call follow one another this way: the first waits for
 // all earlier work as usual, so what was there before the call (operands, plans) may be read ahead of wait_before.
 // A kernel that takes tensor memory calls let_follow behind its allocation: a follower that held it could otherwise keep it waiting.
-// Worth 2 to 4 us a launch: what it takes to start a grid once the last one has drained.
+// Worth up to 3 us a launch, what it takes to start a grid once the last one has drained: the six launches of adapters on 4096 x 4096 of rank 32, forward
+// and backward, take 207 us instead of 221, a loss of 16 x 512 -> 1000 17.5 instead of 18.6.
 #pragma once
 #include <cuda_runtime.h>
 
